@@ -28,13 +28,16 @@ SOURCES = {
     "conv_wgrad.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "groupnorm.hip": [],
     "transformer.hip": [],
+    "block_norm.hip": [],
+    "adapters.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "newton_schulz.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "adam.hip": [],
     "bvh.hip": [],
     "mc_shade.hip": [],
     "host.cpp": [],
 }
 # the net kernels are compiled a second time with -DDM_F16 (dm_elem.h): IEEE-half instantiations, exported with f16 in their names
-F16_SOURCES = ["conv.hip", "conv_small.hip", "groupnorm.hip", "transformer.hip", "attention.hip", "attn_w64.hip", "attn_w128.hip"]
+F16_SOURCES = ["conv.hip", "conv_small.hip", "groupnorm.hip", "transformer.hip", "attention.hip", "attn_w64.hip", "attn_w128.hip", "adapters.hip"]
 HEADERS = ["dm_common.h", "dm_elem.h", "attn_common.h", "raster_core.h", "shade_core.h", "bvh_core.h", "grid_core.h", "mc_shade_core.h"]
 
 

@@ -519,6 +519,74 @@ int dm_attention_fwd_fp8(const void* q, const void* k, const void* vt, void* out
 int dm_adam_step(float* param, float* grad, float* exp_avg, float* exp_avg_sq, long long n, int step, float lr,
                  float beta1, float beta2, float eps, float grad_scale, int zero_grad, dm_stream_t stream);
 
+/* ---- fine-tuning ------------------------------------------------------------------------- */
+/* Norms before and after a transformer block fused with its gate and residual scale (csrc/block_norm.hip):
+ *   y = x + scale * gate * N_post(h),   z = N_pre(y)
+ * x, h, y, z [rows, C] contiguous, C <= 8192; gate NULL, [C] (item_rows = 0) or [rows / item_rows, C]; post / pre != 0: that norm is
+ * there, with gamma (NULL = 1) and beta (NULL = 0) [C]; rms != 0: RMS norms, else LayerNorm (eps inside the root).  stats fp32
+ * [rows, 4], 16-byte aligned, or NULL: what the backward needs.  The backward returns the wanted gradients (NULL = not wanted): dx, dh
+ * [rows, C], dgate as the gate, the norms' parameters [C]; dy may be NULL (zero), dz is needed with pre.  ws fp32,
+ * dm_gated_add_norm_workspace_floats(rows, item_rows, C) words.  At most 65000 items. */
+size_t dm_gated_add_norm_workspace_floats(long long rows, long long item_rows, int C);
+int dm_gated_add_norm_fwd_bf16(const void* x, const void* h, const void* gate, long long item_rows, int post, const void* post_g, const void* post_b,
+                              int pre, const void* pre_g, const void* pre_b, void* y, void* z, float* stats, long long rows, int C, float scale,
+                              float eps, int rms, dm_stream_t stream);
+int dm_gated_add_norm_bwd_bf16(const void* x, const void* h, const void* gate, long long item_rows, int post, const void* post_g, const void* post_b,
+                              int pre, const void* pre_g, const void* dy, const void* dz, const float* stats, void* dx, void* dh, void* dgate,
+                              void* dpost_g, void* dpost_b, void* dpre_g, void* dpre_b, float* ws, size_t ws_floats, long long rows, int C,
+                              float scale, float eps, int rms, dm_stream_t stream);
+int dm_gated_add_norm_fwd_f16(const void* x, const void* h, const void* gate, long long item_rows, int post, const void* post_g, const void* post_b,
+                              int pre, const void* pre_g, const void* pre_b, void* y, void* z, float* stats, long long rows, int C, float scale,
+                              float eps, int rms, dm_stream_t stream);
+int dm_gated_add_norm_bwd_f16(const void* x, const void* h, const void* gate, long long item_rows, int post, const void* post_g, const void* post_b,
+                              int pre, const void* pre_g, const void* dy, const void* dz, const float* stats, void* dx, void* dh, void* dgate,
+                              void* dpost_g, void* dpost_b, void* dpre_g, void* dpre_b, float* ws, size_t ws_floats, long long rows, int C,
+                              float scale, float eps, int rms, dm_stream_t stream);
+int dm_gated_add_norm_fwd_f32(const void* x, const void* h, const void* gate, long long item_rows, int post, const void* post_g, const void* post_b,
+                              int pre, const void* pre_g, const void* pre_b, void* y, void* z, float* stats, long long rows, int C, float scale,
+                              float eps, int rms, dm_stream_t stream);
+int dm_gated_add_norm_bwd_f32(const void* x, const void* h, const void* gate, long long item_rows, int post, const void* post_g, const void* post_b,
+                              int pre, const void* pre_g, const void* dy, const void* dz, const float* stats, void* dx, void* dh, void* dgate,
+                              void* dpost_g, void* dpost_b, void* dpre_g, void* dpre_b, float* ws, size_t ws_floats, long long rows, int C,
+                              float scale, float eps, int rms, dm_stream_t stream);
+
+/* Low-rank adapters of many requests beside a frozen projection (csrc/adapters.hip); the _f16 forms take IEEE half.
+ *   y = x w^T + bias + scale (x A_e^T) B_e^T + residual,   e = ids[request of the row]
+ * x [M, K], w [N, K], bias [N] / residual [M, N] or NULL, lora_a [E, R, K], lora_b [E, N] rows of R <= 128 elements ldb apart; ids int32 [n];
+ * offsets int32 [n + 1], ascending, or NULL (n requests of M / n rows).  Rows of no request and ids outside [0, E) have no adapter.
+ * K, N, ldb multiples of 8, pointers 16-byte aligned.  u: scratch of dm_adapter_u_bytes(M, R); keep_u != 0 leaves scale x A^T in it for
+ * dm_adapter_wgrad_* (and y = NULL computes only that). */
+size_t dm_adapter_u_bytes(long long M, int R);
+int dm_linear_adapted_bf16(const void* x, const void* w, const void* bias, const void* residual, const void* lora_a, const void* lora_b, int ldb,
+                           const int32_t* ids, const int32_t* offsets, long long n, float scale, void* u, size_t u_bytes, void* y, long long M, int K,
+                           int N, int R, int E, int keep_u, dm_stream_t stream);
+int dm_linear_adapted_f16(const void* x, const void* w, const void* bias, const void* residual, const void* lora_a, const void* lora_b, int ldb,
+                          const int32_t* ids, const int32_t* offsets, long long n, float scale, void* u, size_t u_bytes, void* y, long long M, int K,
+                          int N, int R, int E, int keep_u, dm_stream_t stream);
+/* layouts of the adapters: mode 0 copies src [E, C, R] to rows padded to 16 | 32 | 64 | 128 ranks (zeros), mode 1 the same from src [E, R, C],
+ * mode 2 transposes src [E, C, R] to [E, R, C] */
+int dm_adapter_layout_bf16(const void* src, void* dst, int E, int C, int R, int mode, dm_stream_t stream);
+int dm_adapter_layout_f16(const void* src, void* dst, int E, int C, int R, int mode, dm_stream_t stream);
+/* weight gradients: out[e] = sum over the rows of adapter e of u^T X ([E, R, C], or [E, C, R] with transpose); plan = the rows in adapter order,
+ * dm_adapter_plan_words int32, built by dm_adapter_plan for items of `chunk` rows (a multiple of 64); part fp32
+ * [dm_adapter_plan_items][padded rank][C] */
+size_t dm_adapter_plan_words(long long M, long long n, int E);
+long long dm_adapter_plan_items(long long M, int E, int chunk);
+int dm_adapter_plan(const int32_t* ids, const int32_t* offsets, long long n, long long M, int E, int chunk, int32_t* plan, dm_stream_t stream);
+int dm_adapter_wgrad_bf16(const void* X, const void* u, const int32_t* plan, long long n, long long M, int C, int R, int E, int chunk, int transpose,
+                          float* part, size_t part_floats, void* out, dm_stream_t stream);
+int dm_adapter_wgrad_f16(const void* X, const void* u, const int32_t* plan, long long n, long long M, int C, int R, int E, int chunk, int transpose,
+                         float* part, size_t part_floats, void* out, dm_stream_t stream);
+
+/* Orthogonalised updates by Newton-Schulz products (csrc/newton_schulz.hip).  `count` matrices [rows, cols], contiguous, behind HOST arrays
+ * of device pointers; dtype of g and out: 0 bf16 | 1 half | 2 fp32.  dm_muon_step (mom, p fp32): mom <- mu mom + g; u = g + mu mom (nesterov)
+ * or mom; p <- p decay - step orth(u).  ws: 256-byte aligned, dm_orthogonalize_workspace_bytes (less, down to one matrix's: more launches). */
+size_t dm_orthogonalize_workspace_bytes(int count, int rows, int cols);
+int dm_orthogonalize(const void* const* g_host, void* const* out_host, int count, int rows, int cols, int dtype, int steps, float eps, void* ws,
+                     size_t ws_bytes, dm_stream_t stream);
+int dm_muon_step(const void* const* g_host, float* const* mom_host, float* const* p_host, int count, int rows, int cols, int dtype, int steps,
+                 float mu, int nesterov, float eps, float decay, float step, void* ws, size_t ws_bytes, dm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

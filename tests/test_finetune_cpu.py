@@ -1,0 +1,165 @@
+"""Refusals of the fine-tuning operators (CPU: every check comes before the first launch) and the size queries of their C entries."""
+import pytest
+import torch
+
+from dreammat_amd import _lib, hipops
+
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
+
+
+def adapter(**kw):
+    v = dict(x=torch.zeros(4, 6, 64, dtype=BF), w=torch.zeros(72, 64, dtype=BF), bias=torch.zeros(72, dtype=BF), lora_a=torch.zeros(3, 16, 64, dtype=BF),
+             lora_b=torch.zeros(3, 72, 16, dtype=BF), ids=torch.zeros(4, dtype=torch.int32))
+    v.update(kw)
+    return v
+
+
+BAD_ADAPTER = [
+    (TypeError, dict(x=torch.zeros(4, 6, 64))),
+    (TypeError, dict(w=torch.zeros(72, 64, dtype=HF))),
+    (TypeError, dict(bias=torch.zeros(72))),
+    (TypeError, dict(residual=torch.zeros(4, 6, 72, dtype=HF))),
+    (ValueError, dict(x=torch.zeros(4, 6, 32, dtype=BF))),
+    (ValueError, dict(w=torch.zeros(72 * 64, dtype=BF))),
+    (ValueError, dict(lora_b=torch.zeros(3, 72, 8, dtype=BF))),
+    (ValueError, dict(lora_b=torch.zeros(2, 72, 16, dtype=BF))),
+    (ValueError, dict(lora_a=torch.zeros(3, 129, 64, dtype=BF), lora_b=torch.zeros(3, 72, 129, dtype=BF))),
+    (ValueError, dict(lora_a=torch.zeros(3, 0, 64, dtype=BF), lora_b=torch.zeros(3, 72, 0, dtype=BF))),
+    (ValueError, dict(lora_a=torch.zeros(0, 16, 64, dtype=BF), lora_b=torch.zeros(0, 72, 16, dtype=BF))),
+    (ValueError, dict(w=torch.zeros(70, 64, dtype=BF), bias=None, lora_b=torch.zeros(3, 70, 16, dtype=BF))),
+    (ValueError, dict(bias=torch.zeros(64, dtype=BF))),
+    (ValueError, dict(ids=torch.zeros(4, dtype=torch.int64))),
+    (ValueError, dict(ids=torch.zeros(0, dtype=torch.int32))),
+    (ValueError, dict(ids=torch.zeros(2, 2, dtype=torch.int32))),
+    (ValueError, dict(ids=torch.zeros(5, dtype=torch.int32))),                       # 24 rows are not 5 equal requests
+    (ValueError, dict(offsets=torch.zeros(4, dtype=torch.int32))),
+    (ValueError, dict(offsets=torch.zeros(5, dtype=torch.int64))),
+    (ValueError, dict(residual=torch.zeros(24, 72, dtype=BF))),
+    (_lib.DmError, dict()),                                                          # all right, but on the CPU
+]
+
+
+@pytest.mark.parametrize("case", range(len(BAD_ADAPTER)))
+def test_linear_adapted_refuses(case):
+    error, change = BAD_ADAPTER[case]
+    v = adapter(**change)
+    with pytest.raises(error):
+        hipops.linear_adapted(**v)
+    if v["w"].dim() == 2:
+        with pytest.raises(error):
+            hipops.linear_adapted_autograd(w_t=v["w"].t().contiguous(), **v)
+
+
+def test_linear_adapted_autograd_refuses_a_trainable_projection_and_a_foreign_transpose():
+    v = adapter()
+    with pytest.raises(ValueError):
+        hipops.linear_adapted_autograd(w_t=v["w"], **v)
+    with pytest.raises(ValueError):
+        hipops.linear_adapted_autograd(w_t=v["w"].t().contiguous(), **adapter(w=torch.zeros(72, 64, dtype=BF, requires_grad=True)))
+    with pytest.raises(ValueError):
+        hipops.linear_adapted_autograd(w_t=v["w"].t().contiguous(), **adapter(bias=torch.zeros(72, dtype=BF, requires_grad=True)))
+
+
+ONE = torch.ones(64)
+BAD_NORM = [
+    (TypeError, dict(x=torch.zeros(3, 64, dtype=torch.float64), h=torch.zeros(3, 64, dtype=torch.float64))),
+    (TypeError, dict(h=torch.zeros(2, 3, 64, dtype=BF))),
+    (TypeError, dict(post=(ONE.to(BF), None))),
+    (TypeError, dict(gate=ONE.to(HF))),
+    (ValueError, dict(h=torch.zeros(2, 4, 64))),
+    (ValueError, dict(kind="batch")),
+    (ValueError, dict(gate=torch.ones(3, 64))),
+    (ValueError, dict(gate=torch.ones(2, 1, 64))),
+    (ValueError, dict(gate=torch.ones(32))),
+    (ValueError, dict(post=ONE)),
+    (ValueError, dict(pre=(ONE, torch.ones(32)))),
+    (ValueError, dict(pre=(ONE, ONE, ONE))),
+    (ValueError, dict(x=torch.zeros(2, 8193), h=torch.zeros(2, 8193))),
+    (ValueError, dict(x=torch.zeros(2, 0), h=torch.zeros(2, 0))),
+    (ValueError, dict(x=torch.zeros(65001, 1), h=torch.zeros(65001, 1), gate=torch.zeros(65001, 1))),
+    (_lib.DmError, dict()),
+]
+
+
+@pytest.mark.parametrize("case", range(len(BAD_NORM)))
+def test_gated_add_norm_refuses(case):
+    error, change = BAD_NORM[case]
+    v = dict(x=torch.zeros(2, 3, 64), h=torch.zeros(2, 3, 64))
+    v.update(change)
+    with pytest.raises(error):
+        hipops.gated_add_norm(**v)
+
+
+def test_orthogonalize_refuses():
+    for error, g, kw in [(ValueError, torch.zeros(4), {}), (ValueError, torch.zeros(4, 4, dtype=torch.float64), {}), (ValueError, torch.zeros(4, 4), dict(steps=0)),
+                         (ValueError, torch.zeros(4, 4), dict(steps=65)), (ValueError, torch.empty(1, 1, device="meta").expand(40000, 40000), {}),
+                         (_lib.DmError, torch.zeros(4, 4), {})]:
+        with pytest.raises(error):
+            hipops.orthogonalize(g, **kw)
+
+
+def test_muon_step_refuses():
+    z = lambda *s, **k: torch.zeros(*s, **k)
+    p, g, m = z(4, 6), z(4, 6), z(4, 6)
+    for error, args, kw in [
+            (ValueError, ([p], [g, g], [m]), {}), (ValueError, ([z(4)], [z(4)], [z(4)]), {}), (TypeError, ([p.to(BF)], [g], [m]), {}),
+            (TypeError, ([p], [g], [m.to(BF)]), {}), (TypeError, ([p], [g.double()], [m]), {}), (ValueError, ([p], [z(6, 4)], [m]), {}),
+            (ValueError, ([p], [g], [z(4, 7)]), {}), (ValueError, ([z(6, 4).t()], [g], [m]), {}), (ValueError, ([p, p], [g, g], [m, z(4, 6)]), {}),
+            (ValueError, ([p], [g], [p]), {}), (ValueError, ([p], [g], [m]), dict(steps=0)), (ValueError, ([p], [g], [m]), dict(scale="none")),
+            (_lib.DmError, ([p], [g], [m]), {})]:
+        with pytest.raises(error):
+            hipops.muon_step(*args, lr=0.1, **kw)
+    assert not p.any() and not m.any()
+    hipops.muon_step([], [], [], lr=0.1)                                              # nothing to do
+
+
+def test_c_entries_refuse_before_any_launch():
+    L = _lib.lib()
+    ARG, WS, UNS = -1, -2, -3
+    P = 1 << 12                                                                       # an aligned address that no check dereferences
+
+    def lin(x=P, ldb=16, ids=P, offsets=None, n=2, u=P, ub=1 << 20, y=P, M=4, K=64, N=64, R=16, E=1, keep=0, w=P, b=P):
+        return L.dm_linear_adapted_bf16(x, w, None, None, P, b, ldb, ids, offsets, n, 1.0, u, ub, y, M, K, N, R, E, keep, None)
+    for kw, rc in [(dict(x=None), ARG), (dict(ids=None), ARG), (dict(n=0), ARG), (dict(n=3), ARG), (dict(E=0), ARG), (dict(R=0), ARG), (dict(K=0), ARG),
+                   (dict(w=None), ARG), (dict(b=None), ARG), (dict(y=None), ARG), (dict(u=None), ARG), (dict(x=P + 2), ARG), (dict(ldb=8), ARG), (dict(M=-4), ARG),
+                   (dict(R=129, ldb=136), UNS), (dict(K=60), UNS), (dict(N=60), UNS), (dict(ldb=20), UNS), (dict(ub=16), WS)]:
+        assert lin(**kw) == rc, kw
+    assert lin(M=0) == 0
+
+    def wg(X=P, chunk=128, part=1 << 20, M=4, C=64, R=16, E=1):
+        return L.dm_adapter_wgrad_f16(X, P, P, 2, M, C, R, E, chunk, 0, P, part, P, None)
+    for kw, rc in [(dict(X=None), ARG), (dict(X=P + 2), ARG), (dict(chunk=100), ARG), (dict(M=0), ARG), (dict(C=60), UNS), (dict(R=200), UNS), (dict(part=10), WS)]:
+        assert wg(**kw) == rc, kw
+    assert L.dm_adapter_plan(P, None, 2, 4, 1, 100, P, None) == ARG and L.dm_adapter_plan(P, None, 3, 4, 1, 128, P, None) == ARG
+    assert L.dm_adapter_layout_bf16(P, P, 1, 8, 8, 3, None) == ARG and L.dm_adapter_layout_bf16(P, P, 1, 8, 129, 0, None) == UNS
+
+    def norm(x=P, rows=6, items=0, C=64, gate=None, pre=0, z=None, stats=None):
+        return L.dm_gated_add_norm_fwd_f32(x, P, gate, items, 0, None, None, pre, None, None, P, z, stats, rows, C, 1.0, 1e-5, 0, None)
+    for kw, rc in [(dict(x=None), ARG), (dict(rows=-1), ARG), (dict(C=0), ARG), (dict(C=8193), UNS), (dict(pre=1), ARG), (dict(stats=P + 4), ARG),
+                   (dict(gate=P, items=4), ARG)]:
+        assert norm(**kw) == rc, kw
+    assert norm(rows=0) == 0
+    bwd = lambda ws, words, **k: L.dm_gated_add_norm_bwd_bf16(P, P, P, 2, 1, P, P, 0, None, P, None, P, P, P, P, P, P, None, None, ws, words, 6, 64, 1.0, 1e-5, 0, None)
+    assert bwd(None, 0) == WS and bwd(P, 100) == WS
+
+    import ctypes
+    ptrs = (ctypes.c_void_p * 1)(P)
+    null = (ctypes.c_void_p * 1)(None)
+    need = L.dm_orthogonalize_workspace_bytes(1, 8, 8)
+    ns = lambda g=ptrs, o=ptrs, count=1, rows=8, cols=8, dt=0, steps=5, ws=P, wb=need: L.dm_orthogonalize(g, o, count, rows, cols, dt, steps, 1e-7, ws, wb, None)
+    for kw, rc in [(dict(g=None), ARG), (dict(g=null), ARG), (dict(o=null), ARG), (dict(count=-1), ARG), (dict(rows=0), ARG), (dict(dt=3), ARG), (dict(steps=0), ARG),
+                   (dict(ws=P + 16), ARG), (dict(ws=None), ARG), (dict(wb=need - 1), WS), (dict(rows=40000, cols=40000), UNS)]:
+        assert ns(**kw) == rc, kw
+    assert ns(count=0) == 0
+    assert L.dm_muon_step(ptrs, null, ptrs, 1, 8, 8, 2, 5, 0.9, 1, 1e-7, 1.0, 0.1, P, need, None) == ARG
+
+
+def test_size_queries():
+    L = _lib.lib()
+    assert [L.dm_adapter_u_bytes(10, r) for r in (1, 16, 17, 33, 128)] == [10 * (4 * p + 4) for p in (16, 16, 32, 64, 128)]
+    assert L.dm_adapter_u_bytes(0, 4) == L.dm_adapter_u_bytes(4, 129) == 0
+    # every adapter may end inside an item: full items and one more each, but never more items than rows
+    assert L.dm_adapter_plan_items(1000, 3, 128) == 7 + 3 and L.dm_adapter_plan_items(2, 9, 128) == 2
+    assert L.dm_adapter_plan_words(100, 7, 3) == 2 * 4 + 7 + 100
+    assert L.dm_orthogonalize_workspace_bytes(40, 65, 10) == 16 * L.dm_orthogonalize_workspace_bytes(1, 65, 10)
+    assert L.dm_gated_add_norm_workspace_floats(0, 0, 8) == 0 and L.dm_gated_add_norm_workspace_floats(6, 2, 8) == (5 + 3) * 8

@@ -695,9 +695,9 @@ __global__ __launch_bounds__(NW * 64) void k_conv3x3_dma(ConvArgs a, long long n
             // The gate function is the exact (erf) GELU evaluated as value * gate * Phi(gate) with
             //   Phi(g) = g < 0 ? h : 1 - h,   h = erfc(|g| / sqrt 2) / 2 = poly5(t) 2^(-z^2),  t = 1 / (1 + p |z|),  z = g sqrt(log2(e) / 2)
             // (Abramowitz-Stegun 7.1.26, coefficients halved; |error| of Phi < 3e-7, the negative tail without the cancellation
-            // of 1 + erf), two elements per instruction on the packed fp32 pipe: 17 VALU instructions per PAIR of outputs
-            // where 0.5 g (1 + erff(g / sqrt 2)) took ~44 per ELEMENT, divergent branches included.  At K = 320 this epilogue was
-            // 70 % of a tile (2834 VALU instructions per wave against 5 K-steps of 32 MFMAs; round 5).
+            // of 1 + erf), two elements side by side, where 0.5 g (1 + erff(g / sqrt 2)) took ~44 VALU instructions per element,
+            // divergent branches included.  At K = 320 that epilogue was 70 % of a tile (2834 VALU instructions per wave against 5
+            // K-steps of 32 MFMAs).  (The library is built without packed fp32 instructions, csrc/build.py.)
             static_assert(EPI != 1 || NT % 2 == 0, "GEGLU needs value/gate fragment pairs");
             const f32x2 kKz = {0.84932180028801905f, 0.84932180028801905f};          // sqrt(log2(e) / 2)
             const f32x2 kKp = {0.27273748f, 0.27273748f};                              // 0.3275911 / sqrt(log2 e)

@@ -5,7 +5,7 @@ set -u
 R=${GRAFT_REPO_ROOT:-$(cd "$(dirname "$0")/.." && pwd)}
 cd $R
 C=dreammat_amd/csrc
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -munsafe-fp-atomics -c $C/shade.hip -o /tmp/shade_nofast.o || exit 1
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Xclang -target-feature -Xclang -packed-fp32-ops -munsafe-fp-atomics -c $C/shade.hip -o /tmp/shade_nofast.o || exit 1
 objs=$(ls $C/_obj/*.o | grep -v "/shade.hip.o")
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o /tmp/libdm_nofast.so $objs /tmp/shade_nofast.o || exit 1
 python tools/grad_budget.py fastmath

@@ -25,6 +25,7 @@ import numpy as np
 import torch
 import torch.nn.functional as F
 
+from . import hipops
 from .sd import ControlNetModel, DDIMScheduler
 from .sd.layers import PaddedContext
 
@@ -82,6 +83,50 @@ def controlnet_training_loss(vae, unet, controlnet, scheduler, pixel_values, con
     return F.mse_loss(pred.float(), noise.float(), reduction="mean")
 
 
+class MuonAdamW:
+    """Orthogonalised momentum steps (hipops.muon_step: the matrices of one shape share their launches) for every parameter that is a matrix --
+    Linear weights, convolution weights as [Cout, Cin kh kw] -- and AdamW for the others (biases, norms).  The "rms" scale of the orthogonalised
+    step is AdamW's update size, so both halves share one learning rate and one weight decay.  GPU only: the products have no CPU form."""
+
+    def __init__(self, params, lr, weight_decay=1e-2, momentum=0.95):
+        params = list(params)
+        self.lr, self.weight_decay, self.momentum = lr, weight_decay, momentum
+        self.matrices = [p for p in params if p.dim() >= 2]
+        rest = [p for p in params if p.dim() < 2]
+        self.adamw = torch.optim.AdamW(rest, lr=lr, weight_decay=weight_decay) if rest else None
+        self.momenta = [None] * len(self.matrices)
+
+    def step(self):
+        live = [i for i, p in enumerate(self.matrices) if p.grad is not None]
+        for i in live:
+            if self.momenta[i] is None:
+                self.momenta[i] = torch.zeros_like(self.matrices[i], memory_format=torch.contiguous_format)
+        hipops.muon_step([self.matrices[i].detach() for i in live], [self.matrices[i].grad for i in live], [self.momenta[i] for i in live], lr=self.lr,
+                         momentum=self.momentum, weight_decay=self.weight_decay, scale="rms")
+        if self.adamw is not None:
+            self.adamw.step()
+
+    def zero_grad(self, set_to_none=True):
+        for p in self.matrices:
+            if set_to_none:
+                p.grad = None
+            elif p.grad is not None:
+                p.grad.zero_()
+        if self.adamw is not None:
+            self.adamw.zero_grad(set_to_none=set_to_none)
+
+    def state_dict(self):
+        return {"momenta": self.momenta, "adamw": self.adamw.state_dict() if self.adamw is not None else None}
+
+    def load_state_dict(self, state):
+        if len(state["momenta"]) != len(self.matrices) or (state["adamw"] is None) != (self.adamw is None):
+            raise ValueError("MuonAdamW: the state belongs to other parameters")
+        self.momenta = [None if m is None else m.to(p.device, torch.float32).reshape(p.shape).clone(memory_format=torch.contiguous_format)
+                        for m, p in zip(state["momenta"], self.matrices)]
+        if self.adamw is not None:
+            self.adamw.load_state_dict(state["adamw"])
+
+
 class ControlNetTrainer:
     """AdamW(lr 1e-5 by default in the reference's train.sh) over the ControlNet parameters only; gradient clipping at
     max_grad_norm (:899-902).
@@ -90,9 +135,13 @@ class ControlNetTrainer:
     training kernels need bf16 weights), the optimizer runs on fp32 MASTER copies of its parameters -- pure bf16 parameters
     under AdamW at lr 1e-5 lose most updates to rounding (a bf16 ulp at |w| = 0.02 is 1.2e-4).  The masters are created the
     first time gradients are applied, from whatever dtype the module has then (so `trainer.controlnet.bfloat16()` after
-    construction works); the state dict is the masters' values."""
+    construction works); the state dict is the masters' values.  optimizer="muon" (an addition; AdamW is the reference's): orthogonalised steps
+    for the matrices, see MuonAdamW."""
 
-    def __init__(self, vae, unet, controlnet=None, lr=1e-5, weight_decay=1e-2, max_grad_norm=1.0, compute_dtype=None):
+    def __init__(self, vae, unet, controlnet=None, lr=1e-5, weight_decay=1e-2, max_grad_norm=1.0, compute_dtype=None, optimizer="adamw"):
+        if optimizer not in ("adamw", "muon"):
+            raise ValueError(f"ControlNetTrainer: optimizer is 'adamw' or 'muon', not {optimizer!r}")
+        self.optimizer = optimizer
         freeze(vae, unet)
         self.vae, self.unet = vae, unet
         self.controlnet = controlnet if controlnet is not None else init_controlnet(unet)
@@ -113,11 +162,13 @@ class ControlNetTrainer:
         self._opt_dtype = params[0].dtype
         self._opt_device = params[0].device
         if any(p.dtype != torch.float32 for p in params):
-            self.master = [p.detach().float().clone().requires_grad_() for p in params]
+            self.master = [p.detach().float().clone(memory_format=torch.contiguous_format if self.optimizer == "muon" else torch.preserve_format)
+                           .requires_grad_() for p in params]
             target = self.master
         else:
             self.master, target = None, params
-        self.opt = torch.optim.AdamW(target, lr=self.lr, weight_decay=self.weight_decay)
+        make = MuonAdamW if self.optimizer == "muon" else torch.optim.AdamW
+        self.opt = make(target, lr=self.lr, weight_decay=self.weight_decay)
 
     def apply_gradients(self, world=1):
         """all-reduce (ONE flat collective) -> clip -> AdamW on the fp32 masters -> cast back; called after loss.backward()."""
@@ -300,6 +351,7 @@ def main(argv=None):
     ap.add_argument("--resolution", type=int, default=512)
     ap.add_argument("--train_batch_size", type=int, default=4)
     ap.add_argument("--learning_rate", type=float, default=1e-5)
+    ap.add_argument("--optimizer", choices=("adamw", "muon"), default="adamw")
     ap.add_argument("--max_train_steps", type=int, default=1000)
     ap.add_argument("--checkpointing_steps", type=int, default=500)
     ap.add_argument("--use_cfg", action="store_true")
@@ -321,7 +373,7 @@ def main(argv=None):
     dt = torch.bfloat16 if dev.type == "cuda" else torch.float32
     vae.to(dev, dt); unet.to(dev, dt)
     cn = init_controlnet(unet).to(dev, dt)            # the compute dtype of the frozen nets; fp32 masters live in the trainer
-    tr = ControlNetTrainer(vae, unet, cn, lr=a.learning_rate)
+    tr = ControlNetTrainer(vae, unet, cn, lr=a.learning_rate, optimizer=a.optimizer)
     ds = ControlNetRenderDataset(a.train_data_dir, a.prompt_file, a.resolution, a.use_cfg)
     sampler = torch.utils.data.distributed.DistributedSampler(ds, world, rank, shuffle=True, seed=0) if world > 1 else None
     dl = torch.utils.data.DataLoader(ds, batch_size=a.train_batch_size, shuffle=sampler is None, sampler=sampler,

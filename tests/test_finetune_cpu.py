@@ -163,3 +163,22 @@ def test_size_queries():
     assert L.dm_adapter_plan_words(100, 7, 3) == 2 * 4 + 7 + 100
     assert L.dm_orthogonalize_workspace_bytes(40, 65, 10) == 16 * L.dm_orthogonalize_workspace_bytes(1, 65, 10)
     assert L.dm_gated_add_norm_workspace_floats(0, 0, 8) == 0 and L.dm_gated_add_norm_workspace_floats(6, 2, 8) == (5 + 3) * 8
+
+
+def test_trainer_optimizer_names_and_cpu():
+    from dreammat_amd import controlnet_train as ct
+    from dreammat_amd.sd import ARCHS, AutoencoderKLEncoder, UNet2DConditionModel
+    a = ARCHS["tiny"]
+    unet, vae = UNet2DConditionModel(a), AutoencoderKLEncoder(a)
+    with pytest.raises(ValueError):
+        ct.ControlNetTrainer(vae, unet, optimizer="sgd")
+    tr = ct.ControlNetTrainer(vae, unet, optimizer="muon")
+    assert len(tr.opt.matrices) + len(tr.opt.adamw.param_groups[0]["params"]) == len(tr._params())
+    tr.opt.matrices[0].grad = torch.ones_like(tr.opt.matrices[0])
+    with pytest.raises(_lib.DmError):                                                # no CPU form
+        tr.opt.step()
+    tr.opt.zero_grad()
+    assert tr.opt.matrices[0].grad is None
+    with pytest.raises(ValueError):
+        tr.opt.load_state_dict({"momenta": [], "adamw": None})
+    assert isinstance(ct.ControlNetTrainer(vae, unet).opt, torch.optim.AdamW)

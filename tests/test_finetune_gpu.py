@@ -570,3 +570,58 @@ def test_operators_on_a_side_stream():
         got, go = block(hipops, x2, w, wt, leaves, ids).detach(), hipops.orthogonalize(w)
     side.synchronize()
     assert torch.equal(got, want) and torch.equal(go, wo)
+
+
+def test_controlnet_trainer_with_orthogonalised_steps():
+    """ControlNetTrainer(optimizer="muon"): every matrix master moves by the formula's step (64 bits, from the gradient the trainer used), the others
+    by AdamW, the bf16 module holds the rounded masters, and the optimizer's state survives a round trip"""
+    from dreammat_amd import controlnet_train as ct
+    from dreammat_amd.sd import ARCHS, AutoencoderKLEncoder, UNet2DConditionModel
+    torch.manual_seed(0)
+    a = ARCHS["tiny"]
+    unet, vae = UNet2DConditionModel(a).to(DEV, BF), AutoencoderKLEncoder(a).to(DEV, BF)
+    tr = ct.ControlNetTrainer(vae, unet, ct.init_controlnet(unet).to(DEV, BF), lr=1e-3, weight_decay=0.01, max_grad_norm=1e9, optimizer="muon")
+    g = gen(60)
+    img, cond = rand(g, 2, 3, 64, 64, dtype=BF).clamp(-1, 1), torch.rand(2, 22, 64, 64, generator=g, device=DEV)
+    text = rand(g, 2, 77, a.cross_dim, dtype=BF)
+    for step in range(2):
+        loss = ct.controlnet_training_loss(tr.vae, tr.unet, tr.controlnet, tr.scheduler, img, cond, text, timesteps=torch.tensor([300, 700], device=DEV),
+                                           noise=rand(g, 2, 4, 8, 8), posterior_noise=rand(g, 2, 4, 8, 8))
+        loss.backward()
+        assert torch.isfinite(loss)
+        params = tr._params()
+        grads = [None if p.grad is None else p.grad.double() for p in params]
+        masters = [m.detach().double() for m in tr.master]
+        before = [None if m is None else m.double() for m in tr.opt.momenta]
+        tr.apply_gradients()
+        at = 0
+        for p, gr, old, new in zip(params, grads, masters, tr.master):
+            assert torch.equal(p, new.to(BF))
+            if p.dim() < 2:
+                continue
+            mom = before[at] if before[at] is not None else torch.zeros_like(gr)
+            at += 1
+            mom = 0.95 * mom + gr
+            u = (gr + 0.95 * mom).flatten(1)
+            up = 1e-3 * 0.2 * math.sqrt(max(u.shape)) * ns_formula(u).view(p.shape)
+            assert (tr.opt.momenta[at - 1].double() - mom).norm() <= 3 * 2.0 ** -24 * (mom.norm() + gr.norm())
+            if not gr.any():
+                assert not up.any()
+            # (the directions of a real gradient that lie 1e-4 below its norm are amplified in full: the bound of the file's head holds for them too)
+            assert (new.detach().double() - (old * (1 - 1e-5) - up)).norm() <= NS_TOL[FP] * up.norm() + 3 * 2.0 ** -24 * old.norm()
+    moved = [bool((m.detach() != o.float()).any()) for m, o in zip(tr.master, masters) if m.dim() < 2]
+    assert any(moved)
+    state = tr.opt.state_dict()
+    other = ct.MuonAdamW(tr.master, lr=1e-3)
+    other.load_state_dict(state)
+    assert all(torch.equal(p, q) for p, q in zip(other.momenta, tr.opt.momenta))
+
+
+def test_controlnet_launcher_with_orthogonalised_steps(tmp_path):
+    from dreammat_amd import controlnet_train as ct
+    from tests.test_nets_cpu import _tiny_render_tree
+    _tiny_render_tree(tmp_path / "data", tmp_path / "prompts.json")
+    tr = ct.main(["--synthetic", "--pretrained_model_name_or_path", "tiny", "--train_data_dir", str(tmp_path / "data"), "--prompt_file",
+                  str(tmp_path / "prompts.json"), "--resolution", "64", "--train_batch_size", "2", "--max_train_steps", "2", "--output_dir",
+                  str(tmp_path / "out"), "--checkpointing_steps", "2", "--optimizer", "muon"])
+    assert tr.global_step == 2 and isinstance(tr.opt, ct.MuonAdamW) and all(torch.isfinite(m).all() for m in tr.master)

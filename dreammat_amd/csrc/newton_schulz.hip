@@ -21,6 +21,7 @@
 #include <type_traits>
 
 #include "dm_common.h"
+#include "dm_elem.h"
 
 namespace {
 
@@ -31,7 +32,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 [[maybe_unused]] constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 [[maybe_unused]] constexpr float kScale = 8192.f, kInv = 1.f / 8192.f;        // 2^13, see above
 constexpr int kGroup = 16;                                   // matrices of one launch
-constexpr int kNormParts = 64;                               // partial sums of a squared norm
+constexpr int kNormParts = 512;                              // most partial sums of a squared norm
 
 // One group of same-shaped matrices [rows, cols] (row-major, contiguous)
 struct Mats {
@@ -47,7 +48,10 @@ struct NsArgs {
     int m, n;                // m <= n: the iteration's orientation
     int mp, np;              // padded to multiples of 64
     int flip;                // rows > cols
+    int whole;               // rows and pointers of the norm pass are whole 16-byte chunks
+    int parts;               // workgroups per matrix of the norm pass
     double* norm;            // [count][kNormParts]
+    float* part;             // partial sums of a split contraction
     _Float16* x;             // pairs [count][mp][np]
     _Float16* xt[2];         // pairs [count][np][mp], ping-pong
     _Float16* s;             // pairs [count][mp][mp]
@@ -73,17 +77,38 @@ __device__ __forceinline__ float direction(const NsArgs& a, int b, long long i) 
     return a.nesterov ? g + a.mu * m : m;
 }
 
-// momentum update and the squared norm of the direction: kNormParts workgroups per matrix, sums in 64 bits
+// momentum update and the squared norm of the direction: a.parts workgroups per matrix, four elements per thread, sums in 64 bits
 template <typename T>
 __global__ __launch_bounds__(256) void k_ns_norm(NsArgs a) {
     __shared__ double red[4];
     const int b = blockIdx.y;
     const long long total = (long long)a.rows * a.cols;
+    const T* g = reinterpret_cast<const T*>(a.t.g[b]);
+    float* mom = a.t.mom[b];
     double s = 0.0;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += 256 * kNormParts) {
-        if (a.t.mom[b]) a.t.mom[b][i] = a.mu * a.t.mom[b][i] + (float)reinterpret_cast<const T*>(a.t.g[b])[i];
-        const double u = (double)direction<T>(a, b, i);
-        s += u * u;
+    auto add = [&](float u) { s += (double)u * (double)u; };
+    if (a.whole) {
+        typedef T vec __attribute__((ext_vector_type(4)));
+        for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < total; i += 1024LL * a.parts) {
+            const vec gv = *reinterpret_cast<const vec*>(g + i);
+            if (mom) {
+                float4 m = *reinterpret_cast<const float4*>(mom + i);
+                m.x = a.mu * m.x + (float)gv[0]; m.y = a.mu * m.y + (float)gv[1]; m.z = a.mu * m.z + (float)gv[2]; m.w = a.mu * m.w + (float)gv[3];
+                *reinterpret_cast<float4*>(mom + i) = m;
+                add(a.nesterov ? (float)gv[0] + a.mu * m.x : m.x);
+                add(a.nesterov ? (float)gv[1] + a.mu * m.y : m.y);
+                add(a.nesterov ? (float)gv[2] + a.mu * m.z : m.z);
+                add(a.nesterov ? (float)gv[3] + a.mu * m.w : m.w);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) add((float)gv[k]);
+            }
+        }
+    } else {
+        for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += 256LL * a.parts) {
+            if (mom) mom[i] = a.mu * mom[i] + (float)g[i];
+            add(direction<T>(a, b, i));
+        }
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
@@ -96,58 +121,92 @@ __global__ __launch_bounds__(256) void k_ns_norm(NsArgs a) {
 template <typename T>
 __global__ __launch_bounds__(256) void k_ns_pack(NsArgs a) {
     __shared__ float tile[64][65];
+    __shared__ double red[4];
     const int b = blockIdx.z, i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;       // rows / columns of X
-    double sum = 0.0;
-    for (int k = 0; k < kNormParts; ++k) sum += a.norm[(long long)b * kNormParts + k];
-    const float inv = (float)((double)kScale / (sqrt(sum) + (double)a.eps));
     const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-    for (int r = ty; r < 64; r += 4) {
-        // read along the rows as given
-        const int i = a.flip ? i0 + tx : i0 + r, j = a.flip ? j0 + r : j0 + tx;
-        const bool ok = i < a.m && j < a.n;
-        const float v = ok ? direction<T>(a, b, a.flip ? (long long)j * a.cols + i : (long long)i * a.cols + j) * inv : 0.f;
-        if (a.flip) tile[tx][r] = v;
-        else tile[r][tx] = v;
+    float v[16];
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {                                              // read along the rows as given
+        const int r = ty + 4 * q, i = a.flip ? i0 + tx : i0 + r, j = a.flip ? j0 + r : j0 + tx;
+        v[q] = i < a.m && j < a.n ? direction<T>(a, b, a.flip ? (long long)j * a.cols + i : (long long)i * a.cols + j) : 0.f;
+    }
+    double s = 0.0;
+    for (int k = threadIdx.x; k < a.parts; k += 256) s += a.norm[(long long)b * kNormParts + k];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if (tx == 0) red[ty] = s;
+    __syncthreads();
+    const float inv = (float)((double)kScale / (sqrt(red[0] + red[1] + red[2] + red[3]) + (double)a.eps));
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+        const int r = ty + 4 * q;
+        if (a.flip) tile[tx][r] = v[q] * inv;
+        else tile[r][tx] = v[q] * inv;
     }
     __syncthreads();
     _Float16* x = a.x + (long long)b * a.mp * 2 * a.np;
     _Float16* xt = a.xt[0] + (long long)b * a.np * 2 * a.mp;
-    for (int r = ty; r < 64; r += 4) {
-        _Float16 hi, lo;
-        split(tile[r][tx], hi, lo);
-        const long long p = pair_at(i0 + r, j0 + tx, a.np);
-        x[p] = hi;
-        x[p + 32] = lo;
-        split(tile[tx][r], hi, lo);
-        const long long q = pair_at(j0 + r, i0 + tx, a.mp);
-        xt[q] = hi;
-        xt[q + 32] = lo;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {                                               // eight entries of a row per thread: 16-byte stores
+        const int r = (threadIdx.x >> 3) + 32 * q, c = (threadIdx.x & 7) * 8;
+        half8 h, l;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            _Float16 p, w;
+            split(tile[r][c + k], p, w);
+            h[k] = p;
+            l[k] = w;
+        }
+        const long long at = pair_at(i0 + r, j0 + c, a.np);
+        *reinterpret_cast<half8*>(x + at) = h;
+        *reinterpret_cast<half8*>(x + at + 32) = l;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            _Float16 p, w;
+            split(tile[c + k][r], p, w);
+            h[k] = p;
+            l[k] = w;
+        }
+        const long long to = pair_at(j0 + r, i0 + c, a.mp);
+        *reinterpret_cast<half8*>(xt + to) = h;
+        *reinterpret_cast<half8*>(xt + to + 32) = l;
     }
 }
 
 enum { NS_GRAM = 0, NS_POLY = 1, NS_STEP = 2, NS_LAST = 3 };
 
-// C[i, j] = sum_k A[i, k] B[j, k] over pair matrices, tile T x T, four waves of T/2 x T/2.  K goes in blocks of 32 pairs = 128 bytes per
-// row, two LDS stages filled by buffer_load ... lds, chunks XOR-swizzled by (row >> 1) & 7.  PAIR: three products per block, else the
-// values only (half of the loaded bytes; the block layout stays).
+// A T x T tile of pairs in LDS: 128-byte blocks [row][T / 32], the two blocks of a 256-byte line swapped and the 16-byte chunks of a block
+// XOR-ed by the row: the accumulator's layout (a lane owns a row), rows (the copy-out) and the transposing reads all spread over the banks.
+constexpr int threads_of(int T) { return T == 256 ? 512 : 256; }
+
+template <int T>
+__device__ __forceinline__ int tile_at(int row, int blk, int chunk) {
+    return (row * (T / 32) + (blk ^ ((row >> 3) & 1))) * 128 + ((chunk ^ (row & 7)) << 4);
+}
+
+// C[i, j] = sum_k A[i, k] B[j, k] over pair matrices, tile T x T, two rows of WJ waves of T/2 x T/WJ.  K goes in blocks of 32 pairs = 128 bytes per
+// row through a ring of NST LDS stages filled by buffer_load ... lds (chunks XOR-swizzled by (row >> 1) & 7), NST - 1 of them in flight.
+// PAIR: three products per block, else the values only (half of the loaded bytes; the block layout stays).
 //   GRAM  A = B = X,          S = C                       (tiles i >= j, stored twice)
 //   POLY  A = B = S,          P = b S + c C               (tiles i >= j, stored twice)
 //   STEP  A = P, B = X^T,     X <- a X + C  in both orientations (X in place: a tile is read and written by its own workgroup only)
 //   LAST  the same, into the parameter or the output
-template <int KIND, int T, bool PAIR, typename OT>
-__global__ __launch_bounds__(256) void k_ns_gemm(NsArgs a, int in, int tiles_i, int tiles_j) {
-    [[maybe_unused]] constexpr int ROWB = 128, STAGE = 2 * T * ROWB, TW = T / 2, FT = TW / 32, PIECES = T / 32;
-    [[maybe_unused]] __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
+// The epilogue goes through LDS: the tile of S or X arrives as whole lines, every lane replaces its own entries, and whole lines leave in
+// both orientations (the transposed one by ds_read_b64_tr_b16); a 256 tile does that half by half.
+// mode 0: the whole product.  1: this workgroup's share (blockIdx.z) of a split contraction, fp32 sums to a.part.  2: joins those shares.
+template <int KIND, int T, int NST, bool PAIR, typename OT>
+__global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, int in, int tiles_i, int tiles_j, int count, int mode, int splits) {
+    [[maybe_unused]] constexpr int NT = threads_of(T), NW = NT / 64, WJ = NW / 2, ROWB = 128, STAGE = 2 * T * ROWB, TI = T / 2, TJ = T / WJ, FI = TI / 32, FJ = TJ / 32,
+                                   PIECES = T / 8 / NW, H = T == 256 ? 2 : 1, TR = T / H;       // TR rows per epilogue pass
+    extern __shared__ __attribute__((aligned(16))) char smem[];      // max(NST * STAGE, 4 TR T)
 #if defined(__HIP_DEVICE_COMPILE__)
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, hi = lane >> 5, l31 = lane & 31;
-    const int wi = wave >> 1, wj = wave & 1;
+    const int wi = wave / WJ, wj = wave % WJ;
     // XCD-contiguous tile order (block b runs on XCD b % 8), matrix by matrix
     const int per_mat = KIND <= NS_POLY ? tiles_i * (tiles_i + 1) / 2 : tiles_i * tiles_j;
-    const int total = per_mat * (int)gridDim.y;
-    const int lin = blockIdx.y * gridDim.x + blockIdx.x;
-    const int per = (total + 7) / 8;
-    const int id = (lin & 7) * per + (lin >> 3);
-    if ((lin >> 3) >= per || id >= total) return;
+    const int total = per_mat * count, per = (total + 7) / 8;
+    const int id = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+    if (id >= total) return;
     const int b = id / per_mat, rem = id - b * per_mat;
     int ti, tj;
     if constexpr (KIND <= NS_POLY) {
@@ -160,130 +219,244 @@ __global__ __launch_bounds__(256) void k_ns_gemm(NsArgs a, int in, int tiles_i, 
         tj = rem / tiles_i;
     }
     const int i0 = ti * T, j0 = tj * T;
-    const int kw = KIND == NS_GRAM ? a.np : a.mp;                 // contraction width (padded)
-    const _Float16* A = KIND == NS_GRAM ? a.x + (long long)b * a.mp * 2 * a.np : (KIND == NS_POLY ? a.s : a.pm) + (long long)b * a.mp * 2 * a.mp;
-    const _Float16* B = KIND <= NS_POLY ? A : a.xt[in] + (long long)b * a.np * 2 * a.mp;
-    const int arows = min(T, a.mp - i0), brows = min(T, (KIND <= NS_POLY ? a.mp : a.np) - j0);
-    const __amdgpu_buffer_rsrc_t ars = __builtin_amdgcn_make_buffer_rsrc((void*)(A + (long long)i0 * 2 * kw), 0, arows * kw * 4, 0x00020000);
-    const __amdgpu_buffer_rsrc_t brs = __builtin_amdgcn_make_buffer_rsrc((void*)(B + (long long)j0 * 2 * kw), 0, brows * kw * 4, 0x00020000);
-    unsigned off[PIECES];                                          // rows past the matrix lie past the descriptor: zeros
+    f32x16 acc[FI][FJ];
+    if (mode == 2) {
 #pragma unroll
-    for (int p = 0; p < PIECES; ++p) {
-        const int row = wave * (T / 4) + 8 * p + (lane >> 3);
-        off[p] = (unsigned)row * (unsigned)kw * 4u + (unsigned)(((lane & 7) ^ ((row >> 1) & 7)) * 16);
-    }
-    auto issue = [&](int s, int stage) __attribute__((always_inline)) {
-        char* base = smem + stage * STAGE;
+        for (int i = 0; i < FI; ++i)
 #pragma unroll
-        for (int p = 0; p < PIECES; ++p)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(ars, (__attribute__((address_space(3))) void*)(base + (wave * (T / 4) + 8 * p) * ROWB), 16, (int)off[p], s * 128, 0, 0);
+            for (int j = 0; j < FJ; ++j)
 #pragma unroll
-        for (int p = 0; p < PIECES; ++p)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(brs, (__attribute__((address_space(3))) void*)(base + T * ROWB + (wave * (T / 4) + 8 * p) * ROWB), 16, (int)off[p], s * 128, 0, 0);
-    };
-    f32x16 acc[FT][FT];
-#pragma unroll
-    for (int i = 0; i < FT; ++i)
-#pragma unroll
-        for (int j = 0; j < FT; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-    auto frag = [&](const char* base, int row, int chunk) __attribute__((always_inline)) {
-        return *reinterpret_cast<const half8*>(base + row * ROWB + ((chunk ^ ((row >> 1) & 7)) << 4));
-    };
-    const int steps = kw / 32;
-    issue(0, 0);
-    for (int s = 0; s < steps; ++s) {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        if (s + 1 < steps) issue(s + 1, (s + 1) & 1);
-        const char* ab = smem + (s & 1) * STAGE;
-        const char* bb = ab + T * ROWB;
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            half8 ah[FT], al[FT], bh[FT], bl[FT];
-#pragma unroll
-            for (int i = 0; i < FT; ++i) {
-                const int ra = TW * wi + 32 * i + l31, rb = TW * wj + 32 * i + l31;
-                ah[i] = frag(ab, ra, 2 * kk + hi);
-                bh[i] = frag(bb, rb, 2 * kk + hi);
-                if constexpr (PAIR) {
-                    al[i] = frag(ab, ra, 4 + 2 * kk + hi);
-                    bl[i] = frag(bb, rb, 4 + 2 * kk + hi);
-                }
-            }
-            // B as the matrix instruction's first operand: a lane holds one row i and four consecutive columns j per group
-#pragma unroll
-            for (int i = 0; i < FT; ++i)
-#pragma unroll
-                for (int j = 0; j < FT; ++j) {
-                    if constexpr (PAIR) {
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bl[j], ah[i], acc[i][j], 0, 0, 0);
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bh[j], al[i], acc[i][j], 0, 0, 0);
+                for (int g = 0; g < 4; ++g) {
+                    const float4* p = reinterpret_cast<const float4*>(a.part) + ((long long)id * splits * FI * FJ * 4 + (i * FJ + j) * 4 + g) * NT + tid;
+                    float4 v = p[0];
+                    for (int z = 1; z < splits; ++z) {
+                        const float4 w = p[(long long)z * FI * FJ * 4 * NT];
+                        v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
                     }
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bh[j], ah[i], acc[i][j], 0, 0, 0);
+                    acc[i][j][4 * g] = v.x; acc[i][j][4 * g + 1] = v.y; acc[i][j][4 * g + 2] = v.z; acc[i][j][4 * g + 3] = v.w;
                 }
+    } else {
+        const int kw = KIND == NS_GRAM ? a.np : a.mp;              // contraction width (padded)
+        const _Float16* A = KIND == NS_GRAM ? a.x + (long long)b * a.mp * 2 * a.np : (KIND == NS_POLY ? a.s : a.pm) + (long long)b * a.mp * 2 * a.mp;
+        const _Float16* B = KIND <= NS_POLY ? A : a.xt[in] + (long long)b * a.np * 2 * a.mp;
+        const int arows = min(T, a.mp - i0), brows = min(T, (KIND <= NS_POLY ? a.mp : a.np) - j0);
+        const __amdgpu_buffer_rsrc_t ars = __builtin_amdgcn_make_buffer_rsrc((void*)(A + (long long)i0 * 2 * kw), 0, arows * kw * 4, 0x00020000);
+        const __amdgpu_buffer_rsrc_t brs = __builtin_amdgcn_make_buffer_rsrc((void*)(B + (long long)j0 * 2 * kw), 0, brows * kw * 4, 0x00020000);
+        unsigned off[PIECES];                                      // rows past the matrix lie past the descriptor: zeros
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            const int row = wave * (T / NW) + 8 * p + (lane >> 3);
+            off[p] = (unsigned)row * (unsigned)kw * 4u + (unsigned)(((lane & 7) ^ ((row >> 1) & 7)) * 16);
+        }
+        auto issue = [&](int s, int stage) __attribute__((always_inline)) {
+            char* base = smem + stage * STAGE;
+#pragma unroll
+            for (int p = 0; p < PIECES; ++p)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(ars, (__attribute__((address_space(3))) void*)(base + (wave * (T / NW) + 8 * p) * ROWB), 16, (int)off[p], s * 128, 0, 0);
+#pragma unroll
+            for (int p = 0; p < PIECES; ++p)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(brs, (__attribute__((address_space(3))) void*)(base + T * ROWB + (wave * (T / NW) + 8 * p) * ROWB), 16, (int)off[p], s * 128, 0, 0);
+        };
+#pragma unroll
+        for (int i = 0; i < FI; ++i)
+#pragma unroll
+            for (int j = 0; j < FJ; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+        auto frag = [&](const char* base, int row, int chunk) __attribute__((always_inline)) {
+            return *reinterpret_cast<const half8*>(base + row * ROWB + ((chunk ^ ((row >> 1) & 7)) << 4));
+        };
+        const int all = kw / 32;
+        const int s_lo = mode == 1 ? (int)((long long)all * blockIdx.z / splits) : 0, s_hi = mode == 1 ? (int)((long long)all * (blockIdx.z + 1) / splits) : all;
+#pragma unroll
+        for (int q = 0; q < NST - 1; ++q)
+            if (s_lo + q < s_hi) issue(s_lo + q, q);
+        int st = 0;
+        for (int s = s_lo; s < s_hi; ++s) {
+            // this wave's pieces of stage s have landed when at most the younger stages' (2 PIECES each) are outstanding
+            if (s + NST - 2 < s_hi) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 2) * 2 * PIECES) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            const int fill = st == 0 ? NST - 1 : st - 1;           // the stage read one step ago
+            if (s + NST - 1 < s_hi) issue(s + NST - 1, fill);
+            const char* ab = smem + st * STAGE;
+            const char* bb = ab + T * ROWB;
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+                half8 ah[FI], al[FI], bh[FJ], bl[FJ];
+#pragma unroll
+                for (int i = 0; i < FI; ++i) {
+                    const int row = TI * wi + 32 * i + l31;
+                    ah[i] = frag(ab, row, 2 * kk + hi);
+                    if constexpr (PAIR) al[i] = frag(ab, row, 4 + 2 * kk + hi);
+                }
+#pragma unroll
+                for (int j = 0; j < FJ; ++j) {
+                    const int row = TJ * wj + 32 * j + l31;
+                    bh[j] = frag(bb, row, 2 * kk + hi);
+                    if constexpr (PAIR) bl[j] = frag(bb, row, 4 + 2 * kk + hi);
+                }
+                // B as the matrix instruction's first operand: a lane holds one row i and four consecutive columns j per group
+#pragma unroll
+                for (int i = 0; i < FI; ++i)
+#pragma unroll
+                    for (int j = 0; j < FJ; ++j) {
+                        if constexpr (PAIR) {
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bl[j], ah[i], acc[i][j], 0, 0, 0);
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bh[j], al[i], acc[i][j], 0, 0, 0);
+                        }
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bh[j], ah[i], acc[i][j], 0, 0, 0);
+                    }
+            }
+            st = st + 1 == NST ? 0 : st + 1;
+        }
+        if (mode == 1) {
+#pragma unroll
+            for (int i = 0; i < FI; ++i)
+#pragma unroll
+                for (int j = 0; j < FJ; ++j)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        reinterpret_cast<float4*>(a.part)[(((long long)id * splits + blockIdx.z) * FI * FJ * 4 + (i * FJ + j) * 4 + g) * NT + tid] =
+                            make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
+            return;
         }
     }
 
-    // ---- epilogue.  lane: row i = l31 of the fragment, registers 4 g + r: columns 8 g + 4 hi + r.
+    // ---- epilogue.  lane: row i = l31 of the fragment, registers 4 g + r: columns 8 g + 4 hi + r
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
     const int ow = KIND <= NS_POLY ? a.mp : a.np, oh = a.mp;
+    for (int h = 0; h < H; ++h) {
+        const int r0 = i0 + h * TR;                                    // first row of this pass
+        if (h && r0 >= oh) break;
+        __syncthreads();                                               // every wave has read its last fragments (its share of the last pass)
+        if constexpr (KIND != NS_GRAM) {
+            constexpr int P = TR * T / 256 / NW;                       // 1 KB = 8 blocks per wave and request
+            const _Float16* src = KIND == NS_POLY ? a.s + (long long)b * a.mp * 2 * a.mp : a.x + (long long)b * a.mp * 2 * a.np;
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(src + (long long)r0 * 2 * ow), 0, min(TR, oh - r0) * ow * 4, 0x00020000);
 #pragma unroll
-    for (int fi = 0; fi < FT; ++fi) {
-        const int i = i0 + TW * wi + 32 * fi + l31;
+            for (int p = 0; p < P; ++p) {
+                const int q = (wave * P + p) * 8 + (lane >> 3), row = q / (T / 32), blk = (q % (T / 32)) ^ ((row >> 3) & 1);
+                const unsigned o = (unsigned)row * (unsigned)ow * 4u + (unsigned)((j0 / 32 + blk) * 128 + (((lane & 7) ^ (row & 7)) << 4));
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(smem + (wave * P + p) * 1024), 16, (int)o, 0, 0, 0);
+            }
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+        }
+        if (H == 1 || wi == h) {
 #pragma unroll
-        for (int fj = 0; fj < FT; ++fj) {
+            for (int fi = 0; fi < FI; ++fi)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int j = j0 + TW * wj + 32 * fj + 8 * g + 4 * hi;
-                if (i >= oh || j >= ow) continue;
-                float v[4];
+                for (int fj = 0; fj < FJ; ++fj)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = acc[fi][fj][4 * g + r] * kInv;
-                const long long at = pair_at(i, j, ow);
-                if constexpr (KIND == NS_POLY) {
-                    const _Float16* S = a.s + (long long)b * a.mp * 2 * a.mp + at;
-                    const half4 h = *reinterpret_cast<const half4*>(S), l = *reinterpret_cast<const half4*>(S + 32);
+                    for (int g = 0; g < 4; ++g) {
+                        const int row = (H == 1 ? TI * wi : 0) + 32 * fi + l31, blk = (TJ * wj) / 32 + fj;
+                        half4* vp = reinterpret_cast<half4*>(smem + tile_at<T>(row, blk, g) + 8 * hi);
+                        half4* rp = reinterpret_cast<half4*>(smem + tile_at<T>(row, blk, 4 + g) + 8 * hi);
+                        float v[4];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) v[r] = kB * ((float)h[r] + (float)l[r]) + kC * v[r];
-                }
-                if constexpr (KIND >= NS_STEP) {
-                    const _Float16* X = a.x + (long long)b * a.mp * 2 * a.np + at;
-                    const half4 h = *reinterpret_cast<const half4*>(X), l = *reinterpret_cast<const half4*>(X + 32);
+                        for (int r = 0; r < 4; ++r) v[r] = acc[fi][fj][4 * g + r] * kInv;
+                        if constexpr (KIND != NS_GRAM) {
+                            const half4 hv = *vp, lv = *rp;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) v[r] = kA * ((float)h[r] + (float)l[r]) + v[r];
-                }
-                if constexpr (KIND == NS_LAST) {
+                            for (int r = 0; r < 4; ++r) {
+                                const float old = (float)hv[r] + (float)lv[r];
+                                v[r] = KIND == NS_POLY ? kB * old + kC * v[r] : kA * old + v[r];
+                            }
+                        }
+                        if constexpr (KIND == NS_LAST) {               // fp32 in the pair's place: columns 0, 1 | 2, 3 of the four
+                            *reinterpret_cast<float2*>(vp) = make_float2(v[0] * kInv, v[1] * kInv);
+                            *reinterpret_cast<float2*>(rp) = make_float2(v[2] * kInv, v[3] * kInv);
+                        } else {
+                            half4 hv, lv;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        if (i >= a.m || j + r >= a.n) continue;
-                        const long long to = a.flip ? (long long)(j + r) * a.cols + i : (long long)i * a.cols + j + r;
-                        const float o = v[r] * kInv;
-                        if (a.t.p[b]) a.t.p[b][to] = a.t.p[b][to] * a.decay - a.step * o;
-                        else reinterpret_cast<OT*>(a.t.out[b])[to] = (OT)o;
-                    }
-                } else {
-                    half4 h, l;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        _Float16 p, q;
-                        split(v[r], p, q);
-                        h[r] = p;
-                        l[r] = q;
-                    }
-                    _Float16* D = KIND == NS_GRAM ? a.s : KIND == NS_POLY ? a.pm : a.x;
-                    D += (long long)b * oh * 2 * ow;
-                    *reinterpret_cast<half4*>(D + at) = h;
-                    *reinterpret_cast<half4*>(D + at + 32) = l;
-                    if (KIND == NS_STEP || ti != tj) {             // the other orientation
-                        _Float16* E = KIND == NS_STEP ? a.xt[in ^ 1] + (long long)b * a.np * 2 * a.mp : D;
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const long long q = pair_at(j + r, i, a.mp);
-                            E[q] = h[r];
-                            E[q + 32] = l[r];
+                            for (int r = 0; r < 4; ++r) {
+                                _Float16 p, q;
+                                split(v[r], p, q);
+                                hv[r] = p;
+                                lv[r] = q;
+                            }
+                            *vp = hv;
+                            *rp = lv;
                         }
                     }
+        }
+        __syncthreads();
+        if constexpr (KIND == NS_LAST) {
+            float* p = a.t.p[b];
+            OT* out = reinterpret_cast<OT*>(a.t.out[b]);
+            // four entries per thread along the fast axis of the matrix as given, a batch of loads in flight
+            constexpr int Q = TR * T / 4 / NT, U = T == 256 ? 4 : Q < 8 ? Q : 8;
+            static_assert(Q % U == 0, "whole batches");
+            const bool four = (a.flip ? a.m : a.n) % 4 == 0 && !((uintptr_t)(p ? (void*)p : (void*)out) & 15);
+            for (int k0 = 0; k0 < Q; k0 += U) {
+                float4 old[U];
+                long long to[U];
+                int ok[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int k = tid + (k0 + u) * NT;
+                    const int row = a.flip ? k % (TR / 4) * 4 : k / (T / 4), col = a.flip ? k / (TR / 4) : k % (T / 4) * 4, i = r0 + row, j = j0 + col;
+                    const int fast = a.flip ? a.m - i : a.n - j, slow = a.flip ? a.n - j : a.m - i;
+                    ok[u] = slow > 0 ? max(0, min(4, fast)) : 0;
+                    to[u] = a.flip ? (long long)j * a.cols + i : (long long)i * a.cols + j;
+                    if (p && ok[u]) {
+                        if (four) old[u] = *reinterpret_cast<const float4*>(p + to[u]);
+                        else {
+                            old[u].x = p[to[u]];
+                            old[u].y = ok[u] > 1 ? p[to[u] + 1] : 0.f;
+                            old[u].z = ok[u] > 2 ? p[to[u] + 2] : 0.f;
+                            old[u].w = ok[u] > 3 ? p[to[u] + 3] : 0.f;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (!ok[u]) continue;
+                    const int k = tid + (k0 + u) * NT;
+                    const int row = a.flip ? k % (TR / 4) * 4 : k / (T / 4), col = a.flip ? k / (TR / 4) : k % (T / 4) * 4;
+                    float o[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int rr = a.flip ? row + r : row, cc = a.flip ? col : col + r;
+                        o[r] = *reinterpret_cast<const float*>(smem + tile_at<T>(rr, cc >> 5, ((cc & 31) >> 3) + ((cc & 2) << 1)) + ((cc & 4) << 1) + ((cc & 1) << 2));
+                    }
+                    if (p) {
+                        const float w[4] = {old[u].x * a.decay - a.step * o[0], old[u].y * a.decay - a.step * o[1], old[u].z * a.decay - a.step * o[2],
+                                            old[u].w * a.decay - a.step * o[3]};
+                        if (four) *reinterpret_cast<float4*>(p + to[u]) = make_float4(w[0], w[1], w[2], w[3]);
+                        else
+                            for (int r = 0; r < ok[u]; ++r) p[to[u] + r] = w[r];
+                    } else if (four) {
+                        typedef OT vec __attribute__((ext_vector_type(4)));
+                        *reinterpret_cast<vec*>(out + to[u]) = vec{(OT)o[0], (OT)o[1], (OT)o[2], (OT)o[3]};
+                    } else {
+                        for (int r = 0; r < ok[u]; ++r) out[to[u] + r] = (OT)o[r];
+                    }
+                }
+            }
+        } else {
+            _Float16* D = (KIND == NS_GRAM ? a.s : KIND == NS_POLY ? a.pm : a.x) + (long long)b * oh * 2 * ow;
+#pragma unroll 4
+            for (int q = tid; q < TR * T / 4; q += NT) {               // 16-byte chunks, whole rows of blocks
+                const int chunk = q & 7, blk = (q >> 3) % (T / 32), row = (q >> 3) / (T / 32);
+                if (r0 + row < oh && j0 + 32 * blk < ow)
+                    *reinterpret_cast<u32x4*>(D + (long long)(r0 + row) * 2 * ow + (j0 / 32 + blk) * 64 + chunk * 8) =
+                        *reinterpret_cast<const u32x4*>(smem + tile_at<T>(row, blk, chunk));
+            }
+            if (KIND == NS_STEP || ti != tj) {                         // the other orientation: rows j, blocks of 32 i
+                _Float16* E = KIND == NS_STEP ? a.xt[in ^ 1] + (long long)b * a.np * 2 * a.mp : D;
+                const int l15 = lane & 15, grp = lane >> 4;
+                for (int u = wave; u < (T / 16) * (TR / 32) * 2; u += NW) {
+                    const int part = u & 1, ib = (u >> 1) % (TR / 32), c0 = (u >> 1) / (TR / 32) * 16;
+                    const int row = 32 * ib + 8 * grp + (l15 >> 2), cc = (c0 & 31) + 4 * (l15 & 3);
+                    const char* p0 = smem + tile_at<T>(row, c0 >> 5, (cc >> 3) + 4 * part) + ((cc & 4) << 1);
+                    const char* p1 = smem + tile_at<T>(row + 4, c0 >> 5, (cc >> 3) + 4 * part) + ((cc & 4) << 1);
+                    const elem4 q0 = dm_ds_read_tr16_b64(p0), q1 = dm_ds_read_tr16_b64(p1);
+                    const elem8 o = {q0[0], q0[1], q0[2], q0[3], q1[0], q1[1], q1[2], q1[3]};
+                    const int j = j0 + c0 + l15, i = r0 + 32 * ib;
+                    if (j < ow && i < oh) *reinterpret_cast<elem8*>(E + pair_at(j, i, a.mp) + 8 * grp + 32 * part) = o;
                 }
             }
         }
@@ -293,43 +466,81 @@ __global__ __launch_bounds__(256) void k_ns_gemm(NsArgs a, int in, int tiles_i, 
 
 long long pad64(long long v) { return (v + 63) / 64 * 64; }
 
-// bytes of one matrix's workspace and of a group's
+// Split of the Gram contraction: a wide X (n much larger than m) has few tiles with a long K each.  Shares of at least 16 steps, at most
+// two workgroups per CU in all.  1: no split.
+constexpr int kSplitTiles = 512;
+int gram_splits(int mp, int np, int count) {
+    const int t = (mp + 127) / 128, tiles = t * (t + 1) / 2 * count;
+    return std::max(1, std::min(kSplitTiles / tiles, np / 32 / 16));
+}
+
+// bytes of one matrix's workspace; of the split's partial sums
 long long mat_bytes(long long rows, long long cols) {
     const long long m = pad64(std::min(rows, cols)), n = pad64(std::max(rows, cols));
     return 4 * (3 * m * n + 2 * m * m) + 8 * kNormParts;
 }
+long long part_bytes(long long rows, long long cols) {
+    const int m = (int)pad64(std::min(rows, cols)), n = (int)pad64(std::max(rows, cols));
+    return m >= 128 && gram_splits(m, n, 1) > 1 ? kSplitTiles * 4LL * 128 * 128 : 0;
+}
 
-// 128-wide tiles where they fill the chip (and the padded size loses little), else 64
-bool wide_tiles(long long i, long long j, long long count) { return i >= 128 && j >= 128 && (i / 128) * (j / 128) * count >= 256; }
+template <int KIND, int T, int NST, bool PAIR, typename OT>
+int launch_tile(const NsArgs& a, int in, int count, int mode, int splits, hipStream_t stream) {
+    constexpr int LDS = std::max(NST * 2 * T * 128, T == 256 ? 2 * T * T : 4 * T * T);
+    static hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_ns_gemm<KIND, T, NST, PAIR, OT>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    if (attr != hipSuccess) return (int)attr;
+    const int ti = (a.mp + T - 1) / T, tj = ((KIND <= NS_POLY ? a.mp : a.np) + T - 1) / T;
+    const long long total = (KIND <= NS_POLY ? (long long)ti * (ti + 1) / 2 : (long long)ti * tj) * count;
+    hipLaunchKernelGGL((k_ns_gemm<KIND, T, NST, PAIR, OT>), dim3((unsigned)((total + 7) / 8 * 8), 1, mode == 1 ? splits : 1), dim3(threads_of(T)), LDS, stream, a, in, ti, tj, count,
+                       mode, splits);
+    DM_LAUNCH_CHECK();
+    return DM_OK;
+}
 
-template <int KIND, typename OT>
-void launch_gemm(const NsArgs& a, int in, bool pair, int count, hipStream_t stream) {
-    const int cols = KIND <= NS_POLY ? a.mp : a.np;
-    auto go = [&](auto t_tag, auto pair_tag) {
-        constexpr int T = decltype(t_tag)::value;
-        const int ti = (a.mp + T - 1) / T, tj = (cols + T - 1) / T;
-        const int per_mat = KIND <= NS_POLY ? ti * (ti + 1) / 2 : ti * tj;
-        const int per = (per_mat * count + 7) / 8;                 // the kernel's XCD order wants 8 * per blocks in all
-        const unsigned gx = (unsigned)((8LL * per + count - 1) / count);
-        hipLaunchKernelGGL((k_ns_gemm<KIND, T, decltype(pair_tag)::value, OT>), dim3(gx, (unsigned)count), dim3(256), 0, stream, a, in, ti, tj);
+// Tile by the time a launch takes, in rounds of the chip at one 256 tile per CU (measured on 1280^2, paired): a 256 tile needs a third of a
+// 128 tile's LDS and request traffic per product; 128 tiles run two per CU and a round of 512 costs 1.15, half a round 0.6; 64 tiles 0.3
+// per 512, 0.25 where a CU gets one (then with a ring as deep as LDS allows: its loads have nothing else to hide behind).
+template <int KIND, bool PAIR, typename OT>
+int launch_gemm(const NsArgs& a, int in, int count, hipStream_t stream) {
+    auto tiles = [&](int T) {
+        const long long t = (a.mp + T - 1) / T, u = ((KIND <= NS_POLY ? a.mp : a.np) + T - 1) / T;
+        return (KIND <= NS_POLY ? t * (t + 1) / 2 : t * u) * count;
     };
-    const bool wide = wide_tiles(a.mp, cols, count);
-    if (wide) pair ? go(std::integral_constant<int, 128>{}, std::true_type{}) : go(std::integral_constant<int, 128>{}, std::false_type{});
-    else pair ? go(std::integral_constant<int, 64>{}, std::true_type{}) : go(std::integral_constant<int, 64>{}, std::false_type{});
+    if (KIND == NS_GRAM && a.part && a.mp >= 128) {
+        const int splits = gram_splits(a.mp, a.np, count);
+        if (splits > 1) {
+            if (int rc = launch_tile<KIND, 128, 2, PAIR, OT>(a, in, count, 1, splits, stream)) return rc;
+            return launch_tile<KIND, 128, 2, PAIR, OT>(a, in, count, 2, splits, stream);
+        }
+    }
+    const double c256 = a.mp >= 256 ? (double)((tiles(256) + 255) / 256) : 1e30;
+    const double c128 = a.mp >= 128 ? std::max(0.6, 1.15 * (double)tiles(128) / 512) : 1e30;
+    const double c64 = tiles(64) <= 256 ? 0.25 : 0.3 * (double)((tiles(64) + 511) / 512);
+    if (c256 <= c128 && c256 <= c64) return launch_tile<KIND, 256, 2, PAIR, OT>(a, in, count, 0, 1, stream);
+    if (c128 <= c64) return launch_tile<KIND, 128, 2, PAIR, OT>(a, in, count, 0, 1, stream);
+    if (tiles(64) <= 256) return launch_tile<KIND, 64, 8, PAIR, OT>(a, in, count, 0, 1, stream);
+    return launch_tile<KIND, 64, 4, PAIR, OT>(a, in, count, 0, 1, stream);
 }
 
 template <typename T>
-int run_group(NsArgs& a, int count, int steps, int plain_steps, hipStream_t stream) {
-    hipLaunchKernelGGL((k_ns_norm<T>), dim3(kNormParts, count), dim3(256), 0, stream, a);
+int run_group(NsArgs& a, int count, int steps, hipStream_t stream) {
+    hipLaunchKernelGGL((k_ns_norm<T>), dim3(a.parts, count), dim3(256), 0, stream, a);
     hipLaunchKernelGGL((k_ns_pack<T>), dim3(a.np / 64, a.mp / 64, count), dim3(256), 0, stream, a);
     DM_LAUNCH_CHECK();
+    constexpr bool SHORT = std::is_same<T, __bf16>::value;       // bf16: the last two iterations without the rests, see the head of the file
+    const int plain_from = SHORT ? std::max(1, steps - 2) : steps;
     for (int k = 0; k < steps; ++k) {
-        const bool pair = k < steps - plain_steps;
-        launch_gemm<NS_GRAM, T>(a, k & 1, pair, count, stream);
-        launch_gemm<NS_POLY, T>(a, k & 1, pair, count, stream);
-        if (k + 1 < steps) launch_gemm<NS_STEP, T>(a, k & 1, pair, count, stream);
-        else launch_gemm<NS_LAST, T>(a, k & 1, pair, count, stream);
-        DM_LAUNCH_CHECK();
+        int rc;
+        if (k < plain_from) {
+            if ((rc = launch_gemm<NS_GRAM, true, float>(a, k & 1, count, stream)) || (rc = launch_gemm<NS_POLY, true, float>(a, k & 1, count, stream))) return rc;
+            rc = k + 1 < steps ? launch_gemm<NS_STEP, true, float>(a, k & 1, count, stream) : launch_gemm<NS_LAST, true, T>(a, k & 1, count, stream);
+        } else if constexpr (SHORT) {
+            if ((rc = launch_gemm<NS_GRAM, false, float>(a, k & 1, count, stream)) || (rc = launch_gemm<NS_POLY, false, float>(a, k & 1, count, stream))) return rc;
+            rc = k + 1 < steps ? launch_gemm<NS_STEP, false, float>(a, k & 1, count, stream) : launch_gemm<NS_LAST, false, T>(a, k & 1, count, stream);
+        } else {
+            rc = DM_OK;
+        }
+        if (rc) return rc;
     }
     return DM_OK;
 }
@@ -340,25 +551,31 @@ int run(const void* const* g, float* const* mom, float* const* p, void* const* o
     if (count < 0 || rows <= 0 || cols <= 0 || steps < 1 || steps > 64 || dtype < 0 || dtype > 2 || !ws) return DM_ERR_ARG;
     if ((long long)rows * cols > (1LL << 31) || std::min(rows, cols) > 32768 || std::max(rows, cols) > (1 << 20)) return DM_ERR_UNSUPPORTED;
     if ((uintptr_t)ws & 255) return DM_ERR_ARG;
-    const long long one = mat_bytes(rows, cols);
-    const int fit = (int)std::min<long long>(kGroup, (long long)ws_bytes / one);
+    const long long one = mat_bytes(rows, cols), extra = part_bytes(rows, cols);
+    const int fit = (int)std::min<long long>(kGroup, std::max<long long>(0, (long long)ws_bytes - extra) / one);
     if (count && fit < 1) return DM_ERR_WORKSPACE;
     NsArgs a{};
     a.rows = rows; a.cols = cols; a.flip = rows > cols;
     a.m = std::min(rows, cols); a.n = std::max(rows, cols);
     a.mp = (int)pad64(a.m); a.np = (int)pad64(a.n);
     a.mu = mu; a.nesterov = nesterov; a.eps = eps; a.decay = decay; a.step = step;
+    a.parts = (int)std::max<long long>(1, std::min<long long>(kNormParts, (long long)rows * cols / (256 * 8)));
     DM_ENTER();
     for (int at = 0; at < count; at += fit) {
         const int c = std::min(fit, count - at);
+        bool whole = cols % 4 == 0;                                // rows of 16-byte (8-byte) chunks in every operand of the norm pass
         for (int i = 0; i < c; ++i) {
             a.t.g[i] = g[at + i];
             a.t.mom[i] = mom ? mom[at + i] : nullptr;
             a.t.p[i] = p ? p[at + i] : nullptr;
             a.t.out[i] = out ? out[at + i] : nullptr;
             if (!a.t.g[i] || (mom && !a.t.mom[i]) || (p ? !a.t.p[i] : !a.t.out[i])) return DM_ERR_ARG;
+            whole = whole && !(((uintptr_t)a.t.g[i] | (uintptr_t)a.t.mom[i]) & 15);
         }
+        a.whole = whole;
         char* w = (char*)ws;
+        a.part = extra ? (float*)w : nullptr;
+        w += extra;
         auto take = [&](long long bytes) { char* q = w; w += bytes * c; return q; };
         a.norm = (double*)take(8 * kNormParts);
         a.x = (_Float16*)take(4LL * a.mp * a.np);
@@ -366,9 +583,7 @@ int run(const void* const* g, float* const* mom, float* const* p, void* const* o
         a.xt[1] = (_Float16*)take(4LL * a.mp * a.np);
         a.s = (_Float16*)take(4LL * a.mp * a.mp);
         a.pm = (_Float16*)take(4LL * a.mp * a.mp);
-        // (bf16: the last two iterations without the rests, see the head of the file)
-        const int rc = dtype == 0 ? run_group<__bf16>(a, c, steps, std::min(2, steps - 1), stream)
-                     : dtype == 1 ? run_group<_Float16>(a, c, steps, 0, stream) : run_group<float>(a, c, steps, 0, stream);
+        const int rc = dtype == 0 ? run_group<__bf16>(a, c, steps, stream) : dtype == 1 ? run_group<_Float16>(a, c, steps, stream) : run_group<float>(a, c, steps, stream);
         if (rc) return rc;
     }
     return DM_OK;
@@ -381,7 +596,7 @@ extern "C" {
 // workspace bytes that take `count` [rows, cols] matrices in one launch (at most 16 at once; less memory means more launches)
 size_t dm_orthogonalize_workspace_bytes(int count, int rows, int cols) {
     if (count <= 0 || rows <= 0 || cols <= 0) return 0;
-    return (size_t)(std::min(count, kGroup) * mat_bytes(rows, cols));
+    return (size_t)(std::min(count, kGroup) * mat_bytes(rows, cols) + part_bytes(rows, cols));
 }
 
 // out[i] = five-step Newton-Schulz of g[i]: `count` same-shaped matrices [rows, cols] behind HOST arrays of device pointers; dtype 0 bf16 |

@@ -48,30 +48,38 @@ template <> struct Elems<float> { static constexpr int N = 4; };
 template <> struct Elems<__bf16> { static constexpr int N = 8; };
 template <> struct Elems<_Float16> { static constexpr int N = 8; };
 
-// one chunk = 16 bytes (VEC > 1) or one element (VEC == 1: rows that are not whole 16-byte chunks)
+// one chunk = 16 bytes (VEC > 1) or one element (VEC == 1: rows that are not whole 16-byte chunks), held as stored until it is used
+template <typename T, int VEC> struct Chunk {
+    typedef T vec __attribute__((ext_vector_type(VEC)));
+    vec v;
+    __device__ __forceinline__ float operator[](int k) const { return (float)v[k]; }
+};
+
 template <typename T, int VEC>
-__device__ __forceinline__ void load_chunk(const T* p, float (&v)[VEC]) {
-    if constexpr (VEC == 1) {
-        v[0] = (float)p[0];
-    } else {
-        typedef T vec __attribute__((ext_vector_type(VEC)));
-        const vec q = *reinterpret_cast<const vec*>(p);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) v[k] = (float)q[k];
-    }
+__device__ __forceinline__ Chunk<T, VEC> load_chunk(const void* p, long long at) {
+    Chunk<T, VEC> c;
+    const T* q = reinterpret_cast<const T*>(p) + at;
+    if constexpr (VEC == 1) c.v[0] = q[0];
+    else c.v = *reinterpret_cast<const typename Chunk<T, VEC>::vec*>(q);
+    return c;
 }
 
 template <typename T, int VEC>
-__device__ __forceinline__ void store_chunk(T* p, const float (&v)[VEC]) {
-    if constexpr (VEC == 1) {
-        p[0] = (T)v[0];
-    } else {
-        typedef T vec __attribute__((ext_vector_type(VEC)));
-        vec q;
+__device__ __forceinline__ Chunk<T, VEC> fill_chunk(float x) {
+    Chunk<T, VEC> c;
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) q[k] = (T)v[k];
-        *reinterpret_cast<vec*>(p) = q;
-    }
+    for (int k = 0; k < VEC; ++k) c.v[k] = (T)x;
+    return c;
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void store_chunk(void* p, long long at, const float (&v)[VEC]) {
+    Chunk<T, VEC> c;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) c.v[k] = (T)v[k];
+    T* q = reinterpret_cast<T*>(p) + at;
+    if constexpr (VEC == 1) q[0] = c.v[0];
+    else *reinterpret_cast<typename Chunk<T, VEC>::vec*>(q) = c.v;
 }
 
 constexpr int threads_of(int L) { return L < 256 ? 256 : L; }
@@ -115,15 +123,19 @@ __device__ __forceinline__ void row_stats(const float (&v)[NC][VEC], int chunks,
     rstd = 1.f / sqrtf(row_sum<L>(q, red) * inv_c + eps);
 }
 
-// parameter vectors: a NULL gamma is 1, a NULL beta 0
-template <typename T, int VEC>
-__device__ __forceinline__ void load_param(const void* p, int col, float (&v)[VEC], float absent) {
-    if (p) load_chunk<T, VEC>(reinterpret_cast<const T*>(p) + col, v);
-    else
+// this lane's chunks of a parameter vector; a NULL gamma is 1, a NULL beta 0
+template <typename T, int VEC, int L, int NC>
+__device__ __forceinline__ void load_params(const void* p, long long at, int l, int chunks, float absent, Chunk<T, VEC> (&out)[NC]) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) v[k] = absent;
+    for (int c = 0; c < NC; ++c) {
+        const int ch = l + L * c;
+        if (p) out[c] = load_chunk<T, VEC>(p, at + (ch < chunks ? ch : 0) * VEC);
+        else out[c] = fill_chunk<T, VEC>(absent);
+    }
 }
 
+// Workgroup b owns rows [b R, (b + 1) R) (R = rows_per_block), G row groups at a time, one gate item after the other; parameters stay in
+// registers, and the next rows are requested before this one's statistics.
 template <typename T, int VEC, int L, int NC>
 __global__ __launch_bounds__(threads_of(L)) void k_gan_fwd(GanArgs a) {
     __shared__ float red[16];
@@ -131,64 +143,75 @@ __global__ __launch_bounds__(threads_of(L)) void k_gan_fwd(GanArgs a) {
     const int l = threadIdx.x % L, grp = threadIdx.x / L;
     const int chunks = a.C / VEC;
     const float inv_c = 1.f / (float)a.C;
-    const long long step = (long long)gridDim.x * G;
-    // (the loop bound is the workgroup's, not the row's: row_sum<256> synchronises)
-    for (long long r0 = (long long)blockIdx.x * G; r0 < a.rows; r0 += step) {
-        const long long r = min(r0 + grp, a.rows - 1);
-        const bool live = r0 + grp < a.rows;
-        const T* xr = reinterpret_cast<const T*>(a.x) + r * a.C;
-        const T* hr = reinterpret_cast<const T*>(a.h) + r * a.C;
-        const T* gr = a.gate ? reinterpret_cast<const T*>(a.gate) + (a.item_rows ? r / a.item_rows * a.C : 0) : nullptr;
-        float v[NC][VEC], y[NC][VEC];
+    const long long row_lo = (long long)blockIdx.x * a.rows_per_block, row_hi = min(row_lo + a.rows_per_block, a.rows);
+    Chunk<T, VEC> pg[NC], pb[NC], qg[NC], qb[NC], g[NC], xn[NC], hn[NC];
+    auto fetch = [&](long long r) __attribute__((always_inline)) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int ch = l + L * c;
-            const bool ok = ch < chunks;
-            load_chunk<T, VEC>(hr + (ok ? ch : 0) * VEC, v[c]);
-            load_chunk<T, VEC>(xr + (ok ? ch : 0) * VEC, y[c]);
-            if (!ok)
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) v[c][k] = 0.f, y[c][k] = 0.f;
+            const long long at = r * a.C + (ch < chunks ? ch : 0) * VEC;
+            hn[c] = load_chunk<T, VEC>(a.h, at);
+            xn[c] = load_chunk<T, VEC>(a.x, at);
         }
-        float pm = 0.f, pr = 1.f, qm = 0.f, qr = 1.f;
-        if (a.post) row_stats<VEC, L, NC>(v, chunks, l, a.rms, inv_c, a.eps, red, pm, pr);
+    };
+    fetch(min(row_lo + grp, row_hi - 1));
+    load_params<T, VEC, L, NC>(a.post_g, 0, l, chunks, 1.f, pg);
+    load_params<T, VEC, L, NC>(a.post_b, 0, l, chunks, 0.f, pb);
+    load_params<T, VEC, L, NC>(a.pre_g, 0, l, chunks, 1.f, qg);
+    load_params<T, VEC, L, NC>(a.pre_b, 0, l, chunks, 0.f, qb);
+    long long seg_lo = row_lo;
+    while (seg_lo < row_hi) {
+        const long long item = a.item_rows ? seg_lo / a.item_rows : 0;
+        const long long seg_hi = a.item_rows ? min((item + 1) * a.item_rows, row_hi) : row_hi;
+        load_params<T, VEC, L, NC>(a.gate, item * a.C, l, chunks, 1.f, g);
+        // (the loop bounds are the workgroup's, not the row's: row_sum synchronises where a row is the workgroup's)
+        for (long long r0 = seg_lo; r0 < seg_hi; r0 += G) {
+            const long long r = min(r0 + grp, seg_hi - 1);
+            const bool live = r0 + grp < seg_hi;
+            float v[NC][VEC], y[NC][VEC];
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const int ch = l + L * c;
-            if (ch >= chunks) continue;
-            float g[VEC], pg[VEC], pb[VEC];
-            load_param<T, VEC>(gr, ch * VEC, g, 1.f);
-            load_param<T, VEC>(a.post_g, ch * VEC, pg, 1.f);
-            load_param<T, VEC>(a.post_b, ch * VEC, pb, 0.f);
+            for (int c = 0; c < NC; ++c) {
+                const bool ok = l + L * c < chunks;
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-                const float n = a.post ? (v[c][k] - pm) * pr * pg[k] + pb[k] : v[c][k];
-                y[c][k] += a.scale * g[k] * n;
+                for (int k = 0; k < VEC; ++k) v[c][k] = ok ? hn[c][k] : 0.f, y[c][k] = ok ? xn[c][k] : 0.f;
             }
-            if (live) store_chunk<T, VEC>(reinterpret_cast<T*>(a.y) + r * a.C + ch * VEC, y[c]);
-        }
-        if (a.pre) {
-            row_stats<VEC, L, NC>(y, chunks, l, a.rms, inv_c, a.eps, red, qm, qr);
+            const long long next = r0 + G < seg_hi ? min(r0 + G + grp, seg_hi - 1) : min(seg_hi + grp, row_hi - 1);
+            if (r0 + G < seg_hi || seg_hi < row_hi) fetch(next);
+            float pm = 0.f, pr = 1.f, qm = 0.f, qr = 1.f;
+            if (a.post) row_stats<VEC, L, NC>(v, chunks, l, a.rms, inv_c, a.eps, red, pm, pr);
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 const int ch = l + L * c;
                 if (ch >= chunks) continue;
-                float qg[VEC], qb[VEC], z[VEC];
-                load_param<T, VEC>(a.pre_g, ch * VEC, qg, 1.f);
-                load_param<T, VEC>(a.pre_b, ch * VEC, qb, 0.f);
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) z[k] = (y[c][k] - qm) * qr * qg[k] + qb[k];
-                if (live) store_chunk<T, VEC>(reinterpret_cast<T*>(a.z) + r * a.C + ch * VEC, z);
+                for (int k = 0; k < VEC; ++k) {
+                    const float n = a.post ? (v[c][k] - pm) * pr * pg[c][k] + pb[c][k] : v[c][k];
+                    y[c][k] += a.scale * g[c][k] * n;
+                }
+                if (live) store_chunk<T, VEC>(a.y, r * a.C + ch * VEC, y[c]);
             }
+            if (a.pre) {
+                row_stats<VEC, L, NC>(y, chunks, l, a.rms, inv_c, a.eps, red, qm, qr);
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    const int ch = l + L * c;
+                    if (ch >= chunks) continue;
+                    float z[VEC];
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) z[k] = (y[c][k] - qm) * qr * qg[c][k] + qb[c][k];
+                    if (live) store_chunk<T, VEC>(a.z, r * a.C + ch * VEC, z);
+                }
+            }
+            if (a.stats && live && l == 0) *reinterpret_cast<float4*>(a.stats + r * 4) = make_float4(pm, pr, qm, qr);
         }
-        if (a.stats && live && l == 0) *reinterpret_cast<float4*>(a.stats + r * 4) = make_float4(pm, pr, qm, qr);
+        seg_lo = seg_hi;
     }
 }
 
-// Workgroup b owns rows [b R, (b + 1) R) (R = rows_per_block).  Column sums that run over all rows go to part[slot][b][C], one slot
-// per wanted vector.  The gate's gradient is per item where the gate is: rows of an item may span workgroups and a workgroup may hold
-// several items, so its partial sums are flushed at every item boundary to gate_part[item + b][C] -- along a walk over the rows
-// (item, b) only grows, so item + b names the pair -- behind the other slots.
+// Rows as in the forward.  Column sums that run over all rows go to part[slot][b][C], one slot per wanted vector.  The gate's gradient is
+// per item where the gate is: rows of an item may span workgroups and a workgroup may hold several items, so its partial sums are flushed
+// at every item boundary to gate_part[item + b][C] -- along a walk over the rows (item, b) only grows, so item + b names the pair -- behind
+// the other slots.
 template <typename T, int VEC, int L, int NC>
 __global__ __launch_bounds__(threads_of(L)) void k_gan_bwd(GanArgs a) {
     __shared__ float red[16];
@@ -198,6 +221,26 @@ __global__ __launch_bounds__(threads_of(L)) void k_gan_bwd(GanArgs a) {
     const int chunks = a.C / VEC;
     const float inv_c = 1.f / (float)a.C;
     const long long row_lo = (long long)blockIdx.x * a.rows_per_block, row_hi = min(row_lo + a.rows_per_block, a.rows);
+    Chunk<T, VEC> pg[NC], pb[NC], qg[NC], g[NC], xn[NC], hn[NC], dyn[NC], dzn[NC];
+    float4 sn;
+    auto fetch = [&](long long r) __attribute__((always_inline)) {
+        sn = *reinterpret_cast<const float4*>(a.stats + r * 4);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int ch = l + L * c;
+            const long long at = r * a.C + (ch < chunks ? ch : 0) * VEC;
+            hn[c] = load_chunk<T, VEC>(a.h, at);
+            xn[c] = load_chunk<T, VEC>(a.x, at);
+            if (a.dy) dyn[c] = load_chunk<T, VEC>(a.dy, at);
+            if (a.pre) dzn[c] = load_chunk<T, VEC>(a.dz, at);
+        }
+    };
+#pragma unroll
+    for (int c = 0; c < NC; ++c) dyn[c] = fill_chunk<T, VEC>(0.f), dzn[c] = fill_chunk<T, VEC>(0.f);
+    fetch(min(row_lo + grp, row_hi - 1));
+    load_params<T, VEC, L, NC>(a.post_g, 0, l, chunks, 1.f, pg);
+    load_params<T, VEC, L, NC>(a.post_b, 0, l, chunks, 0.f, pb);
+    load_params<T, VEC, L, NC>(a.pre_g, 0, l, chunks, 1.f, qg);
     float dg[NC][VEC], dpg[NC][VEC], dpb[NC][VEC], dqg[NC][VEC], dqb[NC][VEC];
 #pragma unroll
     for (int c = 0; c < NC; ++c)
@@ -226,7 +269,7 @@ __global__ __launch_bounds__(threads_of(L)) void k_gan_bwd(GanArgs a) {
                 if (ch >= chunks) continue;
                 float sum = 0.f;
 #pragma unroll
-                for (int g = 0; g < G; ++g) sum += join[(g * NC * VEC + ck) * L + tl];
+                for (int q = 0; q < G; ++q) sum += join[(q * NC * VEC + ck) * L + tl];
                 out[ch * VEC + ck % VEC] = sum;
             }
         }
@@ -238,53 +281,39 @@ __global__ __launch_bounds__(threads_of(L)) void k_gan_bwd(GanArgs a) {
     while (seg_lo < row_hi) {                                       // one item's rows at a time (uniform for the workgroup)
         const long long item = a.item_rows ? seg_lo / a.item_rows : 0;
         const long long seg_hi = a.item_rows ? min((item + 1) * a.item_rows, row_hi) : row_hi;
-        const T* gr = a.gate ? reinterpret_cast<const T*>(a.gate) + item * a.C : nullptr;
+        load_params<T, VEC, L, NC>(a.gate, item * a.C, l, chunks, 1.f, g);
         for (long long r0 = seg_lo; r0 < seg_hi; r0 += G) {
-            const long long r = min(r0 + grp, seg_hi - 1);
+            const long long base = min(r0 + grp, seg_hi - 1) * a.C;
             const bool live = r0 + grp < seg_hi;
-            const long long base = r * a.C;
+            const float4 st = sn;
             float hh[NC][VEC], y[NC][VEC], d[NC][VEC], dz[NC][VEC];   // hhat, then yhat, dY, dz gamma_pre
-            const float4 st = *reinterpret_cast<const float4*>(a.stats + r * 4);
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                const int ch = l + L * c;
-                const bool ok = ch < chunks;
-                const long long at = base + (ok ? ch : 0) * VEC;
-                load_chunk<T, VEC>(reinterpret_cast<const T*>(a.h) + at, hh[c]);
-                load_chunk<T, VEC>(reinterpret_cast<const T*>(a.x) + at, y[c]);
-                if (a.dy) load_chunk<T, VEC>(reinterpret_cast<const T*>(a.dy) + at, d[c]);
-                if (a.pre) load_chunk<T, VEC>(reinterpret_cast<const T*>(a.dz) + at, dz[c]);
-                const bool use = ok && live;
+                const bool use = l + L * c < chunks && live;
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) {
-                    if (!use) hh[c][k] = y[c][k] = 0.f;
-                    if (!use || !a.dy) d[c][k] = 0.f;
-                    if (!use || !a.pre) dz[c][k] = 0.f;
+                    hh[c][k] = use ? hn[c][k] : 0.f;
+                    y[c][k] = use ? xn[c][k] : 0.f;
+                    d[c][k] = use ? dyn[c][k] : 0.f;
+                    dz[c][k] = use ? dzn[c][k] : 0.f;
                 }
             }
+            if (r0 + G < seg_hi || seg_hi < row_hi) fetch(r0 + G < seg_hi ? min(r0 + G + grp, seg_hi - 1) : min(seg_hi + grp, row_hi - 1));
             // y in fp32, exactly as the forward formed it
             float s1 = 0.f, s2 = 0.f;
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                const int ch = l + L * c;
-                const bool ok = ch < chunks;
-                const int col = (ok ? ch : 0) * VEC;
-                float g[VEC], pg[VEC], pb[VEC], qg[VEC];
-                load_param<T, VEC>(gr, col, g, 1.f);
-                load_param<T, VEC>(a.post_g, col, pg, 1.f);
-                load_param<T, VEC>(a.post_b, col, pb, 0.f);
-                load_param<T, VEC>(a.pre_g, col, qg, 1.f);
-                const bool use = ok && live;
+                const bool use = l + L * c < chunks && live;
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) {
                     if (a.post) hh[c][k] = use ? (hh[c][k] - st.x) * st.y : 0.f;
-                    const float n = a.post ? hh[c][k] * pg[k] + pb[k] : hh[c][k];
-                    y[c][k] += a.scale * g[k] * n;
+                    const float n = a.post ? hh[c][k] * pg[c][k] + pb[c][k] : hh[c][k];
+                    y[c][k] += a.scale * g[c][k] * n;
                     if (a.pre) {
                         y[c][k] = use ? (y[c][k] - st.z) * st.w : 0.f;        // yhat
                         dqg[c][k] += dz[c][k] * y[c][k];
                         dqb[c][k] += dz[c][k];
-                        dz[c][k] *= qg[k];
+                        dz[c][k] *= qg[c][k];
                         s1 += dz[c][k];
                         s2 += dz[c][k] * y[c][k];
                     }
@@ -301,22 +330,17 @@ __global__ __launch_bounds__(threads_of(L)) void k_gan_bwd(GanArgs a) {
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 const int ch = l + L * c;
-                const bool ok = ch < chunks, use = ok && live;
-                const int col = (ok ? ch : 0) * VEC;
-                if (use && a.dx) store_chunk<T, VEC>(reinterpret_cast<T*>(a.dx) + base + col, d[c]);
-                float g[VEC], pg[VEC], pb[VEC];
-                load_param<T, VEC>(gr, col, g, 1.f);
-                load_param<T, VEC>(a.post_g, col, pg, 1.f);
-                load_param<T, VEC>(a.post_b, col, pb, 0.f);
+                const bool use = ch < chunks && live;
+                if (use && a.dx) store_chunk<T, VEC>(a.dx, base + ch * VEC, d[c]);
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) {
                     const float dY = use ? a.scale * d[c][k] : 0.f;
-                    const float n = a.post ? hh[c][k] * pg[k] + pb[k] : hh[c][k];
+                    const float n = a.post ? hh[c][k] * pg[c][k] + pb[c][k] : hh[c][k];
                     dg[c][k] += dY * n;
-                    const float dn = dY * g[k];
+                    const float dn = dY * g[c][k];
                     dpg[c][k] += dn * hh[c][k];
                     dpb[c][k] += dn;
-                    d[c][k] = dn * (a.post ? pg[k] : 1.f);
+                    d[c][k] = dn * (a.post ? pg[c][k] : 1.f);
                     t1 += d[c][k];
                     t2 += d[c][k] * hh[c][k];
                 }
@@ -331,7 +355,7 @@ __global__ __launch_bounds__(threads_of(L)) void k_gan_bwd(GanArgs a) {
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 const int ch = l + L * c;
-                if (ch < chunks && live && a.dh) store_chunk<T, VEC>(reinterpret_cast<T*>(a.dh) + base + ch * VEC, d[c]);
+                if (ch < chunks && live && a.dh) store_chunk<T, VEC>(a.dh, base + ch * VEC, d[c]);
             }
         }
         if (a.want & GAN_DGATE) {
@@ -357,12 +381,12 @@ struct GanReduceArgs {
     long long nblk, rows_per_block, item_rows, rows, items;
 };
 
-// grid (column blocks of 64, 4 + items): y < 4 the vectors summed over all workgroups, y >= 4 the gate row of item y - 4.
-// 256 threads = 64 columns x 4 quarters of the workgroups, joined in order.
+// grid (column blocks of 32, 4 + items): y < 4 the vectors summed over all workgroups, y >= 4 the gate row of item y - 4.  1024 threads =
+// 32 columns x 32 shares of the workgroups, eight loads in flight each, joined in order.
 template <typename T>
-__global__ __launch_bounds__(256) void k_gan_reduce(GanReduceArgs a) {
-    __shared__ float red[4][64];
-    const int col = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
+__global__ __launch_bounds__(1024) void k_gan_reduce(GanReduceArgs a) {
+    __shared__ float red[32][33];
+    const int tx = threadIdx.x & 31, q = threadIdx.x >> 5, col = blockIdx.x * 32 + tx;
     const long long which = blockIdx.y;
     const float* src;
     long long n;
@@ -384,16 +408,22 @@ __global__ __launch_bounds__(256) void k_gan_reduce(GanReduceArgs a) {
     }
     float s = 0.f;
     if (col < a.C) {
-        const long long lo = n * q / 4, hi = n * (q + 1) / 4;
-        for (long long i = lo; i < hi; ++i) s += src[i * a.C + col];
+#pragma unroll 8
+        for (long long i = q; i < n; i += 32) s += src[i * a.C + col];
     }
-    red[q][threadIdx.x & 63] = s;
+    red[q][tx] = s;
     __syncthreads();
-    if (q == 0 && col < a.C) out[col] = (T)(red[0][col & 63] + red[1][col & 63] + red[2][col & 63] + red[3][col & 63]);
+    if (q == 0 && col < a.C) {
+        s = 0.f;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) s += red[k][tx];
+        out[col] = (T)s;
+    }
 }
 
-// rows of 16-byte chunks: the fewest lanes per row that keep a lane at 3 chunks or fewer (the backward holds four rows and five sums of
-// them in registers), else the whole workgroup.  Rows that are not whole aligned chunks go element by element.
+// Rows of 16-byte chunks: the fewest lanes per row that keep a lane at few chunks -- three in the forward, two in the backward, which holds
+// four rows, the next four and five sums of them in registers -- else the whole workgroup.  Rows that are not whole aligned chunks go
+// element by element.
 bool chunked(int C, int per, std::initializer_list<const void*> ptrs) {
     if (C % per) return false;
     for (const void* p : ptrs)
@@ -403,55 +433,55 @@ bool chunked(int C, int per, std::initializer_list<const void*> ptrs) {
 
 constexpr int kMaxC = 8192;
 
-template <typename T, template <typename, int, int, int> class Launch>
-int dispatch(const GanArgs& a, bool vec, int blocks_hint, hipStream_t stream) {
+template <typename T, bool BWD, template <typename, int, int, int> class Launch>
+int dispatch(GanArgs& a, bool vec, hipStream_t stream) {
     constexpr int V = Elems<T>::N;
     if (vec) {
         const int ch = a.C / V;
-        if (ch <= 16) return Launch<T, V, 16, 1>::go(a, blocks_hint, stream);
-        if (ch <= 32) return Launch<T, V, 16, 2>::go(a, blocks_hint, stream);
-        if (ch <= 48) return Launch<T, V, 16, 3>::go(a, blocks_hint, stream);
-        if (ch <= 64) return Launch<T, V, 32, 2>::go(a, blocks_hint, stream);
-        if (ch <= 96) return Launch<T, V, 32, 3>::go(a, blocks_hint, stream);
-        if (ch <= 128) return Launch<T, V, 64, 2>::go(a, blocks_hint, stream);
-        if (ch <= 192) return Launch<T, V, 64, 3>::go(a, blocks_hint, stream);
-        if (ch <= 256) return Launch<T, V, 256, 1>::go(a, blocks_hint, stream);
-        if (ch <= 512) return Launch<T, V, 256, 2>::go(a, blocks_hint, stream);
-        if (ch <= 1024) return Launch<T, V, 512, 2>::go(a, blocks_hint, stream);
-        if constexpr (V == 4) return Launch<T, V, 512, 4>::go(a, blocks_hint, stream);
+        if (ch <= 16) return Launch<T, V, 16, 1>::go(a, stream);
+        if (ch <= 32) return Launch<T, V, 16, 2>::go(a, stream);
+        if (!BWD && ch <= 48) return Launch<T, V, 16, BWD ? 2 : 3>::go(a, stream);
+        if (ch <= 64) return Launch<T, V, 32, 2>::go(a, stream);
+        if (!BWD && ch <= 96) return Launch<T, V, 32, BWD ? 2 : 3>::go(a, stream);
+        if (ch <= 128) return Launch<T, V, 64, 2>::go(a, stream);
+        if (!BWD && ch <= 192) return Launch<T, V, 64, BWD ? 2 : 3>::go(a, stream);
+        if (ch <= 256) return Launch<T, V, 256, 1>::go(a, stream);
+        if (ch <= 512) return Launch<T, V, 256, 2>::go(a, stream);
+        if (ch <= 1024) return Launch<T, V, 512, 2>::go(a, stream);
+        if constexpr (V == 4) return Launch<T, V, 512, 4>::go(a, stream);
         return DM_ERR_UNSUPPORTED;
     }
-    if (a.C <= 256) return Launch<T, 1, 64, 4>::go(a, blocks_hint, stream);
-    if (a.C <= 2048) return Launch<T, 1, 256, 8>::go(a, blocks_hint, stream);
-    return Launch<T, 1, 1024, 8>::go(a, blocks_hint, stream);
+    if (a.C <= 256) return Launch<T, 1, 64, 4>::go(a, stream);
+    if (a.C <= 2048) return Launch<T, 1, 256, 8>::go(a, stream);
+    return Launch<T, 1, 1024, 8>::go(a, stream);
 }
 
 template <typename T, int VEC, int L, int NC>
 struct Fwd {
-    static int go(const GanArgs& a, int, hipStream_t stream) {
-        const int G = threads_of(L) / L;
-        const long long need = (a.rows + G - 1) / G;
-        const unsigned blocks = (unsigned)std::min<long long>(need, 256 * (L > 256 ? 2 : 8));
-        hipLaunchKernelGGL((k_gan_fwd<T, VEC, L, NC>), dim3(blocks), dim3(threads_of(L)), 0, stream, a);
+    static int go(GanArgs& a, hipStream_t stream) {
+        constexpr int G = threads_of(L) / L;
+        const long long most = 256 * (L > 256 ? 2 : 8);            // workgroups that fill the chip
+        a.rows_per_block = ((a.rows + most - 1) / most + G - 1) / G * G;
+        hipLaunchKernelGGL((k_gan_fwd<T, VEC, L, NC>), dim3((unsigned)((a.rows + a.rows_per_block - 1) / a.rows_per_block)), dim3(threads_of(L)), 0, stream, a);
         DM_LAUNCH_CHECK();
         return DM_OK;
     }
 };
 
-template <typename T, int VEC, int L, int NC>
-struct Bwd {
-    static int go(const GanArgs& a, int blocks, hipStream_t stream) {
-        hipLaunchKernelGGL((k_gan_bwd<T, VEC, L, NC>), dim3((unsigned)blocks), dim3(threads_of(L)), 0, stream, a);
-        DM_LAUNCH_CHECK();
-        return DM_OK;
-    }
-};
-
-// workgroups of the backward: two per CU (registers allow no more at three chunks per lane), whole rows groups each
+// workgroups of the backward: two per CU (registers allow no more), whole row groups each
 long long bwd_rows_per_block(long long rows) {
     long long per = (rows + 511) / 512;
     return (per + 15) / 16 * 16;
 }
+
+template <typename T, int VEC, int L, int NC>
+struct Bwd {
+    static int go(GanArgs& a, hipStream_t stream) {
+        hipLaunchKernelGGL((k_gan_bwd<T, VEC, L, NC>), dim3((unsigned)((a.rows + a.rows_per_block - 1) / a.rows_per_block)), dim3(threads_of(L)), 0, stream, a);
+        DM_LAUNCH_CHECK();
+        return DM_OK;
+    }
+};
 
 int check_common(const void* x, const void* h, long long rows, long long item_rows, int C, const void* gate) {
     if (!x || !h || rows < 0 || C <= 0 || item_rows < 0) return DM_ERR_ARG;
@@ -474,7 +504,7 @@ int gan_fwd(const void* x, const void* h, const void* gate, long long item_rows,
     if (pre) { a.pre_g = pre_g; a.pre_b = pre_b; }
     a.rows = rows; a.item_rows = gate ? item_rows : 0; a.C = C; a.scale = scale; a.eps = eps; a.rms = rms;
     DM_ENTER();
-    return dispatch<T, Fwd>(a, chunked(C, Elems<T>::N, {x, h, gate, a.post_g, a.post_b, a.pre_g, a.pre_b, y, z}), 0, stream);
+    return dispatch<T, false, Fwd>(a, chunked(C, Elems<T>::N, {x, h, gate, a.post_g, a.post_b, a.pre_g, a.pre_b, y, z}), stream);
 }
 
 template <typename T>
@@ -501,13 +531,13 @@ int gan_bwd(const void* x, const void* h, const void* gate, long long item_rows,
     if (items > 65000) return DM_ERR_UNSUPPORTED;        // grid.y of the join
     DM_ENTER();
     const bool vec = chunked(C, Elems<T>::N, {x, h, gate, a.post_g, a.post_b, a.pre_g, dy, a.dz, dx, dh});
-    if (int rc = dispatch<T, Bwd>(a, vec, (int)nblk, stream)) return rc;
+    if (int rc = dispatch<T, true, Bwd>(a, vec, stream)) return rc;
     if (a.want) {
         GanReduceArgs r{};
         r.part = ws; r.want = a.want; r.C = C; r.nblk = nblk; r.rows_per_block = a.rows_per_block; r.item_rows = a.item_rows; r.rows = rows;
         r.items = items;
         r.out[0] = dgate; r.out[1] = dpost_g; r.out[2] = dpost_b; r.out[3] = dpre_g; r.out[4] = dpre_b;
-        hipLaunchKernelGGL((k_gan_reduce<T>), dim3((unsigned)((C + 63) / 64), (unsigned)(4 + (a.want & GAN_DGATE ? items : 0))), dim3(256), 0, stream, r);
+        hipLaunchKernelGGL((k_gan_reduce<T>), dim3((unsigned)((C + 31) / 32), (unsigned)(4 + (a.want & GAN_DGATE ? items : 0))), dim3(1024), 0, stream, r);
         DM_LAUNCH_CHECK();
     }
     return DM_OK;

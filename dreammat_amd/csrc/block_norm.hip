@@ -84,18 +84,19 @@ __device__ __forceinline__ void store_chunk(void* p, long long at, const float (
 
 constexpr int threads_of(int L) { return L < 256 ? 256 : L; }
 
-// sum over the L lanes of a row (L >= 256: the whole workgroup, through LDS; every thread of the workgroup must call it)
+// sum over the L lanes of a row (L > 64: several waves, through LDS; every thread of the workgroup must call it)
 template <int L>
 __device__ __forceinline__ float row_sum(float v, float* red) {
 #pragma unroll
     for (int o = (L < 64 ? L : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    if constexpr (L >= 256) {
+    if constexpr (L > 64) {
+        const int w0 = threadIdx.x / L * (L / 64);
         __syncthreads();
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
         __syncthreads();
         v = 0.f;
 #pragma unroll
-        for (int w = 0; w < L / 64; ++w) v += red[w];
+        for (int w = 0; w < L / 64; ++w) v += red[w0 + w];
     }
     return v;
 }
@@ -438,16 +439,26 @@ int dispatch(GanArgs& a, bool vec, hipStream_t stream) {
     constexpr int V = Elems<T>::N;
     if (vec) {
         const int ch = a.C / V;
-        if (ch <= 16) return Launch<T, V, 16, 1>::go(a, stream);
-        if (ch <= 32) return Launch<T, V, 16, 2>::go(a, stream);
-        if (!BWD && ch <= 48) return Launch<T, V, 16, BWD ? 2 : 3>::go(a, stream);
-        if (ch <= 64) return Launch<T, V, 32, 2>::go(a, stream);
-        if (!BWD && ch <= 96) return Launch<T, V, 32, BWD ? 2 : 3>::go(a, stream);
-        if (ch <= 128) return Launch<T, V, 64, 2>::go(a, stream);
-        if (!BWD && ch <= 192) return Launch<T, V, 64, BWD ? 2 : 3>::go(a, stream);
-        if (ch <= 256) return Launch<T, V, 256, 1>::go(a, stream);
-        if (ch <= 512) return Launch<T, V, 256, 2>::go(a, stream);
-        if (ch <= 1024) return Launch<T, V, 512, 2>::go(a, stream);
+        if constexpr (BWD) {
+            if (ch <= 16) return Launch<T, V, 16, 1>::go(a, stream);
+            if (ch <= 32) return Launch<T, V, 32, 1>::go(a, stream);
+            if (ch <= 64) return Launch<T, V, 64, 1>::go(a, stream);
+            if (ch <= 128) return Launch<T, V, 128, 1>::go(a, stream);
+            if (ch <= 256) return Launch<T, V, 256, 1>::go(a, stream);
+            if (ch <= 512) return Launch<T, V, 512, 1>::go(a, stream);
+            if (ch <= 1024) return Launch<T, V, 512, 2>::go(a, stream);
+        } else {
+            if (ch <= 16) return Launch<T, V, 16, 1>::go(a, stream);
+            if (ch <= 32) return Launch<T, V, 16, 2>::go(a, stream);
+            if (ch <= 48) return Launch<T, V, 16, 3>::go(a, stream);
+            if (ch <= 64) return Launch<T, V, 32, 2>::go(a, stream);
+            if (ch <= 96) return Launch<T, V, 32, 3>::go(a, stream);
+            if (ch <= 128) return Launch<T, V, 64, 2>::go(a, stream);
+            if (ch <= 192) return Launch<T, V, 64, 3>::go(a, stream);
+            if (ch <= 256) return Launch<T, V, 256, 1>::go(a, stream);
+            if (ch <= 512) return Launch<T, V, 256, 2>::go(a, stream);
+            if (ch <= 1024) return Launch<T, V, 512, 2>::go(a, stream);
+        }
         if constexpr (V == 4) return Launch<T, V, 512, 4>::go(a, stream);
         return DM_ERR_UNSUPPORTED;
     }

@@ -160,14 +160,11 @@ _SIGS = {
     "dm_softmax_rows_bf16": (c_int, [c_void_p, c_void_p, _LL, c_int, c_float, c_void_p]),
     "dm_softmax_rows_bwd_bf16": (c_int, [c_void_p, c_void_p, c_void_p, _LL, c_int, c_float, c_void_p]),
     "dm_gated_add_norm_workspace_floats": (c_size_t, [_LL, _LL, c_int]),
-    "dm_adapter_u_bytes": (c_size_t, [_LL, c_int]),
-    "dm_adapter_plan_words": (c_size_t, [_LL, _LL, c_int]),
-    "dm_adapter_plan_items": (_LL, [_LL, c_int, c_int]),
-    "dm_adapter_plan": (c_int, [c_void_p, c_void_p, _LL, _LL, c_int, c_int, c_void_p, c_void_p]),
-    "dm_linear_adapted_bf16": (c_int, [c_void_p] * 6 + [c_int, c_void_p, c_void_p, _LL, c_float, c_void_p, c_size_t, c_void_p, _LL]
-                               + [c_int] * 5 + [c_void_p]),
-    "dm_adapter_layout_bf16": (c_int, [c_void_p, c_void_p] + [c_int] * 4 + [c_void_p]),
-    "dm_adapter_wgrad_bf16": (c_int, [c_void_p] * 3 + [_LL, _LL] + [c_int] * 5 + [c_void_p, c_size_t, c_void_p, c_void_p]),
+    "dm_linear_adapted_workspace_bytes": (c_size_t, [_LL, c_int, c_int, c_int]),
+    "dm_linear_adapted_bf16": (c_int, [c_void_p] * 8 + [_LL, c_float, c_void_p, c_size_t, c_void_p, _LL] + [c_int] * 5 + [c_void_p]),
+    "dm_linear_adapted_bwd_workspace_bytes": (c_size_t, [_LL, c_int, c_int, c_int, c_int, _LL]),
+    "dm_linear_adapted_bwd_bf16": (c_int, [c_void_p] * 7 + [_LL, c_float, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p, c_void_p, _LL]
+                                   + [c_int] * 4 + [c_void_p]),
     "dm_orthogonalize_workspace_bytes": (c_size_t, [c_int] * 3),
     "dm_orthogonalize": (c_int, [c_void_p, c_void_p] + [c_int] * 5 + [c_float, c_void_p, c_size_t, c_void_p]),
     "dm_muon_step": (c_int, [c_void_p] * 3 + [c_int] * 5 + [c_float, c_int, c_float, c_float, c_float, c_void_p, c_size_t, c_void_p]),
@@ -181,7 +178,7 @@ for _n in ("dm_attention_fwd_bf16", "dm_attention_fwd_lse_bf16", "dm_conv3x3_nhw
            "dm_conv2x2_nhwc_bf16", "dm_conv2x2_subpixel_nhwc_bf16", "dm_conv3x3_small_nhwc_bf16", "dm_conv3x3_small_res_nhwc_bf16", "dm_gemm_bf16_fused", "dm_gemm_bf16_batched",
            "dm_layernorm_bf16", "dm_geglu_bf16", "dm_cat_add_bf16", "dm_softmax_rows_bf16", "dm_softmax_rows_bwd_bf16",
            "dm_conv3x3_gn_nhwc_bf16_fused", "dm_linear_small_bf16", "dm_transpose_bf16",
-           "dm_linear_adapted_bf16", "dm_adapter_layout_bf16", "dm_adapter_wgrad_bf16"):
+           "dm_linear_adapted_bf16", "dm_linear_adapted_bwd_bf16"):
     _SIGS[_n.replace("bf16", "f16")] = _SIGS[_n]
 for _n in ("dm_groupnorm_nhwc_fwd", "dm_groupnorm_nhwc_infer", "dm_groupnorm_nhwc_bwd", "dm_groupnorm_nhwc_bwd_res", "dm_groupnorm_nhwc_stats"):
     _SIGS[_n + "_f16"] = _SIGS[_n]

@@ -8,7 +8,7 @@
 // Three kernels:
 //   shrink  u = s x A_e^T, one pass over x; u is kept as a PAIR of 16-bit numbers (value and remainder: 16-22 significant bits), so
 //           the second product loses nothing against fp32 and still runs on the 16-bit matrix pipe.  In half precision a row is
-//           scaled by a power of two first (its largest entry near 2^8): half's exponent range must not bound u.
+//           scaled by a power of two where its largest entry leaves [2^-3, 2^14): half's exponent range must not bound u.
 //   expand  the big product, its K loop extended by [u_value | u_rest] [B | B]^T: the low-rank product costs 2 ceil(R/16) 16
 //           columns of K and no pass over y.  Rows of a tile that belong to another adapter are left out by selection (never by
 //           a multiplication with zero: 0 * inf of another request's adapter would reach them).
@@ -16,6 +16,7 @@
 //           a fixed order (no atomics).
 // The data gradient is the same pair of kernels on (dy, W^T, B^T, A^T): dx = dy W + (s dy B_e) A_e.
 #include <algorithm>
+#include <type_traits>
 
 #include "dm_common.h"
 #include "dm_elem.h"
@@ -56,8 +57,8 @@ __device__ __forceinline__ int adapter_of(const Rows& r, long long m) {
 
 __device__ __forceinline__ float pow2_scale(float biggest) {
 #if defined(DM_F16)
-    // 2^k with |u| / 2^k in [2^8, 2^9): half's value and remainder both stay normal; 1 for a row of zeros, infinities or NaN
-    if (!(biggest > 0.f) || biggest > 3.0e38f) return 1.f;
+    // 1 where half holds the row's largest entry with a normal remainder (and for zeros, infinities, NaN), else 2^k that brings it to [2^8, 2^9)
+    if (!(biggest > 0.f) || biggest > 3.0e38f || (biggest >= 0.125f && biggest < 16384.f)) return 1.f;
     int e;
     frexpf(biggest, &e);
     return ldexpf(1.f, min(max(e - 9, -100), 100));
@@ -74,8 +75,24 @@ __device__ __forceinline__ void store_pair(elem_t* u, int Rp, int r, float v) {
     u[Rp + r] = (elem_t)(v - (float)hi);
 }
 
+// the smallest entry of a tile's adapters above cur (INT_MAX: none), the same in every wave
+template <int TR>
+__device__ __forceinline__ int next_adapter(const int* aid, int cur) {
+    const int lane = threadIdx.x & 63;
+    int next = 0x7fffffff;
+#pragma unroll
+    for (int t = 0; t < (TR + 63) / 64; ++t) {
+        const int v = aid[(64 * t + lane) % TR];
+        next = v > cur && v < next ? v : next;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) next = min(next, __shfl_xor(next, o, 64));
+    return __builtin_amdgcn_readfirstlane(next);
+}
+
 // Tile of 16 RT rows; the four waves take 64-wide slices of K in turn, so a tile reads its x rows once (128-byte lines) and the rank
-// rows of A once from L2; the partial products meet in LDS.  One pass per adapter that occurs in the tile.  Bound by the x read.
+// rows of A once from L2; a slice is requested before the last one is multiplied; the partial products meet in LDS.  One pass per adapter
+// that occurs in the tile.  Bound by the x read.
 template <int RT, int NR>
 __global__ __launch_bounds__(256) void k_shrink(const elem_t* __restrict__ x, const elem_t* __restrict__ A, Rows rows, int K, int R, float scale,
                                                 elem_t* __restrict__ u, float* __restrict__ us) {
@@ -91,37 +108,48 @@ __global__ __launch_bounds__(256) void k_shrink(const elem_t* __restrict__ x, co
     for (int t = 0; t < RT; ++t) xr[t] = x + min(m0 + 16 * t + l15, rows.M - 1) * K + 8 * kq;
     int cur = kNone;
     for (;;) {
-        int next = 0x7fffffff;                              // the next adapter of the tile, found by every thread alike
-        for (int t = 0; t < TR; ++t) {
-            const int v = aid[t];
-            next = v > cur && v < next ? v : next;
-        }
-        if (next == 0x7fffffff) break;
-        cur = next;
-        const elem_t* ar = A + (long long)cur * R * K + 8 * kq;
+        cur = next_adapter<TR>(aid, cur);
+        if (cur == 0x7fffffff) break;
+        const elem_t* ar[NR];
+#pragma unroll
+        for (int q = 0; q < NR; ++q) ar[q] = A + ((long long)cur * R + min(16 * q + l15, R - 1)) * K + 8 * kq;
         f32x4 acc[RT][NR];
 #pragma unroll
         for (int t = 0; t < RT; ++t)
 #pragma unroll
             for (int q = 0; q < NR; ++q) acc[t][q] = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (int k0 = 64 * wave; k0 < K; k0 += 256) {
-            elem8 xf[2][RT], af[2][NR];
+        struct Slice { elem8 x[2][RT], a[2][NR]; };
+        auto load = [&](int k0, Slice& f) __attribute__((always_inline)) {
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 const int k = k0 + 32 * s;
                 const bool ok = k + 8 * kq < K;
                 const elem8 zero = {};
 #pragma unroll
-                for (int t = 0; t < RT; ++t) xf[s][t] = ok ? *reinterpret_cast<const elem8*>(xr[t] + k) : zero;
+                for (int t = 0; t < RT; ++t) f.x[s][t] = ok ? *reinterpret_cast<const elem8*>(xr[t] + k) : zero;
 #pragma unroll
-                for (int q = 0; q < NR; ++q) af[s][q] = ok ? *reinterpret_cast<const elem8*>(ar + (long long)min(16 * q + l15, R - 1) * K + k) : zero;
+                for (int q = 0; q < NR; ++q) f.a[s][q] = ok ? *reinterpret_cast<const elem8*>(ar[q] + k) : zero;
             }
+        };
+        auto mul = [&](const Slice& f) __attribute__((always_inline)) {
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
                 for (int t = 0; t < RT; ++t)
 #pragma unroll
-                    for (int q = 0; q < NR; ++q) acc[t][q] = DM_MFMA_16x16x32(xf[s][t], af[s][q], acc[t][q]);
+                    for (int q = 0; q < NR; ++q) acc[t][q] = DM_MFMA_16x16x32(f.x[s][t], f.a[s][q], acc[t][q]);
+        };
+        Slice f0, f1;
+        int k0 = 64 * wave;
+        if (k0 < K) load(k0, f0);
+        while (k0 < K) {
+            if (k0 + 256 < K) load(k0 + 256, f1);
+            mul(f0);
+            k0 += 256;
+            if (k0 >= K) break;
+            if (k0 + 256 < K) load(k0 + 256, f0);
+            mul(f1);
+            k0 += 256;
         }
         // lane: rank 16 q + l15, rows 4 kq + i
 #pragma unroll
@@ -154,6 +182,99 @@ __global__ __launch_bounds__(256) void k_shrink(const elem_t* __restrict__ x, co
         }
         __syncthreads();
     }
+}
+
+// The same for many rows: tiles of 64 rows, x and the rank rows through a ring of LDS stages (buffer_load ... lds, whole 128-byte lines,
+// three stages in flight), a wave 16 rows.  Against the kernel above, whose fragments are gathered from 16 rows by every load: rank 64 of
+// [24576, 5120] 187 -> 66 us.
+template <int NR>
+__global__ __launch_bounds__(256) void k_shrink_ring(const elem_t* __restrict__ x, const elem_t* __restrict__ A, Rows rows, int K, int R, float scale,
+                                                     elem_t* __restrict__ u, float* __restrict__ us) {
+    [[maybe_unused]] constexpr int Rp = 16 * NR, ROWB = 128, STAGE = (64 + Rp) * ROWB, NST = 4, PA = Rp >= 32 ? Rp / 32 : 1;
+    extern __shared__ __attribute__((aligned(16))) char smem[];      // NST STAGE | int aid[64]
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr unsigned OOB = 0x80000000u;
+    int* aid = reinterpret_cast<int*>(smem + NST * STAGE);
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l15 = lane & 15, kq = lane >> 4;
+    const long long m0 = (long long)blockIdx.x * 64;
+    const int mrows = (int)min(64LL, rows.M - m0), steps = (K + 63) / 64;
+    const __amdgpu_buffer_rsrc_t xrs = __builtin_amdgcn_make_buffer_rsrc((void*)(x + m0 * K), 0, mrows * K * 2, 0x00020000);
+    // x pieces: rows 16 wave + 8 i; rank pieces: rows 8 p of A (with 16 ranks two waves fetch each piece)
+    auto chunk_of = [&](int row) __attribute__((always_inline)) { return (unsigned)(((lane & 7) ^ ((row >> 1) & 7)) * 8); };
+    if (tid < 64) aid[tid] = adapter_of(rows, m0 + tid);
+    __syncthreads();
+    int cur = kNone;
+    for (;;) {
+        cur = next_adapter<64>(aid, cur);
+        if (cur == 0x7fffffff) break;
+        const __amdgpu_buffer_rsrc_t ars = __builtin_amdgcn_make_buffer_rsrc((void*)(A + (long long)cur * R * K), 0, R * K * 2, 0x00020000);
+        auto issue = [&](int s, int stage) __attribute__((always_inline)) {
+            char* base = smem + stage * STAGE;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int row = 16 * wave + 8 * i + (lane >> 3);
+                const unsigned k = (unsigned)(s * 64) + chunk_of(row);
+                const unsigned off = row < mrows && k < (unsigned)K ? ((unsigned)row * (unsigned)K + k) * 2u : OOB;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(xrs, (__attribute__((address_space(3))) void*)(base + (16 * wave + 8 * i) * ROWB), 16, (int)off, 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < PA; ++i) {
+                const int p = (PA * wave + i) % (Rp / 8), row = 8 * p + (lane >> 3);
+                const unsigned k = (unsigned)(s * 64) + chunk_of(row);
+                const unsigned off = row < R && k < (unsigned)K ? ((unsigned)row * (unsigned)K + k) * 2u : OOB;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(ars, (__attribute__((address_space(3))) void*)(base + (64 + 8 * p) * ROWB), 16, (int)off, 0, 0, 0);
+            }
+        };
+        f32x4 acc[NR];
+#pragma unroll
+        for (int q = 0; q < NR; ++q) acc[q] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int q = 0; q < NST - 1; ++q)
+            if (q < steps) issue(q, q);
+        int stage = 0;
+        for (int s = 0; s < steps; ++s) {
+            if (s + NST - 2 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 2) * (2 + PA)) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            if (s + NST - 1 < steps) issue(s + NST - 1, stage == 0 ? NST - 1 : stage - 1);
+            const char* xb = smem + stage * STAGE;
+            const char* ab = xb + 64 * ROWB;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                auto frag = [&](const char* base, int row) __attribute__((always_inline)) {
+                    return *reinterpret_cast<const elem8*>(base + row * ROWB + (((4 * h + kq) ^ ((row >> 1) & 7)) << 4));
+                };
+                const elem8 xf = frag(xb, 16 * wave + l15);
+#pragma unroll
+                for (int q = 0; q < NR; ++q) acc[q] = DM_MFMA_16x16x32(xf, frag(ab, 16 * q + l15), acc[q]);
+            }
+            stage = stage + 1 == NST ? 0 : stage + 1;
+        }
+        // lane: rank 16 q + l15, rows 4 kq + i of the wave's 16
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int t = 16 * wave + 4 * kq + i;
+            float v[NR], big = 0.f;
+#pragma unroll
+            for (int q = 0; q < NR; ++q) {
+                v[q] = 16 * q + l15 < R ? scale * acc[q][i] : 0.f;
+                big = fmaxf(big, fabsf(v[q]));
+            }
+#if defined(DM_F16)
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor(big, o, 16));
+#endif
+            if (aid[t] == cur) {
+                const float p = pow2_scale(big);
+#pragma unroll
+                for (int q = 0; q < NR; ++q) store_pair(u + (m0 + t) * 2 * Rp, Rp, 16 * q + l15, v[q] / p);
+                if (l15 == 0) us[m0 + t] = p;
+            }
+        }
+        __syncthreads();                                             // the stages are free for the next adapter
+    }
+#endif
 }
 
 // One row per blockIdx.x, one rank row per wave: requests of a few rows each, where a tile would hold many adapters.  Every row reads
@@ -197,64 +318,73 @@ struct ExpandArgs {
     elem_t* y;
     Rows rows;
     int K, N, R, ldb;      // ldb: elements between the rows of B (a multiple of 8)
-    int n_nt, tiles;
+    int n_mt, n_nt, tiles;
 };
 
-// BM x BN x 64 tile, WM x WN waves of 64 x 64, two LDS stages filled by buffer_load ... lds (16 bytes per lane, range-checked: rows and
+// BM x BN x 64 tile, WM x WN waves, NST LDS stages filled by buffer_load ... lds (16 bytes per lane, range-checked: rows and
 // columns past the end read as zeros).  LDS rows are 128 bytes, the 16-byte chunks XOR-swizzled by (row >> 1) & 7 at the source address
 // and at the fragment read: conflict-free without padding.  The weights are the matrix instruction's A operand, so a lane holds one row
 // of y and four consecutive columns per register group: 16-byte stores after one exchange between the wave's halves.
-template <int BM, int BN, int WM, int WN>
+template <int BM, int BN, int WM, int WN, int NST>
 __global__ __launch_bounds__(WM * WN * 64) void k_expand(ExpandArgs a) {
     [[maybe_unused]] constexpr int NW = WM * WN, ROWB = 128;
     [[maybe_unused]] constexpr int TM = BM / WM, TN = BN / WN, MT = TM / 32, NT = TN / 32;
     [[maybe_unused]] constexpr int A_BYTES = BM * ROWB, STAGE = (BM + BN) * ROWB;
     [[maybe_unused]] constexpr int AP = BM / 8 / NW, BP = BN / 8 / NW;                // 1 KB pieces (8 rows) per wave
-    extern __shared__ __attribute__((aligned(16))) char smem[];      // 2 STAGE | int aid[BM]
+    extern __shared__ __attribute__((aligned(16))) char smem[];      // NST STAGE | int aid[BM] | float scale_of[BM] | float bias_of[BN]
 #if defined(__HIP_DEVICE_COMPILE__)
-    constexpr unsigned OOB = 0xfffffff0u;
-    int* aid = reinterpret_cast<int*>(smem + 2 * STAGE);
+    constexpr unsigned OOB = 0x80000000u;             // past every descriptor, also with a step's scalar offset on top
+    int* aid = reinterpret_cast<int*>(smem + NST * STAGE);
+    float* scale_of = reinterpret_cast<float*>(aid + BM);
+    float* bias_of = scale_of + BM;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, hi = lane >> 5, l31 = lane & 31;
     const int wm = wave / WN, wn = wave % WN;
-    // block b runs on XCD b % 8 (its own L2): each XCD gets a contiguous run of tiles, the N tiles of one row panel side by side
+    // block b runs on XCD b % 8 (its own L2): each XCD gets a contiguous run of tiles, walked in bands of eight row panels (the
+    // tiles that run together then share their panels: [24576, 5120, 1280] 418 -> 354 us on 128 tiles against whole rows of tiles)
     const int per = (a.tiles + 7) / 8, id = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
     if ((int)(blockIdx.x >> 3) >= per || id >= a.tiles) return;
-    const long long m0 = (long long)(id / a.n_nt) * BM;
-    const int n0 = id % a.n_nt * BN;
+    constexpr int BAND = 8;
+    const int band = id / (BAND * a.n_nt), in_band = id - band * BAND * a.n_nt, height = min(BAND, a.n_mt - band * BAND);
+    const long long m0 = (long long)(band * BAND + in_band % height) * BM;
+    const int n0 = in_band / height * BN;
     const int mrows = (int)min((long long)BM, a.rows.M - m0), nrows = min(BN, a.N - n0);
     const int K = a.K, Rp = rank_pad(a.R);
 
-    const int lrow = lane >> 3, slot = lane & 7;
-    unsigned a_off[AP], b_off[BP], a_chunk[AP], b_chunk[BP];
+    // this lane's 16 bytes of piece i: row wave * (rows / NW) + 8 i + lane / 8, chunk (lane % 8) ^ ((row >> 1) & 7)
+    auto row_of = [&](int i, int rows) __attribute__((always_inline)) { return wave * (rows / NW) + 8 * i + (lane >> 3); };
+    auto chunk_of = [&](int row) __attribute__((always_inline)) { return (unsigned)(((lane & 7) ^ ((row >> 1) & 7)) * 8); };
+    unsigned a_off[AP], b_off[BP];
 #pragma unroll
     for (int i = 0; i < AP; ++i) {
-        const int row = wave * (BM / NW) + 8 * i + lrow;
-        a_chunk[i] = (unsigned)((slot ^ ((row >> 1) & 7)) * 8);
-        a_off[i] = row < mrows ? (unsigned)row : OOB;
+        const int row = row_of(i, BM);
+        a_off[i] = row < mrows ? ((unsigned)row * (unsigned)K + chunk_of(row)) * 2u : OOB;
     }
 #pragma unroll
     for (int i = 0; i < BP; ++i) {
-        const int row = wave * (BN / NW) + 8 * i + lrow;
-        b_chunk[i] = (unsigned)((slot ^ ((row >> 1) & 7)) * 8);
-        b_off[i] = row < nrows ? (unsigned)row : OOB;
+        const int row = row_of(i, BN);
+        b_off[i] = row < nrows ? ((unsigned)row * (unsigned)K + chunk_of(row)) * 2u : OOB;
     }
     const __amdgpu_buffer_rsrc_t xrs = __builtin_amdgcn_make_buffer_rsrc((void*)(a.x + m0 * K), 0, mrows * K * 2, 0x00020000);
     const __amdgpu_buffer_rsrc_t wrs = __builtin_amdgcn_make_buffer_rsrc((void*)(a.w + (long long)n0 * K), 0, nrows * K * 2, 0x00020000);
     const __amdgpu_buffer_rsrc_t urs = __builtin_amdgcn_make_buffer_rsrc((void*)(a.u + m0 * 2 * Rp), 0, mrows * 2 * Rp * 2, 0x00020000);
 
+    auto to_lds = [&](const __amdgpu_buffer_rsrc_t rs, char* to, unsigned off, int soff) __attribute__((always_inline)) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)to, 16, (int)off, soff, 0, 0);
+    };
     auto issue_main = [&](int s, int stage) __attribute__((always_inline)) {
         char* base = smem + stage * STAGE;
+        const bool ragged = s * 64 + 64 > K;                         // (uniform) the last step of a K that is not whole
 #pragma unroll
         for (int i = 0; i < AP; ++i) {
-            const unsigned k = (unsigned)(s * 64) + a_chunk[i];
-            const unsigned off = a_off[i] != OOB && k < (unsigned)K ? (a_off[i] * (unsigned)K + k) * 2u : OOB;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(xrs, (__attribute__((address_space(3))) void*)(base + (wave * (BM / NW) + 8 * i) * ROWB), 16, (int)off, 0, 0, 0);
+            unsigned off = a_off[i];
+            if (ragged && (unsigned)(s * 64) + chunk_of(row_of(i, BM)) >= (unsigned)K) off = OOB;
+            to_lds(xrs, base + (wave * (BM / NW) + 8 * i) * ROWB, off, s * 128);
         }
 #pragma unroll
         for (int i = 0; i < BP; ++i) {
-            const unsigned k = (unsigned)(s * 64) + b_chunk[i];
-            const unsigned off = b_off[i] != OOB && k < (unsigned)K ? (b_off[i] * (unsigned)K + k) * 2u : OOB;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(wrs, (__attribute__((address_space(3))) void*)(base + A_BYTES + (wave * (BN / NW) + 8 * i) * ROWB), 16, (int)off, 0, 0, 0);
+            unsigned off = b_off[i];
+            if (ragged && (unsigned)(s * 64) + chunk_of(row_of(i, BN)) >= (unsigned)K) off = OOB;
+            to_lds(wrs, base + A_BYTES + (wave * (BN / NW) + 8 * i) * ROWB, off, s * 128);
         }
     };
     // columns [c0, c0 + 64) of [u_value | u_rest] against the same columns of [B_e | B_e]
@@ -263,42 +393,56 @@ __global__ __launch_bounds__(WM * WN * 64) void k_expand(ExpandArgs a) {
         const __amdgpu_buffer_rsrc_t brs = __builtin_amdgcn_make_buffer_rsrc((void*)(a.B + ((long long)e * a.N + n0) * a.ldb), 0, nrows * a.ldb * 2, 0x00020000);
 #pragma unroll
         for (int i = 0; i < AP; ++i) {
-            const unsigned c = (unsigned)c0 + a_chunk[i];
-            const unsigned off = a_off[i] != OOB && c < (unsigned)(2 * Rp) ? (a_off[i] * (unsigned)(2 * Rp) + c) * 2u : OOB;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(urs, (__attribute__((address_space(3))) void*)(base + (wave * (BM / NW) + 8 * i) * ROWB), 16, (int)off, 0, 0, 0);
+            const int row = row_of(i, BM);
+            const unsigned c = (unsigned)c0 + chunk_of(row);
+            to_lds(urs, base + (wave * (BM / NW) + 8 * i) * ROWB, row < mrows && c < (unsigned)(2 * Rp) ? ((unsigned)row * (unsigned)(2 * Rp) + c) * 2u : OOB, 0);
         }
 #pragma unroll
         for (int i = 0; i < BP; ++i) {
-            const unsigned c = (unsigned)c0 + b_chunk[i], r = c >= (unsigned)Rp ? c - (unsigned)Rp : c;
-            const unsigned off = b_off[i] != OOB && c < (unsigned)(2 * Rp) && r < (unsigned)a.R ? (b_off[i] * (unsigned)a.ldb + r) * 2u : OOB;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(brs, (__attribute__((address_space(3))) void*)(base + A_BYTES + (wave * (BN / NW) + 8 * i) * ROWB), 16, (int)off, 0, 0, 0);
+            const int row = row_of(i, BN);
+            const unsigned c = (unsigned)c0 + chunk_of(row), r = c >= (unsigned)Rp ? c - (unsigned)Rp : c;
+            to_lds(brs, base + A_BYTES + (wave * (BN / NW) + 8 * i) * ROWB,
+                   row < nrows && c < (unsigned)(2 * Rp) && r < (unsigned)a.R ? ((unsigned)row * (unsigned)a.ldb + r) * 2u : OOB, 0);
         }
     };
 
-    issue_main(0, 0);
-    for (int t = tid; t < BM; t += NW * 64) aid[t] = adapter_of(a.rows, m0 + t);
-    __syncthreads();
-    int my_aid[MT];
-    float my_us[MT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const int row = TM * wm + 32 * i + l31;
-        my_aid[i] = aid[row];
-        my_us[i] = my_aid[i] != kNone ? a.us[m0 + row] : 0.f;
+    // Steps run 0 .. steps - 1 over K, then the low-rank columns of the tile's adapters in ascending order.  `issue` requests the next
+    // one (NST - 1 ahead of the one being multiplied) and returns whether there was one.
+    const int steps = (K + 63) / 64;
+    int i_step = 0, i_stage = 0, i_e = kNone, i_c0 = 2 * Rp;
+    auto issue = [&]() __attribute__((always_inline)) {
+        if (i_step < steps) issue_main(i_step, i_stage);
+        else {
+            if (i_c0 >= 2 * Rp) {
+                if (i_e == 0x7fffffff) return false;
+                i_e = next_adapter<BM>(aid, i_e);
+                i_c0 = 0;
+                if (i_e == 0x7fffffff) { i_c0 = 2 * Rp; return false; }
+            }
+            issue_low(i_e, i_c0, i_stage);
+            i_c0 += 64;
+        }
+        ++i_step;
+        i_stage = i_stage + 1 == NST ? 0 : i_stage + 1;
+        return true;
+    };
+    issue();                                                         // (the first step of K)
+    int ahead = 1, plain = 1;
+    for (int t = tid; t < BM; t += NW * 64) {
+        const int e = adapter_of(a.rows, m0 + t);
+        aid[t] = e;
+        scale_of[t] = e != kNone ? a.us[m0 + t] : 1.f;
+        if (scale_of[t] != 1.f) plain = 0;
     }
-    // the tile's adapters in ascending order: every wave finds the next one for itself
-    auto next_adapter = [&](int cur) __attribute__((always_inline)) {
-        int next = 0x7fffffff;
+    for (int t = tid; t < BN; t += NW * 64) bias_of[t] = a.bias && n0 + t < a.N ? (float)a.bias[n0 + t] : 0.f;
+    plain = __syncthreads_and(plain);
 #pragma unroll
-        for (int t = 0; t < BM / 64; ++t) {
-            const int v = aid[64 * t + lane];
-            next = v > cur && v < next ? v : next;
-        }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) next = min(next, __shfl_xor(next, o, 64));
-        return __builtin_amdgcn_readfirstlane(next);
-    };
-
+    for (int q = 1; q < NST - 1; ++q) ahead += issue();
+    // A tile of one adapter without row scales (nearly all: a request is longer than a tile): its low-rank columns are K steps like others
+    const int only = next_adapter<BM>(aid, kNone);
+    int others = 0;
+    for (int t = lane; t < mrows; t += 64) others |= aid[t] != only;
+    const bool uniform = plain && only != 0x7fffffff && !__any(others);
     f32x16 acc[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -310,14 +454,20 @@ __global__ __launch_bounds__(WM * WN * 64) void k_expand(ExpandArgs a) {
     auto frag = [&](const char* base, int row, int kk) __attribute__((always_inline)) {
         return *reinterpret_cast<const elem8*>(base + row * ROWB + (((2 * kk + hi) ^ ((row >> 1) & 7)) << 4));
     };
-    const int steps = (K + 63) / 64;
-    int e = next_adapter(kNone);                    // adapter of the low-rank step to issue next (INT_MAX: none left)
-    for (int s = 0; s < steps; ++s) {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    int stage = 0;
+    // waits until the step to multiply has landed (at most the younger NST - 2 steps' pieces stay in flight), then requests another one
+    auto advance = [&]() __attribute__((always_inline)) {
+        if (NST > 2 && ahead == NST - 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 2) * (AP + BP)) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
-        if (s + 1 < steps) issue_main(s + 1, (s + 1) & 1);
-        else if (e != 0x7fffffff) issue_low(e, 0, (s + 1) & 1);
-        const char* ab = smem + (s & 1) * STAGE;
+        asm volatile("" ::: "memory");
+        --ahead;
+        ahead += issue();
+    };
+    const int low = (2 * Rp + 63) / 64, last = uniform ? steps + low : steps;
+    for (int s = 0; s < last; ++s) {
+        advance();
+        const char* ab = smem + stage * STAGE;
         const char* bb = ab + A_BYTES;
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
@@ -331,71 +481,77 @@ __global__ __launch_bounds__(WM * WN * 64) void k_expand(ExpandArgs a) {
 #pragma unroll
                 for (int j = 0; j < NT; ++j) acc[i][j] = DM_MFMA_32x32x16(bf[j], af[i], acc[i][j]);
         }
+        stage = stage + 1 == NST ? 0 : stage + 1;
     }
-    int s = steps, c0 = 0;
+    int e = uniform ? 0x7fffffff : only, c0 = 0;
     while (e != 0x7fffffff) {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        const int cur = e, cols = min(64, 2 * Rp - c0);
-        c0 += 64;
-        if (c0 >= 2 * Rp) { c0 = 0; e = next_adapter(e); }
-        if (e != 0x7fffffff) issue_low(e, c0, (s + 1) & 1);
-        const char* ab = smem + (s & 1) * STAGE;
+        advance();
+        const char* ab = smem + stage * STAGE;
         const char* bb = ab + A_BYTES;
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-            const bool mine = my_aid[i] == cur;
+            const int row = TM * wm + 32 * i + l31;
+            const bool mine = aid[row] == e;
+            const float scale = scale_of[row];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 f32x16 t;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) t[r] = 0.f;
-                for (int kk = 0; 16 * kk < cols; ++kk)
-                    t = DM_MFMA_32x32x16(frag(bb, TN * wn + 32 * j + l31, kk), frag(ab, TM * wm + 32 * i + l31, kk), t);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) acc[i][j][r] += mine ? t[r] * my_us[i] : 0.f;
+                for (int kk = 0; kk < 4; ++kk)                       // (columns past 2 Rp are zeros)
+                    t = DM_MFMA_32x32x16(frag(bb, TN * wn + 32 * j + l31, kk), frag(ab, row, kk), t);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[i][j][r] += mine ? t[r] * scale : 0.f;
+                __builtin_amdgcn_sched_barrier(0);                   // one fragment at a time: the accumulators leave no registers for more
             }
         }
-        ++s;
+        stage = stage + 1 == NST ? 0 : stage + 1;
+        c0 += 64;
+        if (c0 >= 2 * Rp) { c0 = 0; e = next_adapter<BM>(aid, e); }
     }
 
-    // one rounding: y = acc + bias + residual
+    // one rounding: y = acc + bias + residual.  Registers 4 g + r hold columns 8 g + 4 hi + r; exchanging group 2 gp + 1 of the lower lanes with
+    // group 2 gp of the upper ones leaves lanes 0-31 with columns 16 gp .. + 7 of their row, lanes 32-63 with 16 gp + 8 .. + 15.
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
         const long long m = m0 + TM * wm + 32 * i + l31;
         const bool m_ok = m < a.rows.M;
+        elem8 res[NT][2];
+        if (a.res) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int gp = 0; gp < 2; ++gp) {
+                    const int n = n0 + TN * wn + 32 * j + 16 * gp + 8 * hi;
+                    res[j][gp] = elem8{};
+                    if (m_ok && n < a.N) res[j][gp] = *reinterpret_cast<const elem8*>(a.res + m * a.N + n);
+                }
+        }
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int gp = 0; gp < 2; ++gp) {
-                unsigned pk[2][2];
+                const int col = TN * wn + 32 * j + 16 * gp + 8 * hi, n = n0 + col;
+                float v[8];
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const int g = 2 * gp + q, n = n0 + TN * wn + 32 * j + 8 * g + 4 * hi;      // this lane's four columns
-                    float v[4];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) v[r] = acc[i][j][4 * g + r];
-                    if (a.bias && n < a.N) {
-                        const elem4 bv = *reinterpret_cast<const elem4*>(a.bias + n);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) v[r] += (float)bv[r];
-                    }
-                    if (a.res && n < a.N && m_ok) {
-                        const elem4 rv = *reinterpret_cast<const elem4*>(a.res + m * a.N + n);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) v[r] += (float)rv[r];
-                    }
-                    const elem4 o = {(elem_t)v[0], (elem_t)v[1], (elem_t)v[2], (elem_t)v[3]};
-                    const u32x2 w2 = __builtin_bit_cast(u32x2, o);
-                    pk[q][0] = w2[0];
-                    pk[q][1] = w2[1];
+                for (int r = 0; r < 4; ++r) {
+                    const float p = acc[i][j][8 * gp + r], q = acc[i][j][8 * gp + 4 + r];
+                    const auto sw = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, p), __builtin_bit_cast(unsigned, q), false, false);
+                    const unsigned w0 = sw[0], w1 = sw[1];           // (a bit cast of a vector's element would take its first)
+                    v[r] = __builtin_bit_cast(float, w0);
+                    v[4 + r] = __builtin_bit_cast(float, w1);
                 }
-                // lanes 0-31 get columns 16 gp .. + 7 of their row, lanes 32-63 columns 16 gp + 8 .. + 15
-                const auto s0 = __builtin_amdgcn_permlane32_swap(pk[0][0], pk[1][0], false, false);
-                const auto s1 = __builtin_amdgcn_permlane32_swap(pk[0][1], pk[1][1], false, false);
-                const u32x4 out = {s0[0], s1[0], s0[1], s1[1]};
-                const int n = n0 + TN * wn + 32 * j + 16 * gp + 8 * hi;
-                if (m_ok && n < a.N) *reinterpret_cast<u32x4*>(a.y + m * a.N + n) = out;
+                const float4 b0 = *reinterpret_cast<const float4*>(bias_of + col), b1 = *reinterpret_cast<const float4*>(bias_of + col + 4);
+                v[0] += b0.x; v[1] += b0.y; v[2] += b0.z; v[3] += b0.w;
+                v[4] += b1.x; v[5] += b1.y; v[6] += b1.z; v[7] += b1.w;
+                if (a.res)
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) v[r] += (float)res[j][gp][r];
+                elem8 o;
+#pragma unroll
+                for (int r = 0; r < 8; ++r) o[r] = (elem_t)v[r];
+                if (m_ok && n < a.N) *reinterpret_cast<elem8*>(a.y + m * a.N + n) = o;
             }
     }
 #endif
@@ -416,15 +572,21 @@ __global__ __launch_bounds__(512) void k_expand_skinny(ExpandArgs a, const float
     const elem_t* xr[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) xr[t] = a.x + (long long)min(16 * t + l15, M - 1) * K + 8 * kq;
-    for (int k = 32 * wave; k < K; k += 256) {
-        const bool ok = k + 8 * kq < K;
+    for (int k0 = 32 * wave; k0 < K; k0 += 256 * 5) {            // five slices requested at once
+        elem8 wf[5], xf[MT][5];
         const elem8 zero = {};
-        const elem8 wf = ok ? *reinterpret_cast<const elem8*>(wr + k) : zero;
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            const elem8 xf = ok ? *reinterpret_cast<const elem8*>(xr[t] + k) : zero;
-            acc[t] = DM_MFMA_16x16x32(xf, wf, acc[t]);
+        for (int q = 0; q < 5; ++q) {
+            const int k = k0 + 256 * q;
+            const bool ok = k + 8 * kq < K;
+            wf[q] = ok ? *reinterpret_cast<const elem8*>(wr + k) : zero;
+#pragma unroll
+            for (int t = 0; t < MT; ++t) xf[t][q] = ok ? *reinterpret_cast<const elem8*>(xr[t] + k) : zero;
         }
+#pragma unroll
+        for (int q = 0; q < 5; ++q)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[t] = DM_MFMA_16x16x32(xf[t][q], wf[q], acc[t]);
     }
 #pragma unroll
     for (int t = 0; t < MT; ++t)
@@ -457,32 +619,38 @@ __global__ __launch_bounds__(512) void k_expand_skinny(ExpandArgs a, const float
 }
 
 // ------------------------------------------------------------------------------------------------ layouts of the adapters
-// dst[e][c][0 .. Rp) = src[e][0 .. R)[c] (transpose: A^T from A; src [E, R, C]) or src[e][c][0 .. R) (copy: B into padded rows, src
-// [E, C, R]); columns past R are zero.  32 x 32 tiles through LDS; blockIdx = (column tile, rank tile, adapter).
-__global__ __launch_bounds__(256) void k_adapter_rows(const elem_t* __restrict__ src, elem_t* __restrict__ dst, int C, int R, int Rp, int transpose) {
-    __shared__ elem_t tile[32][34];
-    const int c0 = blockIdx.x * 32, r0 = blockIdx.y * 32, tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const elem_t* s = src + (long long)blockIdx.z * R * C;
-    elem_t* d = dst + (long long)blockIdx.z * C * Rp;
-    if (transpose) {
-        for (int r = ty; r < 32; r += 8) tile[r][tx] = r0 + r < R && c0 + tx < C ? s[(long long)(r0 + r) * C + c0 + tx] : (elem_t)0.f;
-        __syncthreads();
-    }
-    for (int c = ty; c < 32; c += 8)
-        if (c0 + c < C && r0 + tx < Rp)
-            d[(long long)(c0 + c) * Rp + r0 + tx] = transpose ? tile[tx][c] : r0 + tx < R ? s[(long long)(c0 + c) * R + r0 + tx] : (elem_t)0.f;
+// 32 x 32 tiles through LDS.  pad: dst[e][c][0 .. Rp) = src[e][c][0 .. R), zeros behind (B whose rank rows are not whole 16-byte chunks)
+__global__ __launch_bounds__(256) void k_adapter_pad(const elem_t* __restrict__ src, elem_t* __restrict__ dst, long long rows, int R, int Rp) {
+    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (at >= rows * Rp) return;
+    const long long c = at / Rp;
+    const int r = (int)(at - c * Rp);
+    dst[at] = r < R ? src[c * R + r] : (elem_t)0.f;
 }
 
-// dst[e][r][n] = src[e][n][r] for r < R: B^T rows of the data gradient's shrink
-__global__ __launch_bounds__(256) void k_adapter_cols(const elem_t* __restrict__ src, elem_t* __restrict__ dst, int N, int R) {
+// The operands of the data gradient: at [E, K, Rp] = A^T with zeros past R (from A [E, R, K]) and bt [E, R, N] = B^T (from B [E, N, R]).
+// blockIdx.x: the column tiles of at (none if at is NULL), then those of bt; y: rank tile; z: adapter.
+__global__ __launch_bounds__(256) void k_adapter_transpose(const elem_t* __restrict__ A, const elem_t* __restrict__ B, elem_t* __restrict__ at,
+                                                           elem_t* __restrict__ bt, int K, int N, int R, int Rp, int at_tiles) {
     __shared__ elem_t tile[32][34];
-    const int n0 = blockIdx.x * 32, r0 = blockIdx.y * 32, tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const elem_t* s = src + (long long)blockIdx.z * R * N;
-    elem_t* d = dst + (long long)blockIdx.z * R * N;
-    for (int n = ty; n < 32; n += 8) tile[n][tx] = n0 + n < N && r0 + tx < R ? s[(long long)(n0 + n) * R + r0 + tx] : (elem_t)0.f;
-    __syncthreads();
-    for (int r = ty; r < 32; r += 8)
-        if (r0 + r < R && n0 + tx < N) d[(long long)(r0 + r) * N + n0 + tx] = tile[tx][r];
+    const int r0 = blockIdx.y * 32, tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    if ((int)blockIdx.x < at_tiles) {
+        const int c0 = blockIdx.x * 32;
+        const elem_t* s = A + (long long)blockIdx.z * R * K;
+        for (int r = ty; r < 32; r += 8) tile[r][tx] = r0 + r < R && c0 + tx < K ? s[(long long)(r0 + r) * K + c0 + tx] : (elem_t)0.f;
+        __syncthreads();
+        elem_t* d = at + (long long)blockIdx.z * K * Rp;
+        for (int c = ty; c < 32; c += 8)
+            if (c0 + c < K && r0 + tx < Rp) d[(long long)(c0 + c) * Rp + r0 + tx] = tile[tx][c];
+    } else {
+        const int n0 = ((int)blockIdx.x - at_tiles) * 32;
+        const elem_t* s = B + (long long)blockIdx.z * R * N;
+        for (int n = ty; n < 32; n += 8) tile[n][tx] = n0 + n < N && r0 + tx < R ? s[(long long)(n0 + n) * R + r0 + tx] : (elem_t)0.f;
+        __syncthreads();
+        elem_t* d = bt + (long long)blockIdx.z * R * N;
+        for (int r = ty; r < 32; r += 8)
+            if (r0 + r < R && n0 + tx < N) d[(long long)(r0 + r) * N + n0 + tx] = tile[tx][r];
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ weight gradient
@@ -548,55 +716,73 @@ __global__ __launch_bounds__(1024) void k_wgrad_plan(Rows rows, int chunk, int* 
     }
 }
 
+// the request of row m (one that adapter_of has found to have an adapter) and its first row
+__device__ __forceinline__ int request_of(const Rows& rows, long long m, long long& begin) {
+    if (!rows.offsets) {
+        const int i = (int)(m / rows.each);
+        begin = i * rows.each;
+        return i;
+    }
+    int lo = 0, hi = rows.n;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (rows.offsets[mid + 1] <= m) lo = mid + 1;
+        else hi = mid;
+    }
+    begin = max(rows.offsets[lo], 0);
+    return lo;
+}
+
 __global__ __launch_bounds__(256) void k_wgrad_perm(Rows rows, const int* __restrict__ start, int* __restrict__ perm) {
     const long long m = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (m >= rows.M) return;
-    if (adapter_of(rows, m) == kNone) return;
-    int lo = 0, hi = rows.n;
+    if (m >= rows.M || adapter_of(rows, m) == kNone) return;
     long long begin;
-    if (rows.offsets) {
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (rows.offsets[mid + 1] <= m) lo = mid + 1;
-            else hi = mid;
-        }
-        begin = max(rows.offsets[lo], 0);
-    } else {
-        lo = (int)(m / rows.each);
-        begin = lo * rows.each;
-    }
-    const long long at = start[lo] + (m - begin);
+    const int i = request_of(rows, m, begin);
+    const long long at = start[i] + (m - begin);
     if (at < rows.M) perm[at] = (int)m;
 }
 
+// Both weight gradients in one launch: dA from (du, x) over K columns, dB from (u, dy) over N.
+struct WgradArgs {
+    const elem_t *X[2], *u[2];
+    const float* us[2];
+    float* part[2];
+    elem_t* out[2];
+    const int *first, *item, *perm;
+    int C[2], tiles[2];      // columns, 128-column tiles (0: not wanted)
+    int E, R, chunk;
+};
+
 // part[item][r < Rp][C] = sum over the item's rows of (value + rest)[m, r] us[m] X[m, c].  Workgroup = one item x 128 columns (a wave 32),
-// rows in stages of 64 through LDS, both operands read with the transposing LDS read (the contraction index is the row).  The rows of a
-// stage sit at a pitch of 16 or 48 dwords past a multiple of 64: the four rows and two column groups of a transposing read hit
-// disjoint banks.  In half precision the pair is rescaled to the item's largest row scale while it is staged.
+// rows in stages of 64 through LDS (requested a stage ahead), both operands read with the transposing LDS read (the contraction index
+// is the row).  The rows of a stage sit at a pitch of 16 or 48 dwords past a multiple of 64: the four rows and two column groups of a
+// transposing read hit disjoint banks.  In half precision the pair is rescaled to the item's largest row scale while it is staged.
 template <int Rp>
-__global__ __launch_bounds__(256) void k_wgrad(const elem_t* __restrict__ X, const elem_t* __restrict__ u, const float* __restrict__ us,
-                                               const int* __restrict__ first, const int* __restrict__ item, const int* __restrict__ perm, int E,
-                                               int chunk, int C, float* __restrict__ part) {
+__global__ __launch_bounds__(256) void k_wgrad(WgradArgs a) {
     constexpr int UC = 2 * Rp, UF = UC / 32;                       // columns of the pair, 32-row fragments
     constexpr int UP = UC == 32 ? 64 : UC * 2 + 64, XP = 320;      // byte pitches
+    constexpr int UN = (64 * (Rp / 8) + 255) / 256;                // pair chunks per thread and stage
     __shared__ __attribute__((aligned(16))) char xs[64 * XP];
     __shared__ __attribute__((aligned(16))) char ub[64 * UP];
     [[maybe_unused]] __shared__ float red[4];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, hi = lane >> 5, l31 = lane & 31;
-    const int it = blockIdx.y;
-    if (it >= item[E]) return;
-    int lo = 0, up = E - 1;                                        // the adapter whose items include `it`
+    const int it = blockIdx.y, side = (int)blockIdx.x >= a.tiles[0];
+    if (it >= a.item[a.E]) return;
+    const elem_t* X = a.X[side];
+    const elem_t* u = a.u[side];
+    [[maybe_unused]] const float* us = a.us[side];
+    const int C = a.C[side], c0 = ((int)blockIdx.x - (side ? a.tiles[0] : 0)) * 128;
+    int lo = 0, up = a.E - 1;                                      // the adapter whose items include `it`
     while (lo < up) {
         const int mid = (lo + up) >> 1;
-        if (item[mid + 1] <= it) lo = mid + 1;
+        if (a.item[mid + 1] <= it) lo = mid + 1;
         else up = mid;
     }
-    const int v0 = first[lo] + (it - item[lo]) * chunk, v1 = min(v0 + chunk, first[lo + 1]);
-    const int c0 = blockIdx.x * 128;
+    const int v0 = a.first[lo] + (it - a.item[lo]) * a.chunk, v1 = min(v0 + a.chunk, a.first[lo + 1]);
     float top = 1.f;
 #if defined(DM_F16)
     float big = 0.f;
-    for (int v = v0 + tid; v < v1; v += 256) big = fmaxf(big, perm[v] >= 0 ? us[perm[v]] : 0.f);
+    for (int v = v0 + tid; v < v1; v += 256) big = fmaxf(big, a.perm[v] >= 0 ? us[a.perm[v]] : 0.f);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor(big, o, 64));
     if (lane == 0) red[wave] = big;
@@ -611,37 +797,71 @@ __global__ __launch_bounds__(256) void k_wgrad(const elem_t* __restrict__ X, con
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[f][r] = 0.f;
     const int i16 = lane & 15, g1 = (lane >> 4) & 1;
+    // this thread's rows of a stage: x rows tid / 16 + 16 q, pair rows (tid + 256 q) / (Rp / 8)
+    int xm[4], um[UN];
+    u32x4 xd[4];
+    elem8 ph[UN], pl[UN];
+    [[maybe_unused]] float pf[UN];
+    auto rows_of = [&](int v) __attribute__((always_inline)) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) xm[q] = v + (tid >> 4) + 16 * q < v1 ? a.perm[v + (tid >> 4) + 16 * q] : kNone;
+#pragma unroll
+        for (int q = 0; q < UN; ++q) {
+            const int row = (tid + 256 * q) / (Rp / 8);
+            um[q] = row < 64 && v + row < v1 ? a.perm[v + row] : kNone;
+        }
+    };
+    const int xc = c0 + (tid & 15) * 8;
+    auto load = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            xd[q] = u32x4{0u, 0u, 0u, 0u};
+            if (xm[q] >= 0 && xc < C) xd[q] = *reinterpret_cast<const u32x4*>(X + (long long)xm[q] * C + xc);
+        }
+#pragma unroll
+        for (int q = 0; q < UN; ++q) {
+            const int c = (tid + 256 * q) % (Rp / 8) * 8;
+            ph[q] = elem8{};
+            pl[q] = elem8{};
+#if defined(DM_F16)
+            pf[q] = 0.f;
+#endif
+            if (um[q] >= 0) {
+                ph[q] = *reinterpret_cast<const elem8*>(u + (long long)um[q] * UC + c);
+                pl[q] = *reinterpret_cast<const elem8*>(u + (long long)um[q] * UC + Rp + c);
+#if defined(DM_F16)
+                pf[q] = us[um[q]] * inv;
+#endif
+            }
+        }
+    };
+    rows_of(v0);
+    load();
+    rows_of(v0 + 64);
     for (int v = v0; v < v1; v += 64) {
         __syncthreads();
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {                              // 64 rows x 16 chunks of x
-            const int idx = tid + 256 * q, row = idx >> 4, c = c0 + (idx & 15) * 8;
-            u32x4 d = {0u, 0u, 0u, 0u};
-            const int m = v + row < v1 ? perm[v + row] : kNone;
-            if (m >= 0 && c < C) d = *reinterpret_cast<const u32x4*>(X + (long long)m * C + c);
-            *reinterpret_cast<u32x4*>(xs + row * XP + (idx & 15) * 16) = d;
-        }
-        for (int idx = tid; idx < 64 * (Rp / 8); idx += 256) {     // 64 rows of pairs
-            const int row = idx / (Rp / 8), c = idx % (Rp / 8) * 8;
-            elem8 p = {}, q = {};
-            const int m = v + row < v1 ? perm[v + row] : kNone;
-            if (m >= 0) {
-                p = *reinterpret_cast<const elem8*>(u + (long long)m * UC + c);
-                q = *reinterpret_cast<const elem8*>(u + (long long)m * UC + Rp + c);
-#if defined(DM_F16)
-                const float f = us[m] * inv;
+        for (int q = 0; q < 4; ++q) *reinterpret_cast<u32x4*>(xs + ((tid >> 4) + 16 * q) * XP + (tid & 15) * 16) = xd[q];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const float w = ((float)p[k] + (float)q[k]) * f;
-                    p[k] = (elem_t)w;
-                    q[k] = (elem_t)(w - (float)p[k]);
-                }
-#endif
+        for (int q = 0; q < UN; ++q) {
+            const int row = (tid + 256 * q) / (Rp / 8), c = (tid + 256 * q) % (Rp / 8) * 8;
+            if (row >= 64) continue;
+#if defined(DM_F16)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float w = ((float)ph[q][k] + (float)pl[q][k]) * pf[q];
+                ph[q][k] = (elem_t)w;
+                pl[q][k] = (elem_t)(w - (float)ph[q][k]);
             }
-            *reinterpret_cast<elem8*>(ub + row * UP + c * 2) = p;
-            *reinterpret_cast<elem8*>(ub + row * UP + (Rp + c) * 2) = q;
+#endif
+            *reinterpret_cast<elem8*>(ub + row * UP + c * 2) = ph[q];
+            *reinterpret_cast<elem8*>(ub + row * UP + (Rp + c) * 2) = pl[q];
         }
         __syncthreads();
+        if (v + 64 < v1) {
+            load();
+            rows_of(v + 128);
+        }
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
             const int row = 16 * ks + 8 * hi + (i16 >> 2), col = 16 * g1 + 4 * (i16 & 3);
@@ -660,7 +880,7 @@ __global__ __launch_bounds__(256) void k_wgrad(const elem_t* __restrict__ X, con
     // acc[f]: lane = column, register r = pair column 32 f + (r & 3) + 8 (r >> 2) + 4 hi; value and rest are Rp columns apart
     const int c = c0 + 32 * wave + l31;
     if (c >= C) return;
-    float* out = part + (long long)it * Rp * C + c;
+    float* out = a.part[side] + (long long)it * Rp * C + c;
     if constexpr (Rp == 16) {
 #pragma unroll
         for (int r = 0; r < 8; ++r) out[(long long)((r & 3) + 8 * (r >> 2) + 4 * hi) * C] = (acc[0][r] + acc[0][r + 8]) * top;
@@ -672,16 +892,25 @@ __global__ __launch_bounds__(256) void k_wgrad(const elem_t* __restrict__ X, con
     }
 }
 
-// out[e][r][c] (transpose: out[e][c][r]) = sum of the adapter's items in order, rounded once; an adapter without rows gets zeros.
-// 64 columns x 4 ranks per workgroup; the transposed store goes through LDS.
-__global__ __launch_bounds__(256) void k_wgrad_join(const float* __restrict__ part, const int* __restrict__ item, int C, int R, int Rp, int transpose,
-                                                    elem_t* __restrict__ out) {
-    const int e = blockIdx.z, c = blockIdx.x * 64 + (threadIdx.x & 63), r = blockIdx.y * 4 + (threadIdx.x >> 6);
-    if (c >= C || r >= R) return;
+// dA[e][r][c] and dB[e][c][r] = the sums of the adapter's items in a fixed order (four shares, eight loads in flight each), rounded once; an
+// adapter without rows gets zeros.  Workgroup = 64 columns x one rank; blockIdx.x: the column blocks of dA, then those of dB.
+__global__ __launch_bounds__(256) void k_wgrad_join(WgradArgs a, int blocks_a, int Rp) {
+    __shared__ float red[4][64];
+    const int side = (int)blockIdx.x >= blocks_a, C = a.C[side];
+    const int e = blockIdx.z, r = blockIdx.y, tx = threadIdx.x & 63, q = threadIdx.x >> 6, c = ((int)blockIdx.x - (side ? blocks_a : 0)) * 64 + tx;
+    const int lo = a.item[e], n = a.item[e + 1] - lo;
+    const float* p = a.part[side] + ((long long)lo * Rp + r) * C + c;
     float s = 0.f;
-    for (int it = item[e]; it < item[e + 1]; ++it) s += part[((long long)it * Rp + r) * C + c];
-    if (transpose) out[((long long)e * C + c) * R + r] = (elem_t)s;
-    else out[((long long)e * R + r) * C + c] = (elem_t)s;
+    if (c < C) {
+#pragma unroll 8
+        for (int i = q; i < n; i += 4) s += p[(long long)i * Rp * C];
+    }
+    red[q][tx] = s;
+    __syncthreads();
+    if (q || c >= C) return;
+    s = red[0][tx] + red[1][tx] + red[2][tx] + red[3][tx];
+    if (side) a.out[1][((long long)e * C + c) * a.R + r] = (elem_t)s;
+    else a.out[0][((long long)e * a.R + r) * C + c] = (elem_t)s;
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -701,98 +930,140 @@ Rows make_rows(const int* ids, const int* offsets, long long n, long long M, int
 // requests shorter than this share a tile with many others: one row at a time then
 bool few_rows_each(long long M, long long n) { return M < 8 * n; }
 
-template <int RT>
-int launch_shrink(const elem_t* x, const elem_t* A, const Rows& rows, int K, int R, float scale, elem_t* u, float* us, hipStream_t stream) {
-    const dim3 grid((unsigned)((rows.M + 16 * RT - 1) / (16 * RT)));
-    switch (rank_pad(R)) {
-        case 16: hipLaunchKernelGGL((k_shrink<RT, 1>), grid, dim3(256), 0, stream, x, A, rows, K, R, scale, u, us); break;
-        case 32: hipLaunchKernelGGL((k_shrink<RT, 2>), grid, dim3(256), 0, stream, x, A, rows, K, R, scale, u, us); break;
-        case 64: hipLaunchKernelGGL((k_shrink<(RT > 2 ? 2 : RT), 4>), dim3((unsigned)((rows.M + 16 * std::min(RT, 2) - 1) / (16 * std::min(RT, 2)))), dim3(256), 0, stream, x, A, rows, K, R, scale, u, us); break;
-        default: hipLaunchKernelGGL((k_shrink<1, 8>), dim3((unsigned)((rows.M + 15) / 16)), dim3(256), 0, stream, x, A, rows, K, R, scale, u, us); break;
-    }
+template <int RT, int NR>
+void launch_shrink(const elem_t* x, const elem_t* A, const Rows& rows, int K, int R, float scale, elem_t* u, float* us, hipStream_t stream) {
+    hipLaunchKernelGGL((k_shrink<RT, NR>), dim3((unsigned)((rows.M + 16 * RT - 1) / (16 * RT))), dim3(256), 0, stream, x, A, rows, K, R, scale, u, us);
+}
+
+template <int NR>
+int launch_ring(const elem_t* x, const elem_t* A, const Rows& rows, int K, int R, float scale, elem_t* u, float* us, hipStream_t stream) {
+    constexpr int LDS = 4 * (64 + 16 * NR) * 128 + 64 * 4;
+    static hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_shrink_ring<NR>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    if (attr != hipSuccess) return (int)attr;
+    hipLaunchKernelGGL((k_shrink_ring<NR>), dim3((unsigned)((rows.M + 63) / 64)), dim3(256), LDS, stream, x, A, rows, K, R, scale, u, us);
     DM_LAUNCH_CHECK();
     return DM_OK;
 }
 
+// Many rows: 64-row tiles through LDS; few: 32 or 16 rows per workgroup, whose waves share K; requests of a few rows: one row each.
 int shrink(const elem_t* x, const elem_t* A, const Rows& rows, int K, int R, float scale, elem_t* u, float* us, hipStream_t stream) {
     if (few_rows_each(rows.M, rows.n)) {
-        const int threads = std::min(1024, 64 * R);
-        hipLaunchKernelGGL(k_shrink_rows, dim3((unsigned)rows.M), dim3(threads), 0, stream, x, A, rows, K, R, scale, u, us, (float*)nullptr);
+        hipLaunchKernelGGL(k_shrink_rows, dim3((unsigned)rows.M), dim3(std::min(1024, 64 * R)), 0, stream, x, A, rows, K, R, scale, u, us, (float*)nullptr);
         DM_LAUNCH_CHECK();
         return DM_OK;
     }
-    if (rows.M >= 64 * 512) return launch_shrink<4>(x, A, rows, K, R, scale, u, us, stream);
-    if (rows.M >= 32 * 512) return launch_shrink<2>(x, A, rows, K, R, scale, u, us, stream);
-    return launch_shrink<1>(x, A, rows, K, R, scale, u, us, stream);
-}
-
-template <int BM, int BN, int WM, int WN>
-int launch_expand(ExpandArgs a, hipStream_t stream) {
-    constexpr int LDS = 2 * (BM + BN) * 128 + BM * 4;
-    const long long n_mt = (a.rows.M + BM - 1) / BM;
-    a.n_nt = (a.N + BN - 1) / BN;
-    if (n_mt * a.n_nt > (1LL << 30)) return DM_ERR_UNSUPPORTED;
-    a.tiles = (int)(n_mt * a.n_nt);
-    static hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_expand<BM, BN, WM, WN>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-    if (attr != hipSuccess) return (int)attr;
-    const unsigned blocks = (unsigned)((a.tiles + 7) / 8 * 8);
-    hipLaunchKernelGGL((k_expand<BM, BN, WM, WN>), dim3(blocks), dim3(WM * WN * 64), LDS, stream, a);
+    const int Rp = rank_pad(R);
+    if (rows.M >= 64 * 192) {                                        // (tiles for three quarters of the CUs)
+        switch (Rp) {
+            case 16: return launch_ring<1>(x, A, rows, K, R, scale, u, us, stream);
+            case 32: return launch_ring<2>(x, A, rows, K, R, scale, u, us, stream);
+            case 64: return launch_ring<4>(x, A, rows, K, R, scale, u, us, stream);
+            default: return launch_ring<8>(x, A, rows, K, R, scale, u, us, stream);
+        }
+    }
+    auto go = [&](auto rt_tag) {
+        constexpr int RT = decltype(rt_tag)::value;
+        switch (Rp) {
+            case 16: launch_shrink<RT, 1>(x, A, rows, K, R, scale, u, us, stream); break;
+            case 32: launch_shrink<RT, 2>(x, A, rows, K, R, scale, u, us, stream); break;
+            case 64: launch_shrink<RT, 4>(x, A, rows, K, R, scale, u, us, stream); break;
+            default: launch_shrink<RT, 8>(x, A, rows, K, R, scale, u, us, stream); break;
+        }
+    };
+    if (rows.M >= 32 * 256) go(std::integral_constant<int, 2>{});
+    else go(std::integral_constant<int, 1>{});
     DM_LAUNCH_CHECK();
     return DM_OK;
 }
 
+template <int BM, int BN, int WM, int WN, int NST>
+int launch_expand(ExpandArgs a, hipStream_t stream) {
+    constexpr int LDS = NST * (BM + BN) * 128 + BM * 8 + BN * 4;
+    const long long n_mt = (a.rows.M + BM - 1) / BM;
+    a.n_nt = (a.N + BN - 1) / BN;
+    if (n_mt * a.n_nt > (1LL << 30)) return DM_ERR_UNSUPPORTED;
+    a.n_mt = (int)n_mt;
+    a.tiles = (int)(n_mt * a.n_nt);
+    static hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_expand<BM, BN, WM, WN, NST>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    if (attr != hipSuccess) return (int)attr;
+    hipLaunchKernelGGL((k_expand<BM, BN, WM, WN, NST>), dim3((unsigned)((a.tiles + 7) / 8 * 8)), dim3(WM * WN * 64), LDS, stream, a);
+    DM_LAUNCH_CHECK();
+    return DM_OK;
+}
+
+// Tile by the rounds a launch takes: a round of 768 tiles of 64 x 64 (three per CU) takes 0.34 / 0.6 of one of 512 tiles of 128 x 128 (two per
+// CU) for 0.37 of the work.  (256 x 256 tiles are 6-14 % faster on the bare product, but their accumulators leave no registers for rows
+// of several adapters: with spills 850 against 500 us on [24576, 1280, 5120].)
+int expand(const ExpandArgs& a, hipStream_t stream) {
+    auto rounds = [&](long long t, long long per) { return (double)(((a.rows.M + t - 1) / t * ((a.N + t - 1) / t) + per - 1) / per); };
+    if (0.6 * rounds(128, 512) <= 0.34 * rounds(64, 768)) return launch_expand<128, 128, 2, 2, 2>(a, stream);
+    return launch_expand<64, 64, 2, 2, 3>(a, stream);
+}
+
 constexpr long long kSkinny = 32;
+
+long long align256(long long v) { return (v + 255) / 256 * 256; }
+long long u_bytes(long long M, int R) { return align256(M * (4LL * rank_pad(R) + 4)); }
+
+int check_product(const Rows& r, const void* x, const void* w, const void* lora_a, const void* lora_b, int K, int N, int R) {
+    if (!x || !lora_a || !lora_b || K <= 0 || N <= 0 || R <= 0) return DM_ERR_ARG;
+    if (R > kMaxRank || K % 8 || N % 8 || K > (1 << 20) || N > (1 << 20) || r.E > 65535) return DM_ERR_UNSUPPORTED;
+    if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)lora_a | (uintptr_t)lora_b) & 15) return DM_ERR_ARG;
+    return DM_OK;
+}
+
+// row ranges of the weight gradients: enough workgroups to fill the chip (four per CU over the 128-column tiles of both), but whole 64-row
+// stages and few partial sums
+int wgrad_chunk(long long M, int K, int N) { return (int)std::max<long long>(128, (M * ((K + N + 127) / 128) / 1024 + 63) / 64 * 64); }
+long long wgrad_items(long long M, int E, int chunk) { return std::min<long long>(M, M / chunk + E); }
 
 }  // namespace
 
 extern "C" {
 
 #if !defined(DM_F16)
-// bytes of the u buffer for M rows: pairs of 16-bit columns, then one fp32 scale per row
-size_t dm_adapter_u_bytes(long long M, int R) {
-    if (M <= 0 || R <= 0 || R > kMaxRank) return 0;
-    return (size_t)M * (4 * rank_pad(R) + 4);
+// bytes of the forward's workspace: u as pairs of 16-bit columns and one fp32 scale per row, then B with padded rank rows where R % 8 != 0
+size_t dm_linear_adapted_workspace_bytes(long long M, int N, int R, int E) {
+    if (M <= 0 || N <= 0 || R <= 0 || R > kMaxRank || E <= 0) return 0;
+    return (size_t)(u_bytes(M, R) + (R % 8 ? 2LL * E * N * rank_pad(R) : 0));
 }
 
-// int32 words of the weight-gradient plan (first | item | start | perm) and its largest number of items
-size_t dm_adapter_plan_words(long long M, long long n, int E) { return M <= 0 || n <= 0 || E <= 0 ? 0 : (size_t)(2 * (E + 1) + n + M); }
-long long dm_adapter_plan_items(long long M, int E, int chunk) { return M <= 0 || E <= 0 || chunk <= 0 ? 0 : std::min<long long>(M, M / chunk + E); }
-
-// the adapter order of the rows for dm_adapter_wgrad_*: plan [dm_adapter_plan_words] int32; chunk = rows per item (a multiple of 64)
-int dm_adapter_plan(const int* ids, const int* offsets, long long n, long long M, int E, int chunk, int* plan, hipStream_t stream) {
-    if (int rc = check_rows(ids, n, M, E, offsets != nullptr)) return rc;
-    if (!plan || chunk <= 0 || chunk % 64 || M == 0) return DM_ERR_ARG;
-    const Rows rows = make_rows(ids, offsets, n, M, E);
-    int *first = plan, *item = first + E + 1, *start = item + E + 1, *perm = start + n;
-    DM_ENTER();
-    hipLaunchKernelGGL(k_wgrad_plan, dim3(1), dim3(1024), 0, stream, rows, chunk, first, item, start, perm);
-    hipLaunchKernelGGL(k_wgrad_perm, dim3((unsigned)((M + 255) / 256)), dim3(256), 0, stream, rows, start, perm);
-    DM_LAUNCH_CHECK();
-    return DM_OK;
+// bytes of the backward's: du, A^T, B^T, the plan (first | item | start | perm) and the weight gradients' partial sums
+size_t dm_linear_adapted_bwd_workspace_bytes(long long M, int K, int N, int R, int E, long long n) {
+    if (M <= 0 || K <= 0 || N <= 0 || R <= 0 || R > kMaxRank || E <= 0 || n <= 0) return 0;
+    const int Rp = rank_pad(R);
+    return (size_t)(u_bytes(M, R) + align256(2LL * E * K * Rp) + align256(2LL * E * N * R) + align256(4 * (2LL * (E + 1) + n + M)) +
+                    4LL * wgrad_items(M, E, wgrad_chunk(M, K, N)) * Rp * (K + N));
 }
 #endif
 
 // y = x W^T + bias + s (x A_e^T) B_e^T + residual, see the head of this file.  x [M, K], w [N, K], bias [N] or NULL, residual [M, N] or
-// NULL, lora_a [E, R, K], lora_b [E, N] rows of R elements `ldb` apart, ids [n] int32, offsets [n + 1] int32 or NULL (then M % n == 0), u
-// scratch of dm_adapter_u_bytes; keep_u != 0: u is left in pair format for dm_adapter_wgrad_* (y NULL: nothing else is computed).  K % 8 == N % 8 == ldb % 8 == 0, R <= 128.
-int DM_T(dm_linear_adapted_, )(const void* x, const void* w, const void* bias, const void* residual, const void* lora_a, const void* lora_b, int ldb,
-                               const int* ids, const int* offsets, long long n, float scale, void* u, size_t u_bytes, void* y, long long M, int K,
-                               int N, int R, int E, int keep_u, hipStream_t stream) {
+// NULL, lora_a [E, R, K], lora_b [E, N, R], ids [n] int32, offsets [n + 1] int32 or NULL (then M % n == 0), ws of
+// dm_linear_adapted_workspace_bytes; keep_u != 0: u is left at its head for dm_linear_adapted_bwd_*.  K % 8 == N % 8 == 0, R <= 128.
+int DM_T(dm_linear_adapted_, )(const void* x, const void* w, const void* bias, const void* residual, const void* lora_a, const void* lora_b, const int* ids,
+                               const int* offsets, long long n, float scale, void* ws, size_t ws_bytes, void* y, long long M, int K, int N, int R, int E,
+                               int keep_u, hipStream_t stream) {
     if (int rc = check_rows(ids, n, M, E, offsets != nullptr)) return rc;
-    if (!x || !lora_a || !u || (y ? !w || !lora_b || ldb < R : !keep_u) || K <= 0 || N <= 0 || R <= 0) return DM_ERR_ARG;
-    if (R > kMaxRank || K % 8 || N % 8 || (y && ldb % 8) || K > (1 << 20) || N > (1 << 24)) return DM_ERR_UNSUPPORTED;
-    if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)bias | (uintptr_t)residual | (uintptr_t)lora_a | (uintptr_t)lora_b | (uintptr_t)u | (uintptr_t)y) & 15) return DM_ERR_ARG;
+    const Rows rows = make_rows(ids, offsets, n, M, E);
+    if (int rc = check_product(rows, x, w, lora_a, lora_b, K, N, R)) return rc;
+    if (!w || !ws || !y || (((uintptr_t)bias | (uintptr_t)residual | (uintptr_t)ws | (uintptr_t)y) & 15)) return DM_ERR_ARG;
     if (M == 0) return DM_OK;
     const int Rp = rank_pad(R);
-    if (u_bytes < (size_t)M * (4 * Rp + 4)) return DM_ERR_WORKSPACE;
+    if ((long long)ws_bytes < u_bytes(M, R) + (R % 8 ? 2LL * E * N * Rp : 0)) return DM_ERR_WORKSPACE;
     ExpandArgs a{};
     a.x = (const elem_t*)x; a.w = (const elem_t*)w; a.bias = (const elem_t*)bias; a.res = (const elem_t*)residual;
-    a.u = (const elem_t*)u; a.us = (const float*)((const elem_t*)u + M * 2 * Rp); a.B = (const elem_t*)lora_b; a.y = (elem_t*)y;
-    a.rows = make_rows(ids, offsets, n, M, E);
-    a.K = K; a.N = N; a.R = R; a.ldb = ldb;
+    a.u = (const elem_t*)ws; a.us = (const float*)((const elem_t*)ws + M * 2 * Rp); a.B = (const elem_t*)lora_b; a.y = (elem_t*)y;
+    a.rows = rows;
+    a.K = K; a.N = N; a.R = R; a.ldb = R;
     DM_ENTER();
+    if (R % 8) {
+        elem_t* padded = (elem_t*)((char*)ws + u_bytes(M, R));
+        hipLaunchKernelGGL(k_adapter_pad, dim3((unsigned)(((long long)E * N * Rp + 255) / 256)), dim3(256), 0, stream, a.B, padded, (long long)E * N, R, Rp);
+        a.B = padded;
+        a.ldb = Rp;
+    }
     if (M <= kSkinny && !keep_u) {
-        float* uf = (float*)u;
+        float* uf = (float*)ws;
         hipLaunchKernelGGL(k_shrink_rows, dim3((unsigned)M), dim3(std::min(1024, 64 * R)), 0, stream, a.x, (const elem_t*)lora_a, a.rows, K, R, scale,
                            (elem_t*)nullptr, (float*)nullptr, uf);
         const dim3 grid((unsigned)((N + 15) / 16));
@@ -801,50 +1072,67 @@ int DM_T(dm_linear_adapted_, )(const void* x, const void* w, const void* bias, c
         DM_LAUNCH_CHECK();
         return DM_OK;
     }
-    if (int rc = shrink(a.x, (const elem_t*)lora_a, a.rows, K, R, scale, (elem_t*)u, const_cast<float*>(a.us), stream)) return rc;
-    if (!y) return DM_OK;
-    return launch_expand<128, 128, 2, 2>(a, stream);
+    if (int rc = shrink(a.x, (const elem_t*)lora_a, a.rows, K, R, scale, (elem_t*)ws, const_cast<float*>(a.us), stream)) return rc;
+    return expand(a, stream);
 }
 
-// the adapters laid out for a product with padded rank rows: dst [E, C, rank padded to 16 | 32 | 64 | 128], zeros past R.  mode 0: src
-// [E, C, R] copied; mode 1: src [E, R, C] transposed; mode 2: src [E, C, R] -> dst [E, R, C] (no padding)
-int DM_T(dm_adapter_layout_, )(const void* src, void* dst, int E, int C, int R, int mode, hipStream_t stream) {
-    if (!src || !dst || E <= 0 || C <= 0 || R <= 0 || mode < 0 || mode > 2) return DM_ERR_ARG;
-    if (R > kMaxRank || E > 65535) return DM_ERR_UNSUPPORTED;
-    const int Rp = rank_pad(R);
-    const dim3 grid((unsigned)((C + 31) / 32), (unsigned)((Rp + 31) / 32), (unsigned)E);
-    DM_ENTER();
-    if (mode == 2) hipLaunchKernelGGL(k_adapter_cols, grid, dim3(256), 0, stream, (const elem_t*)src, (elem_t*)dst, C, R);
-    else hipLaunchKernelGGL(k_adapter_rows, grid, dim3(256), 0, stream, (const elem_t*)src, (elem_t*)dst, C, R, Rp, mode);
-    DM_LAUNCH_CHECK();
-    return DM_OK;
-}
-
-// out[e] = sum over the rows m of adapter e of u[m, :]^T X[m, :]: [E, R, C], or (transpose) [E, C, R].  u as dm_linear_adapted_* left it (keep_u),
-// plan from dm_adapter_plan with the same chunk, part fp32 [dm_adapter_plan_items][rank padded][C].
-int DM_T(dm_adapter_wgrad_, )(const void* X, const void* u, const int* plan, long long n, long long M, int C, int R, int E, int chunk, int transpose,
-                              float* part, size_t part_floats, void* out, hipStream_t stream) {
-    if (!X || !u || !plan || !part || !out || n <= 0 || M <= 0 || M > 0x7fffffff || C <= 0 || R <= 0 || E <= 0 || chunk <= 0 || chunk % 64) return DM_ERR_ARG;
-    if (R > kMaxRank || C % 8 || E > 65535) return DM_ERR_UNSUPPORTED;
-    if (((uintptr_t)X | (uintptr_t)u) & 15) return DM_ERR_ARG;
-    const int Rp = rank_pad(R);
-    const long long items = std::min<long long>(M, M / chunk + E);
+// The gradients: dx [M, K] = dy W + s (dy B_e) A_e (w_t = W^T [K, N]), da [E, R, K], db [E, N, R]; each may be NULL (not wanted).  u = the
+// forward's workspace with keep_u (needed for db).
+int DM_T(dm_linear_adapted_bwd_, )(const void* x, const void* dy, const void* w_t, const void* lora_a, const void* lora_b, const int* ids, const int* offsets,
+                                   long long n, float scale, const void* u, void* ws, size_t ws_bytes, void* dx, void* da, void* db, long long M, int K, int N,
+                                   int R, int E, hipStream_t stream) {
+    if (int rc = check_rows(ids, n, M, E, offsets != nullptr)) return rc;
+    const Rows rows = make_rows(ids, offsets, n, M, E);
+    if (int rc = check_product(rows, x, w_t, lora_a, lora_b, K, N, R)) return rc;
+    if (!dy || !ws || M == 0 || (dx && !w_t) || (db && !u) || (((uintptr_t)dy | (uintptr_t)u | (uintptr_t)ws | (uintptr_t)dx) & 15)) return DM_ERR_ARG;
+    const int Rp = rank_pad(R), chunk = wgrad_chunk(M, K, N);
+    const long long items = wgrad_items(M, E, chunk);
     if (items > 65535) return DM_ERR_UNSUPPORTED;
-    if ((long long)part_floats < items * Rp * C) return DM_ERR_WORKSPACE;
-    const int *first = plan, *item = first + E + 1, *perm = item + E + 1 + n;
-    const elem_t* up = (const elem_t*)u;
-    const float* us = (const float*)(up + M * 2 * Rp);
-    const dim3 grid((unsigned)((C + 127) / 128), (unsigned)items);
+    if ((long long)ws_bytes < u_bytes(M, R) + align256(2LL * E * K * Rp) + align256(2LL * E * N * R) + align256(4 * (2LL * (E + 1) + n + M)) + 4LL * items * Rp * (K + N))
+        return DM_ERR_WORKSPACE;
+    char* p = (char*)ws;
+    auto take = [&](long long bytes) { char* q = p; p += align256(bytes); return q; };
+    elem_t* du = (elem_t*)take(u_bytes(M, R));
+    float* dus = (float*)(du + M * 2 * Rp);
+    elem_t* at = (elem_t*)take(2LL * E * K * Rp);
+    elem_t* bt = (elem_t*)take(2LL * E * N * R);
+    int* plan = (int*)take(4 * (2LL * (E + 1) + n + M));
+    float* part = (float*)p;
     DM_ENTER();
-    switch (Rp) {
-        case 16: hipLaunchKernelGGL(k_wgrad<16>, grid, dim3(256), 0, stream, (const elem_t*)X, up, us, first, item, perm, E, chunk, C, part); break;
-        case 32: hipLaunchKernelGGL(k_wgrad<32>, grid, dim3(256), 0, stream, (const elem_t*)X, up, us, first, item, perm, E, chunk, C, part); break;
-        case 64: hipLaunchKernelGGL(k_wgrad<64>, grid, dim3(256), 0, stream, (const elem_t*)X, up, us, first, item, perm, E, chunk, C, part); break;
-        default: hipLaunchKernelGGL(k_wgrad<128>, grid, dim3(256), 0, stream, (const elem_t*)X, up, us, first, item, perm, E, chunk, C, part); break;
+    if (dx || da) {
+        const int at_tiles = dx ? (K + 31) / 32 : 0;
+        hipLaunchKernelGGL(k_adapter_transpose, dim3((unsigned)(at_tiles + (N + 31) / 32), (unsigned)((Rp + 31) / 32), (unsigned)E), dim3(256), 0, stream,
+                           (const elem_t*)lora_a, (const elem_t*)lora_b, at, bt, K, N, R, Rp, at_tiles);
+        if (int rc = shrink((const elem_t*)dy, bt, rows, N, R, scale, du, dus, stream)) return rc;
     }
-    hipLaunchKernelGGL(k_wgrad_join, dim3((unsigned)((C + 63) / 64), (unsigned)((R + 3) / 4), (unsigned)E), dim3(256), 0, stream, part, item, C, R, Rp,
-                       transpose, (elem_t*)out);
-    DM_LAUNCH_CHECK();
+    if (dx) {
+        ExpandArgs a{};
+        a.x = (const elem_t*)dy; a.w = (const elem_t*)w_t; a.u = du; a.us = dus; a.B = at; a.y = (elem_t*)dx; a.rows = rows;
+        a.K = N; a.N = K; a.R = R; a.ldb = Rp;
+        if (int rc = expand(a, stream)) return rc;
+    }
+    if (da || db) {
+        int *first = plan, *item = first + E + 1, *start = item + E + 1, *perm = start + n;
+        hipLaunchKernelGGL(k_wgrad_plan, dim3(1), dim3(1024), 0, stream, rows, chunk, first, item, start, perm);
+        hipLaunchKernelGGL(k_wgrad_perm, dim3((unsigned)((M + 255) / 256)), dim3(256), 0, stream, rows, start, perm);
+        WgradArgs g{};
+        g.X[0] = (const elem_t*)x; g.u[0] = du; g.us[0] = dus; g.C[0] = K; g.out[0] = (elem_t*)da; g.part[0] = part;
+        g.X[1] = (const elem_t*)dy; g.u[1] = (const elem_t*)u; g.us[1] = (const float*)((const elem_t*)u + M * 2 * Rp); g.C[1] = N; g.out[1] = (elem_t*)db;
+        g.part[1] = part + items * Rp * K;
+        g.tiles[0] = da ? (K + 127) / 128 : 0;
+        g.tiles[1] = db ? (N + 127) / 128 : 0;
+        g.first = first; g.item = item; g.perm = perm; g.E = E; g.R = R; g.chunk = chunk;
+        const dim3 grid((unsigned)(g.tiles[0] + g.tiles[1]), (unsigned)items);
+        switch (Rp) {
+            case 16: hipLaunchKernelGGL(k_wgrad<16>, grid, dim3(256), 0, stream, g); break;
+            case 32: hipLaunchKernelGGL(k_wgrad<32>, grid, dim3(256), 0, stream, g); break;
+            case 64: hipLaunchKernelGGL(k_wgrad<64>, grid, dim3(256), 0, stream, g); break;
+            default: hipLaunchKernelGGL(k_wgrad<128>, grid, dim3(256), 0, stream, g); break;
+        }
+        const int ba = da ? (K + 63) / 64 : 0, bb = db ? (N + 63) / 64 : 0;
+        hipLaunchKernelGGL(k_wgrad_join, dim3((unsigned)(ba + bb), (unsigned)R, (unsigned)E), dim3(256), 0, stream, g, ba, Rp);
+        DM_LAUNCH_CHECK();
+    }
     return DM_OK;
 }
 

@@ -4,6 +4,7 @@ stream go straight into libdreammat_hip.so; `torch.autograd.Function`s provide t
 PyTorch is plumbing here (memory, streams, autograd graph) -- all arithmetic of these ops runs in the
 hand-written gfx950 kernels.  There is no fallback: CPU tensors or a missing library raise.
 """
+import contextlib
 import ctypes
 import os
 
@@ -1729,15 +1730,40 @@ def adam_step(param, grad, exp_avg, exp_avg_sq, step, lr, beta1, beta2, eps, gra
 
 
 # ------------------------------------------------------------------------------------------ fine-tuning: low-rank adapters
-def _need_same_device(first, *ts):
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _guard(device):
+    """makes `device` current for a launch (nothing to do where it is)"""
+    return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _stream_of(device):
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _timed(key, work):
+    """_Timed(key(), work) when timing is on (its key is a string that need not be built otherwise)"""
+    return _Timed(key(), work) if _TIMING["on"] else _NO_GUARD
+
+
+def _on_one_gpu(*ts):
+    """every tensor is on the first one's GPU -> its device"""
+    device = ts[0].device
     for t in ts:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"tensors on {first.device} and {t.device}: one device is needed")
+        if t is not None and t.device != device:
+            if t.is_cuda and ts[0].is_cuda:
+                raise ValueError(f"tensors on {device} and {t.device}: one device is needed")
+            _need_cuda(*ts)
+    if device.type != "cuda":
+        _need_cuda(*ts)
+    return device
 
 
 def _rows16(t):
     """contiguous and 16-byte aligned (a view that is neither is copied)"""
-    t = t.contiguous()
+    if not t.is_contiguous():
+        t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
@@ -1746,21 +1772,31 @@ def _ptr(t):
 
 
 MAX_ADAPTER_RANK = 128
+_ADAPTER_FN = {}        # element type -> forward, backward entry points
+
+
+def _adapter_fn(dtype):
+    fns = _ADAPTER_FN.get(dtype)
+    if fns is None:
+        fns = _ADAPTER_FN[dtype] = (_sym("dm_linear_adapted_bf16", dtype), _sym("dm_linear_adapted_bwd_bf16", dtype))
+    return fns
 
 
 def _adapter_sizes(x, w, bias, lora_a, lora_b, ids, residual, offsets):
     """the checks of linear_adapted -> (M, K, N, R, E, n)"""
-    if x.dtype not in HALF_DTYPES or any(t is not None and t.dtype != x.dtype for t in (w, bias, lora_a, lora_b, residual)):
+    dtype = x.dtype
+    if dtype not in HALF_DTYPES or w.dtype != dtype or lora_a.dtype != dtype or lora_b.dtype != dtype or (
+            bias is not None and bias.dtype != dtype) or (residual is not None and residual.dtype != dtype):
         raise TypeError("linear_adapted: bf16 or f16 tensors of one type expected")
     if w.dim() != 2 or lora_a.dim() != 3 or lora_b.dim() != 3 or x.dim() < 1:
         raise ValueError("linear_adapted: w [N, K], lora_a [E, R, K], lora_b [E, N, R] expected")
-    (N, K), (E, R) = w.shape, lora_a.shape[:2]
-    if x.shape[-1] != K or lora_a.shape[2] != K or tuple(lora_b.shape) != (E, N, R):
+    (N, K), (E, R, Ka) = w.shape, lora_a.shape
+    if x.shape[-1] != K or Ka != K or lora_b.shape != (E, N, R):
         raise ValueError(f"linear_adapted: x {tuple(x.shape)}, w {tuple(w.shape)}, lora_a {tuple(lora_a.shape)}, lora_b {tuple(lora_b.shape)} do not fit")
-    if E == 0 or not 1 <= R <= MAX_ADAPTER_RANK:
-        raise ValueError(f"linear_adapted: rank {R}, {E} adapters: 1 to {MAX_ADAPTER_RANK} ranks and at least one adapter are needed")
-    if K == 0 or N == 0 or K % 8 or N % 8:
-        raise ValueError(f"linear_adapted: K = {K} and N = {N} have to be multiples of 8")
+    if not 1 <= E <= 65535 or not 1 <= R <= MAX_ADAPTER_RANK:
+        raise ValueError(f"linear_adapted: rank {R}, {E} adapters: 1 to {MAX_ADAPTER_RANK} ranks and 1 to 65535 adapters are needed")
+    if K == 0 or N == 0 or K % 8 or N % 8 or max(K, N) > 1 << 20:
+        raise ValueError(f"linear_adapted: K = {K} and N = {N} have to be multiples of 8 (up to 2^20)")
     M = x.numel() // K
     if ids.dtype != torch.int32 or ids.dim() != 1 or ids.numel() == 0:
         raise ValueError("linear_adapted: ids is a non-empty int32 vector, one adapter per request")
@@ -1768,52 +1804,34 @@ def _adapter_sizes(x, w, bias, lora_a, lora_b, ids, residual, offsets):
     if offsets is None:
         if M % n:
             raise ValueError(f"linear_adapted: {M} rows are not {n} requests of one length (give offsets)")
-    elif offsets.dtype != torch.int32 or tuple(offsets.shape) != (n + 1,):
+    elif offsets.dtype != torch.int32 or offsets.shape != (n + 1,):
         raise ValueError("linear_adapted: offsets is an int32 vector of one more entry than ids")
-    if bias is not None and tuple(bias.shape) != (N,):
+    if bias is not None and bias.shape != (N,):
         raise ValueError("linear_adapted: bias [N] expected")
-    if residual is not None and tuple(residual.shape) != (*x.shape[:-1], N):
+    if residual is not None and residual.shape != (*x.shape[:-1], N):
         raise ValueError("linear_adapted: the residual has the result's shape")
-    if M >= 2 ** 31:
+    if M >= 1 << 31:
         raise ValueError("linear_adapted: fewer than 2^31 rows")
     return M, K, N, R, E, n
 
 
-def _adapter_layout(t, C, R, mode):
-    """dm_adapter_layout_*: 0 / 1 padded rank rows from [E, C, R] / [E, R, C], 2 [E, C, R] -> [E, R, C]"""
-    E, rp = t.shape[0], 16 if R <= 16 else 32 if R <= 32 else 64 if R <= 64 else 128
-    out = torch.empty((E, R, C) if mode == 2 else (E, C, rp), device=t.device, dtype=t.dtype)
-    fn, name = _sym("dm_adapter_layout_bf16", t.dtype)
-    check(fn(t.data_ptr(), out.data_ptr(), E, C, R, mode, _stream()), name)
-    return out
-
-
-def _adapter_product(x, w, bias, residual, a, b, ids, offsets, scale, sizes, keep_u, with_y=True):
-    """-> (y [M, N] or None, u): dm_linear_adapted_* on contiguous operands; b [E, N, ldb >= R]"""
-    M, K, N, R, E, n = sizes
-    u = torch.empty(int(_lib.lib().dm_adapter_u_bytes(M, R)), device=x.device, dtype=torch.uint8)
-    y = torch.empty(M, N, device=x.device, dtype=x.dtype) if with_y else None
-    fn, name = _sym("dm_linear_adapted_bf16", x.dtype)
-    with _Timed(f"linear_adapted[M={M},K={K},N={N},R={R}]", 2.0 * M * (K * N + R * (K + N))):
-        check(fn(x.data_ptr(), _ptr(w), _ptr(bias), _ptr(residual), a.data_ptr(), _ptr(b), 0 if b is None else b.shape[2], ids.data_ptr(), _ptr(offsets), n,
-                 float(scale), u.data_ptr(), u.numel(), _ptr(y), M, K, N, R, E, int(keep_u), _stream()), name)
-    return y, u
-
-
 def _adapter_forward(x, w, bias, lora_a, lora_b, ids, scale, residual, offsets, keep_u):
-    sizes = _adapter_sizes(x, w, bias, lora_a, lora_b, ids, residual, offsets)
-    _need_cuda(x, w, bias, lora_a, lora_b, ids, residual, offsets)
-    _need_same_device(x, w, bias, lora_a, lora_b, ids, residual, offsets)
-    M, K, N, R, E, n = sizes
+    M, K, N, R, E, n = _adapter_sizes(x, w, bias, lora_a, lora_b, ids, residual, offsets)
+    device = _on_one_gpu(x, w, bias, lora_a, lora_b, ids, residual, offsets)
+    y = torch.empty(*x.shape[:-1], N, device=device, dtype=x.dtype)
     if M == 0:
-        return x.new_empty(*x.shape[:-1], N), None
-    with torch.cuda.device(x.device):
-        b = _rows16(lora_b)
-        if R % 8:                                         # rank rows that are not whole 16-byte chunks: padded
-            b = _adapter_layout(b, N, R, 0)
-        y, u = _adapter_product(_rows16(x), _rows16(w), None if bias is None else _rows16(bias), None if residual is None else _rows16(residual),
-                                _rows16(lora_a), b, ids.contiguous(), None if offsets is None else offsets.contiguous(), scale, sizes, keep_u)
-    return y.view(*x.shape[:-1], N), u
+        return y, None
+    fn, name = _adapter_fn(x.dtype)[0]
+    with _guard(device):
+        x, w, lora_a, lora_b, ids = _rows16(x), _rows16(w), _rows16(lora_a), _rows16(lora_b), ids.contiguous()
+        bias, residual = None if bias is None else _rows16(bias), None if residual is None else _rows16(residual)
+        offsets = None if offsets is None else offsets.contiguous()
+        nb = _lib.lib().dm_linear_adapted_workspace_bytes(M, N, R, E)
+        ws = torch.empty(nb, device=device, dtype=torch.uint8)
+        with _timed(lambda: f"linear_adapted[M={M},K={K},N={N},R={R}]", 2.0 * M * (K * N + R * (K + N))):
+            check(fn(x.data_ptr(), w.data_ptr(), _ptr(bias), _ptr(residual), lora_a.data_ptr(), lora_b.data_ptr(), ids.data_ptr(), _ptr(offsets), n, scale,
+                     ws.data_ptr(), nb, y.data_ptr(), M, K, N, R, E, keep_u, _stream_of(device)), name)
+    return y, ws
 
 
 def linear_adapted(x, w, bias, lora_a, lora_b, ids, scale=1.0, residual=None, offsets=None):
@@ -1824,61 +1842,40 @@ def linear_adapted(x, w, bias, lora_a, lora_b, ids, scale=1.0, residual=None, of
     multiples of 8); ids int32 [n]: adapter of each request, outside [0, E) = none.  The rows of x (its leading dimensions flattened)
     are n requests of one length -- ids may be one per image, per sequence or per row -- or, with offsets int32 [n + 1] (ascending), request i is
     rows offsets[i] .. offsets[i + 1]; rows before the first and behind the last request have no adapter.  fp32 sums, one rounding."""
-    return _adapter_forward(x, w, bias, lora_a, lora_b, ids, scale, residual, offsets, False)[0]
+    return _adapter_forward(x, w, bias, lora_a, lora_b, ids, float(scale), residual, offsets, 0)[0]
 
 
 class _LinearAdapted(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, w_t, bias, lora_a, lora_b, ids, scale, residual, offsets):
-        y, u = _adapter_forward(x, w, bias, lora_a, lora_b, ids, scale, residual, offsets, True)
-        ctx.save_for_backward(x, lora_a, lora_b, ids, offsets, u if ctx.needs_input_grad[5] else None)
-        ctx.w_t, ctx.scale = w_t, float(scale)
+        y, u = _adapter_forward(x, w, bias, lora_a, lora_b, ids, scale, residual, offsets, 1)
+        ctx.save_for_backward(x, lora_a, lora_b, ids, offsets, u)
+        ctx.w_t, ctx.scale = w_t, scale
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         x, lora_a, lora_b, ids, offsets, u = ctx.saved_tensors
-        E, R, K = lora_a.shape
-        N = lora_b.shape[1]
-        M, n = x.numel() // K, ids.numel()
-        need_x, need_a, need_b = (ctx.needs_input_grad[i] for i in (0, 4, 5))
-        dx = da = db = None
+        (E, R, K), N = lora_a.shape, lora_b.shape[1]
+        M, n, device = x.numel() // K, ids.numel(), x.device
+        need = ctx.needs_input_grad
+        dx = torch.empty(x.shape, device=device, dtype=x.dtype) if need[0] else None
+        da = torch.empty(lora_a.shape, device=device, dtype=x.dtype) if need[4] else None
+        db = torch.empty(lora_b.shape, device=device, dtype=x.dtype) if need[5] else None
         if M == 0:
-            return (torch.zeros_like(x) if need_x else None, None, None, None, torch.zeros_like(lora_a) if need_a else None,
-                    torch.zeros_like(lora_b) if need_b else None, None, None, g if ctx.needs_input_grad[8] else None, None)
-        with torch.cuda.device(x.device):
-            g2 = _rows16(g)
-            ids, offsets = ids.contiguous(), None if offsets is None else offsets.contiguous()
-            if need_x or need_a:
-                # the same product on (dy, w^T, B^T, A^T): du = scale dy B_e, dx = dy w + du A_e
-                bt = _adapter_layout(_rows16(lora_b), N, R, 2)
-                at = _adapter_layout(_rows16(lora_a), K, R, 1) if need_x else None
-                dx, du = _adapter_product(g2, _rows16(ctx.w_t) if need_x else None, None, None, bt, at, ids, offsets, ctx.scale, (M, N, K, R, E, n),
-                                          need_a, need_x)
-                dx = None if dx is None else dx.view(x.shape)
-            if need_a or need_b:
-                L = _lib.lib()
-                # row ranges: enough workgroups to fill the chip (four per CU over 128-column tiles), but whole 64-row stages and few partial sums
-                tiles = (K + N + 255) // 256
-                chunk = max(128, (M * tiles // 1024 + 63) // 64 * 64)
-                plan = torch.empty(int(L.dm_adapter_plan_words(M, n, E)), device=x.device, dtype=torch.int32)
-                check(L.dm_adapter_plan(ids.data_ptr(), _ptr(offsets), n, M, E, chunk, plan.data_ptr(), _stream()), "dm_adapter_plan")
-                rp = 16 if R <= 16 else 32 if R <= 32 else 64 if R <= 64 else 128
-                part = torch.empty(int(L.dm_adapter_plan_items(M, E, chunk)) * rp * max(K if need_a else 0, N if need_b else 0), device=x.device)
-                fn, name = _sym("dm_adapter_wgrad_bf16", x.dtype)
-
-                def wgrad(X, C, uu, like, transpose):
-                    out = torch.empty(like.shape, device=like.device, dtype=like.dtype)
-                    with _Timed(f"adapter_wgrad[M={M},C={C},R={R}]", 2.0 * M * R * C):
-                        check(fn(X.data_ptr(), uu.data_ptr(), plan.data_ptr(), n, M, C, R, E, chunk, transpose, part.data_ptr(), part.numel(),
-                                 out.data_ptr(), _stream()), name)
-                    return out
-                if need_a:
-                    da = wgrad(_rows16(x), K, du, lora_a, 0)
-                if need_b:
-                    db = wgrad(g2, N, u, lora_b, 1)
-        return dx, None, None, None, da, db, None, None, (g if ctx.needs_input_grad[8] else None), None
+            da, db = (None if t is None else t.zero_() for t in (da, db))
+        elif need[0] or need[4] or need[5]:
+            fn, name = _adapter_fn(x.dtype)[1]
+            with _guard(device):
+                x, g2, lora_a, lora_b, ids = _rows16(x), _rows16(g), _rows16(lora_a), _rows16(lora_b), ids.contiguous()
+                w_t, offsets = _rows16(ctx.w_t), None if offsets is None else offsets.contiguous()
+                nb = _lib.lib().dm_linear_adapted_bwd_workspace_bytes(M, K, N, R, E, n)
+                ws = torch.empty(nb, device=device, dtype=torch.uint8)
+                with _timed(lambda: f"linear_adapted_bwd[M={M},K={K},N={N},R={R}]", 2.0 * M * (K * N + 2 * R * (K + N))):
+                    check(fn(x.data_ptr(), g2.data_ptr(), w_t.data_ptr(), lora_a.data_ptr(), lora_b.data_ptr(), ids.data_ptr(), _ptr(offsets), n, ctx.scale,
+                             u.data_ptr(), ws.data_ptr(), nb, _ptr(dx), _ptr(da), _ptr(db), M, K, N, R, E, _stream_of(device)), name)
+        return dx, None, None, None, da, db, None, None, (g if need[8] else None), None
 
 
 def linear_adapted_autograd(x, w, w_t, bias, lora_a, lora_b, ids, scale=1.0, residual=None, offsets=None):
@@ -1886,9 +1883,9 @@ def linear_adapted_autograd(x, w, w_t, bias, lora_a, lora_b, ids, scale=1.0, res
     [K, N] (prepared once by the caller, as for linear_frozen_autograd).  An adapter without rows gets a zero gradient."""
     if torch.is_grad_enabled() and (w.requires_grad or (bias is not None and bias.requires_grad)):
         raise ValueError("linear_adapted_autograd: the projection is frozen (w or bias requires a gradient)")
-    if tuple(w_t.shape) != tuple(w.shape[::-1]) or w_t.dtype != w.dtype or w_t.device != w.device:
+    if w_t.shape != w.shape[::-1] or w_t.dtype != w.dtype or w_t.device != w.device:
         raise ValueError("linear_adapted_autograd: w_t is w transposed, of its type and on its device")
-    return _LinearAdapted.apply(x, w, w_t, bias, lora_a, lora_b, ids, scale, residual, offsets)
+    return _LinearAdapted.apply(x, w, w_t, bias, lora_a, lora_b, ids, float(scale), residual, offsets)
 
 
 # ------------------------------------------------------------------------------------------ fine-tuning: norms around a block
@@ -1908,43 +1905,52 @@ def _gated_check(x, h, gate, post, pre, kind):
     if not 1 <= C <= MAX_NORM_CHANNELS:
         raise ValueError(f"gated_add_norm: {C} channels: 1 to {MAX_NORM_CHANNELS} are supported")
     item_rows = 0
-    if gate is not None and gate.dim() == 2 and x.dim() >= 2 and tuple(gate.shape) == (x.shape[0], C):
+    if gate is not None and gate.dim() == 2 and x.dim() >= 2 and gate.shape == (x.shape[0], C):
         item_rows = x.numel() // (C * x.shape[0]) if x.shape[0] else 0
         if x.shape[0] > 65000:
             raise ValueError("gated_add_norm: at most 65000 items with a gate of their own")
-    elif gate is not None and tuple(gate.shape) != (C,):
+    elif gate is not None and gate.shape != (C,):
         raise ValueError(f"gated_add_norm: gate {tuple(gate.shape)}: [C] or [items, C] with items = x.shape[0] expected")
     for name, q in (("post", post), ("pre", pre)):
-        if q is not None and (not isinstance(q, (tuple, list)) or len(q) != 2 or any(t is not None and tuple(t.shape) != (C,) for t in q)):
+        if q is None:
+            continue
+        if not isinstance(q, (tuple, list)) or len(q) != 2:
             raise ValueError(f"gated_add_norm: {name} is (gamma [C] or None, beta [C] or None)")
-    flat = [x, h, gate] + [t for q in (post, pre) if q is not None for t in q]
-    if any(t is not None and t.dtype != x.dtype for t in flat):
-        raise TypeError("gated_add_norm: tensors of one type expected")
-    _need_cuda(*flat)
-    _need_same_device(*[t for t in flat if t is not None])
+        for t in q:
+            if t is not None and t.shape != (C,):
+                raise ValueError(f"gated_add_norm: {name} is (gamma [C] or None, beta [C] or None)")
+    flat = (x, h, gate, *(post or ()), *(pre or ()))
+    for t in flat:
+        if t is not None and t.dtype != x.dtype:
+            raise TypeError("gated_add_norm: tensors of one type expected")
+    _on_one_gpu(*flat)
     return item_rows
+
+
+def _gated_forward(x, h, gate, post_g, post_b, pre_g, pre_b, flags, item_rows, scale, eps, keep):
+    """-> y, z or None, row statistics or None (keep)"""
+    post, pre, rms = flags
+    C, device = x.shape[-1], x.device
+    rows = x.numel() // C
+    y = torch.empty_like(x)
+    z = torch.empty_like(x) if pre else None
+    stats = torch.empty(rows, 4, device=device) if keep else None
+    if rows:
+        name = "dm_gated_add_norm_fwd_" + _NORM_SFX[x.dtype]
+        fn = getattr(_lib.lib(), name)
+        with _guard(device), _timed(lambda: f"gated_add_norm[C={C}]", float((4 if pre else 3) * rows * C * x.element_size())):
+            check(fn(x.data_ptr(), h.data_ptr(), _ptr(gate), item_rows, post, _ptr(post_g), _ptr(post_b), pre, _ptr(pre_g), _ptr(pre_b), y.data_ptr(), _ptr(z),
+                     _ptr(stats), rows, C, scale, eps, rms, _stream_of(device)), name)
+    return y, z, stats
 
 
 class _GatedAddNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, h, gate, post_g, post_b, pre_g, pre_b, flags, item_rows, scale, eps):
-        post, pre, rms = flags
-        x, h = x.contiguous(), h.contiguous()
-        gate, post_g, post_b, pre_g, pre_b = (None if t is None else t.contiguous() for t in (gate, post_g, post_b, pre_g, pre_b))
-        C = x.shape[-1]
-        rows = x.numel() // C
-        y = torch.empty_like(x)
-        z = torch.empty_like(x) if pre else None
-        stats = torch.empty(rows, 4, device=x.device) if any(ctx.needs_input_grad) else None
+        y, z, stats = _gated_forward(x, h, gate, post_g, post_b, pre_g, pre_b, flags, item_rows, scale, eps, True)
         ctx.save_for_backward(x, h, gate, post_g, post_b, pre_g, stats)
         ctx.args = (flags, item_rows, scale, eps, pre_b)
-        if rows == 0:
-            return (y, z) if pre else y
-        with torch.cuda.device(x.device), _Timed(f"gated_add_norm[C={C}]", float((4 if pre else 3) * rows * C * x.element_size())):
-            name = "dm_gated_add_norm_fwd_" + _NORM_SFX[x.dtype]
-            check(getattr(_lib.lib(), name)(x.data_ptr(), h.data_ptr(), _ptr(gate), item_rows, post, _ptr(post_g), _ptr(post_b), pre, _ptr(pre_g), _ptr(pre_b),
-                                            y.data_ptr(), _ptr(z), _ptr(stats), rows, C, scale, eps, rms, _stream()), name)
-        return (y, z) if pre else y
+        return y if z is None else (y, z)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -1961,13 +1967,13 @@ class _GatedAddNorm(torch.autograd.Function):
             return (dx, dh, *[None if t is None else t.zero_() for t in params], None, None, None, None)
         dy = dy.contiguous()
         dz = dz.contiguous() if pre else None
-        with torch.cuda.device(x.device), _Timed(f"gated_add_norm_bwd[C={C}]", float((6 if pre else 5) * rows * C * x.element_size())):
+        with _guard(x.device), _timed(lambda: f"gated_add_norm_bwd[C={C}]", float((6 if pre else 5) * rows * C * x.element_size())):
             words = int(_lib.lib().dm_gated_add_norm_workspace_floats(rows, item_rows, C)) if any(t is not None for t in params) else 0
             ws = torch.empty(words, device=x.device) if words else None
             name = "dm_gated_add_norm_bwd_" + _NORM_SFX[x.dtype]
             check(getattr(_lib.lib(), name)(x.data_ptr(), h.data_ptr(), _ptr(gate), item_rows, post, _ptr(post_g), _ptr(post_b), pre, _ptr(pre_g), dy.data_ptr(),
                                             _ptr(dz), stats.data_ptr(), _ptr(dx), _ptr(dh), *[_ptr(t) for t in params], _ptr(ws), words, rows, C, scale, eps,
-                                            rms, _stream()), name)
+                                            rms, _stream_of(x.device)), name)
         return (dx, dh, *params, None, None, None, None)
 
 
@@ -1979,10 +1985,13 @@ def gated_add_norm(x, h, gate=None, post=None, pre=None, scale=1.0, eps=1e-5, ki
     be None inside; kind "layer" (mean and variance) or "rms".  -> y, or (y, z) with pre.  Statistics and sums in fp32; z is formed from the
     unrounded y."""
     item_rows = _gated_check(x, h, gate, post, pre, kind)
-    pg, pb = post if post is not None else (None, None)
-    qg, qb = pre if pre is not None else (None, None)
-    return _GatedAddNorm.apply(x, h, gate, pg, pb, qg, qb, (int(post is not None), int(pre is not None), int(kind == "rms")), item_rows, float(scale),
-                               float(eps))
+    flat = [x, h, gate, *(post or (None, None)), *(pre or (None, None))]
+    flat = [t if t is None or t.is_contiguous() else t.contiguous() for t in flat]
+    flags, scale, eps = (int(post is not None), int(pre is not None), int(kind == "rms")), float(scale), float(eps)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in flat):
+        return _GatedAddNorm.apply(*flat, flags, item_rows, scale, eps)
+    y, z, _ = _gated_forward(*flat, flags, item_rows, scale, eps, False)
+    return y if z is None else (y, z)
 
 
 # ------------------------------------------------------------------------------------------ fine-tuning: orthogonalised updates
@@ -2020,10 +2029,10 @@ def orthogonalize(g, steps=5, eps=1e-7):
     g = g.detach().contiguous()
     out = torch.empty_like(g)
     gs, outs = g.view(-1, rows, cols), out.view(-1, rows, cols)
-    with torch.cuda.device(g.device):
+    with _guard(g.device):
         ws = _ns_workspace(gs.shape[0], rows, cols, g.device)
         check(_lib.lib().dm_orthogonalize(_ptr_array(list(gs)), _ptr_array(list(outs)), gs.shape[0], rows, cols, _NS_DTYPES[g.dtype], int(steps), float(eps),
-                                          ws.data_ptr(), ws.numel(), _stream()), "dm_orthogonalize")
+                                          ws.data_ptr(), ws.numel(), _stream_of(g.device)), "dm_orthogonalize")
     return out
 
 
@@ -2062,15 +2071,14 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
         raise ValueError("muon_step: a parameter or momentum buffer occurs twice")
     for (rows, cols, dtype, device), v in groups.items():
         for p, g, m in v:
-            _need_cuda(p, g, m)
-            _need_same_device(p, g, m)
+            _on_one_gpu(p, g, m)
     for (rows, cols, dtype, device), v in groups.items():
         s = 0.2 * max(rows, cols) ** 0.5 if scale == "rms" else max(1.0, rows / cols) ** 0.5 if scale == "spectral" else float(scale)
         gs = [g.detach().contiguous() for _, g, _ in v]
-        with torch.cuda.device(device):
+        with _guard(device):
             ws = _ns_workspace(len(v), rows, cols, device)
             check(_lib.lib().dm_muon_step(_ptr_array(gs), _ptr_array([m for _, _, m in v]), _ptr_array([p for p, _, _ in v]), len(v), rows, cols,
                                           _NS_DTYPES[dtype], int(steps), float(momentum), int(bool(nesterov)), float(eps), float(1.0 - lr * weight_decay),
-                                          float(lr * s), ws.data_ptr(), ws.numel(), _stream()), "dm_muon_step")
+                                          float(lr * s), ws.data_ptr(), ws.numel(), _stream_of(device)), "dm_muon_step")
     if live:
         torch.autograd.graph.increment_version(live)      # caches keyed on a parameter's version see the update

@@ -552,31 +552,25 @@ int dm_gated_add_norm_bwd_f32(const void* x, const void* h, const void* gate, lo
 
 /* Low-rank adapters of many requests beside a frozen projection (csrc/adapters.hip); the _f16 forms take IEEE half.
  *   y = x w^T + bias + scale (x A_e^T) B_e^T + residual,   e = ids[request of the row]
- * x [M, K], w [N, K], bias [N] / residual [M, N] or NULL, lora_a [E, R, K], lora_b [E, N] rows of R <= 128 elements ldb apart; ids int32 [n];
- * offsets int32 [n + 1], ascending, or NULL (n requests of M / n rows).  Rows of no request and ids outside [0, E) have no adapter.
- * K, N, ldb multiples of 8, pointers 16-byte aligned.  u: scratch of dm_adapter_u_bytes(M, R); keep_u != 0 leaves scale x A^T in it for
- * dm_adapter_wgrad_* (and y = NULL computes only that). */
-size_t dm_adapter_u_bytes(long long M, int R);
-int dm_linear_adapted_bf16(const void* x, const void* w, const void* bias, const void* residual, const void* lora_a, const void* lora_b, int ldb,
-                           const int32_t* ids, const int32_t* offsets, long long n, float scale, void* u, size_t u_bytes, void* y, long long M, int K,
+ * x [M, K], w [N, K], bias [N] / residual [M, N] or NULL, lora_a [E, R, K], lora_b [E, N, R], R <= 128; ids int32 [n]; offsets int32 [n + 1],
+ * ascending, or NULL (n requests of M / n rows).  Rows of no request and ids outside [0, E) have no adapter.  K, N multiples of 8, pointers
+ * 16-byte aligned.  ws: dm_linear_adapted_workspace_bytes; keep_u != 0 leaves scale x A^T in it for the backward. */
+size_t dm_linear_adapted_workspace_bytes(long long M, int N, int R, int E);
+int dm_linear_adapted_bf16(const void* x, const void* w, const void* bias, const void* residual, const void* lora_a, const void* lora_b,
+                           const int32_t* ids, const int32_t* offsets, long long n, float scale, void* ws, size_t ws_bytes, void* y, long long M, int K,
                            int N, int R, int E, int keep_u, dm_stream_t stream);
-int dm_linear_adapted_f16(const void* x, const void* w, const void* bias, const void* residual, const void* lora_a, const void* lora_b, int ldb,
-                          const int32_t* ids, const int32_t* offsets, long long n, float scale, void* u, size_t u_bytes, void* y, long long M, int K,
+int dm_linear_adapted_f16(const void* x, const void* w, const void* bias, const void* residual, const void* lora_a, const void* lora_b,
+                          const int32_t* ids, const int32_t* offsets, long long n, float scale, void* ws, size_t ws_bytes, void* y, long long M, int K,
                           int N, int R, int E, int keep_u, dm_stream_t stream);
-/* layouts of the adapters: mode 0 copies src [E, C, R] to rows padded to 16 | 32 | 64 | 128 ranks (zeros), mode 1 the same from src [E, R, C],
- * mode 2 transposes src [E, C, R] to [E, R, C] */
-int dm_adapter_layout_bf16(const void* src, void* dst, int E, int C, int R, int mode, dm_stream_t stream);
-int dm_adapter_layout_f16(const void* src, void* dst, int E, int C, int R, int mode, dm_stream_t stream);
-/* weight gradients: out[e] = sum over the rows of adapter e of u^T X ([E, R, C], or [E, C, R] with transpose); plan = the rows in adapter order,
- * dm_adapter_plan_words int32, built by dm_adapter_plan for items of `chunk` rows (a multiple of 64); part fp32
- * [dm_adapter_plan_items][padded rank][C] */
-size_t dm_adapter_plan_words(long long M, long long n, int E);
-long long dm_adapter_plan_items(long long M, int E, int chunk);
-int dm_adapter_plan(const int32_t* ids, const int32_t* offsets, long long n, long long M, int E, int chunk, int32_t* plan, dm_stream_t stream);
-int dm_adapter_wgrad_bf16(const void* X, const void* u, const int32_t* plan, long long n, long long M, int C, int R, int E, int chunk, int transpose,
-                          float* part, size_t part_floats, void* out, dm_stream_t stream);
-int dm_adapter_wgrad_f16(const void* X, const void* u, const int32_t* plan, long long n, long long M, int C, int R, int E, int chunk, int transpose,
-                         float* part, size_t part_floats, void* out, dm_stream_t stream);
+/* the gradients, each NULL if not wanted: dx [M, K] (w_t = w transposed [K, N]), da [E, R, K], db [E, N, R] (u = the forward's ws with keep_u);
+ * an adapter without rows gets zeros.  Sums in a fixed order. */
+size_t dm_linear_adapted_bwd_workspace_bytes(long long M, int K, int N, int R, int E, long long n);
+int dm_linear_adapted_bwd_bf16(const void* x, const void* dy, const void* w_t, const void* lora_a, const void* lora_b, const int32_t* ids,
+                               const int32_t* offsets, long long n, float scale, const void* u, void* ws, size_t ws_bytes, void* dx, void* da, void* db,
+                               long long M, int K, int N, int R, int E, dm_stream_t stream);
+int dm_linear_adapted_bwd_f16(const void* x, const void* dy, const void* w_t, const void* lora_a, const void* lora_b, const int32_t* ids,
+                              const int32_t* offsets, long long n, float scale, const void* u, void* ws, size_t ws_bytes, void* dx, void* da, void* db,
+                              long long M, int K, int N, int R, int E, dm_stream_t stream);
 
 /* Orthogonalised updates by Newton-Schulz products (csrc/newton_schulz.hip).  `count` matrices [rows, cols], contiguous, behind HOST arrays
  * of device pointers; dtype of g and out: 0 bf16 | 1 half | 2 fp32.  dm_muon_step (mom, p fp32): mom <- mu mom + g; u = g + mu mom (nesterov)

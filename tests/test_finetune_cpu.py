@@ -118,20 +118,21 @@ def test_c_entries_refuse_before_any_launch():
     ARG, WS, UNS = -1, -2, -3
     P = 1 << 12                                                                       # an aligned address that no check dereferences
 
-    def lin(x=P, ldb=16, ids=P, offsets=None, n=2, u=P, ub=1 << 20, y=P, M=4, K=64, N=64, R=16, E=1, keep=0, w=P, b=P):
-        return L.dm_linear_adapted_bf16(x, w, None, None, P, b, ldb, ids, offsets, n, 1.0, u, ub, y, M, K, N, R, E, keep, None)
+    def lin(x=P, w=P, b=P, ids=P, offsets=None, n=2, ws=P, wb=1 << 20, y=P, M=4, K=64, N=64, R=16, E=1, res=None):
+        return L.dm_linear_adapted_bf16(x, w, None, res, P, b, ids, offsets, n, 1.0, ws, wb, y, M, K, N, R, E, 0, None)
     for kw, rc in [(dict(x=None), ARG), (dict(ids=None), ARG), (dict(n=0), ARG), (dict(n=3), ARG), (dict(E=0), ARG), (dict(R=0), ARG), (dict(K=0), ARG),
-                   (dict(w=None), ARG), (dict(b=None), ARG), (dict(y=None), ARG), (dict(u=None), ARG), (dict(x=P + 2), ARG), (dict(ldb=8), ARG), (dict(M=-4), ARG),
-                   (dict(R=129, ldb=136), UNS), (dict(K=60), UNS), (dict(N=60), UNS), (dict(ldb=20), UNS), (dict(ub=16), WS)]:
+                   (dict(w=None), ARG), (dict(b=None), ARG), (dict(y=None), ARG), (dict(ws=None), ARG), (dict(x=P + 2), ARG), (dict(res=P + 2), ARG),
+                   (dict(M=-4), ARG), (dict(R=129), UNS), (dict(K=60), UNS), (dict(N=60), UNS), (dict(E=70000), UNS), (dict(wb=16), WS),
+                   (dict(R=12, wb=4 * 68 + 64), WS)]:
         assert lin(**kw) == rc, kw
     assert lin(M=0) == 0
 
-    def wg(X=P, chunk=128, part=1 << 20, M=4, C=64, R=16, E=1):
-        return L.dm_adapter_wgrad_f16(X, P, P, 2, M, C, R, E, chunk, 0, P, part, P, None)
-    for kw, rc in [(dict(X=None), ARG), (dict(X=P + 2), ARG), (dict(chunk=100), ARG), (dict(M=0), ARG), (dict(C=60), UNS), (dict(R=200), UNS), (dict(part=10), WS)]:
-        assert wg(**kw) == rc, kw
-    assert L.dm_adapter_plan(P, None, 2, 4, 1, 100, P, None) == ARG and L.dm_adapter_plan(P, None, 3, 4, 1, 128, P, None) == ARG
-    assert L.dm_adapter_layout_bf16(P, P, 1, 8, 8, 3, None) == ARG and L.dm_adapter_layout_bf16(P, P, 1, 8, 129, 0, None) == UNS
+    def bwd(x=P, dy=P, wt=P, u=P, ws=P, wb=1 << 30, dx=P, da=P, db=P, M=4, K=64, N=64, R=16, E=1, n=2):
+        return L.dm_linear_adapted_bwd_f16(x, dy, wt, P, P, P, None, n, 1.0, u, ws, wb, dx, da, db, M, K, N, R, E, None)
+    need = L.dm_linear_adapted_bwd_workspace_bytes(4, 64, 64, 16, 1, 2)
+    for kw, rc in [(dict(x=None), ARG), (dict(dy=None), ARG), (dict(wt=None), ARG), (dict(u=None), ARG), (dict(ws=None), ARG), (dict(M=0), ARG), (dict(n=3), ARG),
+                   (dict(dx=P + 2), ARG), (dict(K=60), UNS), (dict(R=200), UNS), (dict(wb=need - 1), WS)]:
+        assert bwd(**kw) == rc, kw
 
     def norm(x=P, rows=6, items=0, C=64, gate=None, pre=0, z=None, stats=None):
         return L.dm_gated_add_norm_fwd_f32(x, P, gate, items, 0, None, None, pre, None, None, P, z, stats, rows, C, 1.0, 1e-5, 0, None)
@@ -139,8 +140,8 @@ def test_c_entries_refuse_before_any_launch():
                    (dict(gate=P, items=4), ARG)]:
         assert norm(**kw) == rc, kw
     assert norm(rows=0) == 0
-    bwd = lambda ws, words, **k: L.dm_gated_add_norm_bwd_bf16(P, P, P, 2, 1, P, P, 0, None, P, None, P, P, P, P, P, P, None, None, ws, words, 6, 64, 1.0, 1e-5, 0, None)
-    assert bwd(None, 0) == WS and bwd(P, 100) == WS
+    nbwd = lambda ws, words: L.dm_gated_add_norm_bwd_bf16(P, P, P, 2, 1, P, P, 0, None, P, None, P, P, P, P, P, P, None, None, ws, words, 6, 64, 1.0, 1e-5, 0, None)
+    assert nbwd(None, 0) == WS and nbwd(P, 100) == WS
 
     import ctypes
     ptrs = (ctypes.c_void_p * 1)(P)
@@ -156,11 +157,13 @@ def test_c_entries_refuse_before_any_launch():
 
 def test_size_queries():
     L = _lib.lib()
-    assert [L.dm_adapter_u_bytes(10, r) for r in (1, 16, 17, 33, 128)] == [10 * (4 * p + 4) for p in (16, 16, 32, 64, 128)]
-    assert L.dm_adapter_u_bytes(0, 4) == L.dm_adapter_u_bytes(4, 129) == 0
-    # every adapter may end inside an item: full items and one more each, but never more items than rows
-    assert L.dm_adapter_plan_items(1000, 3, 128) == 7 + 3 and L.dm_adapter_plan_items(2, 9, 128) == 2
-    assert L.dm_adapter_plan_words(100, 7, 3) == 2 * 4 + 7 + 100
+    up = lambda v: (v + 255) // 256 * 256
+    u = lambda M, r: up(M * (4 * r + 4))                                             # pairs of 16-bit columns (padded rank), a scale per row
+    assert [L.dm_linear_adapted_workspace_bytes(10, 64, r, 3) for r in (16, 24, 64, 128)] == [u(10, p) for p in (16, 32, 64, 128)]
+    assert [L.dm_linear_adapted_workspace_bytes(10, 64, r, 3) for r in (1, 33)] == [u(10, p) + 2 * 3 * 64 * p for p in (16, 64)]      # + B in padded rows
+    assert L.dm_linear_adapted_workspace_bytes(0, 64, 16, 1) == L.dm_linear_adapted_workspace_bytes(4, 64, 129, 1) == 0
+    # every adapter may end inside an item of 128 rows: full items and one more each
+    assert L.dm_linear_adapted_bwd_workspace_bytes(1000, 64, 72, 16, 3, 7) == u(1000, 16) + up(2 * 3 * 64 * 16) + up(2 * 3 * 72 * 16) + up(4 * (8 + 7 + 1000)) + 4 * 10 * 16 * 136
     assert L.dm_orthogonalize_workspace_bytes(40, 65, 10) == 16 * L.dm_orthogonalize_workspace_bytes(1, 65, 10)
     assert L.dm_gated_add_norm_workspace_floats(0, 0, 8) == 0 and L.dm_gated_add_norm_workspace_floats(6, 2, 8) == (5 + 3) * 8
 

@@ -14,7 +14,9 @@
 // therefore kept as a PAIR of halves, value + rest (22 bits; scaled by 2^13, so that neither leaves half's range: |X| <= 1.2, |S| <=
 // 1.5, |P| <= 2.9), and a product is value value + value rest + rest value with fp32 sums: the result agrees with fp32 arithmetic to its
 // own rounding (1.7e-6 against 1.7e-6 of the fp32 form on a 1024^2 Gaussian).  For bf16 input the last two iterations, whose
-// errors are hardly amplified any more, take the values only: 0.6e-3 of error under the 1.7e-3 of the rounding to bf16.
+// errors are hardly amplified any more, take (and are given) the values only: 1e-3 of error under the 1.7e-3 of the rounding to bf16.
+// (Taking the polynomials of S = X X^T alone and multiplying X0 once saves half the products of a wide matrix, but S holds squared singular
+// values: on the gradients of a small ControlNet, which a few directions dominate, the result was 1e-3 to 1e-2 off where this form is 3e-5.)
 // Pairs are stored as 128-byte blocks, 32 values then their 32 rests: a K step of the paired product loads the same lines as a K
 // step of 64 plain halves.
 #include <algorithm>
@@ -173,10 +175,6 @@ __global__ __launch_bounds__(256) void k_ns_pack(NsArgs a) {
     }
 }
 
-enum { NS_GRAM = 0, NS_POLY = 1, NS_STEP = 2, NS_LAST = 3 };
-
-// A T x T tile of pairs in LDS: 128-byte blocks [row][T / 32], the two blocks of a 256-byte line swapped and the 16-byte chunks of a block
-// XOR-ed by the row: the accumulator's layout (a lane owns a row), rows (the copy-out) and the transposing reads all spread over the banks.
 constexpr int threads_of(int T) { return T == 256 ? 512 : 256; }
 
 template <int T>
@@ -184,39 +182,52 @@ __device__ __forceinline__ int tile_at(int row, int blk, int chunk) {
     return (row * (T / 32) + (blk ^ ((row >> 3) & 1))) * 128 + ((chunk ^ (row & 7)) << 4);
 }
 
-// C[i, j] = sum_k A[i, k] B[j, k] over pair matrices, tile T x T, two rows of WJ waves of T/2 x T/WJ.  K goes in blocks of 32 pairs = 128 bytes per
-// row through a ring of NST LDS stages filled by buffer_load ... lds (chunks XOR-swizzled by (row >> 1) & 7), NST - 1 of them in flight.
-// PAIR: three products per block, else the values only (half of the loaded bytes; the block layout stays).
-//   GRAM  A = B = X,          S = C                       (tiles i >= j, stored twice)
-//   POLY  A = B = S,          P = b S + c C               (tiles i >= j, stored twice)
-//   STEP  A = P, B = X^T,     X <- a X + C  in both orientations (X in place: a tile is read and written by its own workgroup only)
-//   LAST  the same, into the parameter or the output
-// The epilogue goes through LDS: the tile of S or X arrives as whole lines, every lane replaces its own entries, and whole lines leave in
-// both orientations (the transposed one by ds_read_b64_tr_b16); a 256 tile does that half by half.
+// One launch: D = src_c * src + acc_c * (A B^T) for `count` matrices
+struct Product {
+    const _Float16 *A, *B;           // [a_rows][kw], [b_rows][kw] pairs
+    const _Float16* src;             // [a_rows][b_rows] pairs (SRC)
+    _Float16* D;                     // the result as pairs [a_rows][b_rows]; symmetric: both halves of it
+    _Float16* E;                     // not symmetric: the result transposed [b_rows][a_rows]
+    int a_rows, b_rows, kw;          // padded
+    float src_c, acc_c;
+    int src_rests, rests;            // whether the source has rests, whether the result needs them (its readers take pairs)
+    int tiles_i, tiles_j, count;
+    int mode, splits;
+};
+
+// Tile T x T, two rows of WJ waves of T/2 x T/WJ.  K goes in blocks of 128 bytes per row through a ring of NST LDS stages filled by
+// buffer_load ... lds (chunks XOR-swizzled by (row >> 1) & 7), NST - 1 of them in flight: 32 pairs (PAIR: three products per block) or the
+// values of 64.
+//   SYM   A B^T is symmetric: tiles i >= j, stored twice
+//   SRC   the result adds src_c src (SYM: another matrix; else the matrix that D replaces, read and written by its own workgroup only)
+//   LAST  the result goes into the parameter or the output instead of pairs
+// The epilogue goes through LDS: the source tile arrives as whole lines, every lane replaces its own entries, and whole lines leave in both
+// orientations (the transposed one by ds_read_b64_tr_b16); a 256 tile does that half by half.
 // mode 0: the whole product.  1: this workgroup's share (blockIdx.z) of a split contraction, fp32 sums to a.part.  2: joins those shares.
-template <int KIND, int T, int NST, bool PAIR, typename OT>
-__global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, int in, int tiles_i, int tiles_j, int count, int mode, int splits) {
+template <int T, int NST, bool PAIR, bool SYM, bool SRC, bool LAST, typename OT>
+__global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Product g) {
     [[maybe_unused]] constexpr int NT = threads_of(T), NW = NT / 64, WJ = NW / 2, ROWB = 128, STAGE = 2 * T * ROWB, TI = T / 2, TJ = T / WJ, FI = TI / 32, FJ = TJ / 32,
                                    PIECES = T / 8 / NW, H = T == 256 ? 2 : 1, TR = T / H;       // TR rows per epilogue pass
     extern __shared__ __attribute__((aligned(16))) char smem[];      // max(NST * STAGE, 4 TR T)
 #if defined(__HIP_DEVICE_COMPILE__)
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, hi = lane >> 5, l31 = lane & 31;
     const int wi = wave / WJ, wj = wave % WJ;
+    const int mode = g.mode, splits = g.splits;
     // XCD-contiguous tile order (block b runs on XCD b % 8), matrix by matrix
-    const int per_mat = KIND <= NS_POLY ? tiles_i * (tiles_i + 1) / 2 : tiles_i * tiles_j;
-    const int total = per_mat * count, per = (total + 7) / 8;
+    const int per_mat = SYM ? g.tiles_i * (g.tiles_i + 1) / 2 : g.tiles_i * g.tiles_j;
+    const int total = per_mat * g.count, per = (total + 7) / 8;
     const int id = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
-    if (id >= total) return;
+    if ((int)(blockIdx.x >> 3) >= per || id >= total) return;
     const int b = id / per_mat, rem = id - b * per_mat;
     int ti, tj;
-    if constexpr (KIND <= NS_POLY) {
+    if constexpr (SYM) {
         ti = (int)((sqrtf(8.f * (float)rem + 1.f) - 1.f) * 0.5f);
         while ((ti + 1) * (ti + 2) / 2 <= rem) ++ti;
         while (ti * (ti + 1) / 2 > rem) --ti;
         tj = rem - ti * (ti + 1) / 2;
     } else {
-        ti = rem % tiles_i;                     // the row tiles of one X^T panel side by side
-        tj = rem / tiles_i;
+        ti = rem % g.tiles_i;                   // the row tiles of one panel of B side by side
+        tj = rem / g.tiles_i;
     }
     const int i0 = ti * T, j0 = tj * T;
     f32x16 acc[FI][FJ];
@@ -226,36 +237,37 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, int in, int
 #pragma unroll
             for (int j = 0; j < FJ; ++j)
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const float4* p = reinterpret_cast<const float4*>(a.part) + ((long long)id * splits * FI * FJ * 4 + (i * FJ + j) * 4 + g) * NT + tid;
+                for (int q = 0; q < 4; ++q) {
+                    const float4* p = reinterpret_cast<const float4*>(a.part) + ((long long)id * splits * FI * FJ * 4 + (i * FJ + j) * 4 + q) * NT + tid;
                     float4 v = p[0];
                     for (int z = 1; z < splits; ++z) {
-                        const float4 w = p[(long long)z * FI * FJ * 4 * NT];
-                        v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+                        const float4 o = p[(long long)z * FI * FJ * 4 * NT];
+                        v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
                     }
-                    acc[i][j][4 * g] = v.x; acc[i][j][4 * g + 1] = v.y; acc[i][j][4 * g + 2] = v.z; acc[i][j][4 * g + 3] = v.w;
+                    acc[i][j][4 * q] = v.x; acc[i][j][4 * q + 1] = v.y; acc[i][j][4 * q + 2] = v.z; acc[i][j][4 * q + 3] = v.w;
                 }
     } else {
-        const int kw = KIND == NS_GRAM ? a.np : a.mp;              // contraction width (padded)
-        const _Float16* A = KIND == NS_GRAM ? a.x + (long long)b * a.mp * 2 * a.np : (KIND == NS_POLY ? a.s : a.pm) + (long long)b * a.mp * 2 * a.mp;
-        const _Float16* B = KIND <= NS_POLY ? A : a.xt[in] + (long long)b * a.np * 2 * a.mp;
-        const int arows = min(T, a.mp - i0), brows = min(T, (KIND <= NS_POLY ? a.mp : a.np) - j0);
+        const int kw = g.kw;
+        const _Float16* A = g.A + (long long)b * g.a_rows * 2 * kw;
+        const _Float16* B = g.B + (long long)b * g.b_rows * 2 * kw;
+        const int arows = min(T, g.a_rows - i0), brows = min(T, g.b_rows - j0);
         const __amdgpu_buffer_rsrc_t ars = __builtin_amdgcn_make_buffer_rsrc((void*)(A + (long long)i0 * 2 * kw), 0, arows * kw * 4, 0x00020000);
         const __amdgpu_buffer_rsrc_t brs = __builtin_amdgcn_make_buffer_rsrc((void*)(B + (long long)j0 * 2 * kw), 0, brows * kw * 4, 0x00020000);
         unsigned off[PIECES];                                      // rows past the matrix lie past the descriptor: zeros
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
             const int row = wave * (T / NW) + 8 * p + (lane >> 3);
-            off[p] = (unsigned)row * (unsigned)kw * 4u + (unsigned)(((lane & 7) ^ ((row >> 1) & 7)) * 16);
+            const int chunk = (lane & 7) ^ ((row >> 1) & 7);       // (values only: chunks 4 .. 7 are the next block's values)
+            off[p] = (unsigned)row * (unsigned)kw * 4u + (unsigned)(PAIR ? chunk * 16 : (chunk >> 2) * 128 + (chunk & 3) * 16);
         }
         auto issue = [&](int s, int stage) __attribute__((always_inline)) {
             char* base = smem + stage * STAGE;
 #pragma unroll
             for (int p = 0; p < PIECES; ++p)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(ars, (__attribute__((address_space(3))) void*)(base + (wave * (T / NW) + 8 * p) * ROWB), 16, (int)off[p], s * 128, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(ars, (__attribute__((address_space(3))) void*)(base + (wave * (T / NW) + 8 * p) * ROWB), 16, (int)off[p], s * (PAIR ? 128 : 256), 0, 0);
 #pragma unroll
             for (int p = 0; p < PIECES; ++p)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(brs, (__attribute__((address_space(3))) void*)(base + T * ROWB + (wave * (T / NW) + 8 * p) * ROWB), 16, (int)off[p], s * 128, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(brs, (__attribute__((address_space(3))) void*)(base + T * ROWB + (wave * (T / NW) + 8 * p) * ROWB), 16, (int)off[p], s * (PAIR ? 128 : 256), 0, 0);
         };
 #pragma unroll
         for (int i = 0; i < FI; ++i)
@@ -266,7 +278,7 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, int in, int
         auto frag = [&](const char* base, int row, int chunk) __attribute__((always_inline)) {
             return *reinterpret_cast<const half8*>(base + row * ROWB + ((chunk ^ ((row >> 1) & 7)) << 4));
         };
-        const int all = kw / 32;
+        const int all = kw / (PAIR ? 32 : 64);
         const int s_lo = mode == 1 ? (int)((long long)all * blockIdx.z / splits) : 0, s_hi = mode == 1 ? (int)((long long)all * (blockIdx.z + 1) / splits) : all;
 #pragma unroll
         for (int q = 0; q < NST - 1; ++q)
@@ -283,7 +295,7 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, int in, int
             const char* ab = smem + st * STAGE;
             const char* bb = ab + T * ROWB;
 #pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
+            for (int kk = 0; kk < (PAIR ? 2 : 4); ++kk) {
                 half8 ah[FI], al[FI], bh[FJ], bl[FJ];
 #pragma unroll
                 for (int i = 0; i < FI; ++i) {
@@ -317,28 +329,29 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, int in, int
 #pragma unroll
                 for (int j = 0; j < FJ; ++j)
 #pragma unroll
-                    for (int g = 0; g < 4; ++g)
-                        reinterpret_cast<float4*>(a.part)[(((long long)id * splits + blockIdx.z) * FI * FJ * 4 + (i * FJ + j) * 4 + g) * NT + tid] =
-                            make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
+                    for (int q = 0; q < 4; ++q)
+                        reinterpret_cast<float4*>(a.part)[(((long long)id * splits + blockIdx.z) * FI * FJ * 4 + (i * FJ + j) * 4 + q) * NT + tid] =
+                            make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
             return;
         }
     }
 
     // ---- epilogue.  lane: row i = l31 of the fragment, registers 4 g + r: columns 8 g + 4 hi + r
     typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-    const int ow = KIND <= NS_POLY ? a.mp : a.np, oh = a.mp;
+    const int ow = g.b_rows, oh = g.a_rows;
     for (int h = 0; h < H; ++h) {
         const int r0 = i0 + h * TR;                                    // first row of this pass
         if (h && r0 >= oh) break;
         __syncthreads();                                               // every wave has read its last fragments (its share of the last pass)
-        if constexpr (KIND != NS_GRAM) {
+        if constexpr (SRC) {
             constexpr int P = TR * T / 256 / NW;                       // 1 KB = 8 blocks per wave and request
-            const _Float16* src = KIND == NS_POLY ? a.s + (long long)b * a.mp * 2 * a.mp : a.x + (long long)b * a.mp * 2 * a.np;
+            const _Float16* src = g.src + (long long)b * oh * 2 * ow;
             const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(src + (long long)r0 * 2 * ow), 0, min(TR, oh - r0) * ow * 4, 0x00020000);
 #pragma unroll
             for (int p = 0; p < P; ++p) {
                 const int q = (wave * P + p) * 8 + (lane >> 3), row = q / (T / 32), blk = (q % (T / 32)) ^ ((row >> 3) & 1);
-                const unsigned o = (unsigned)row * (unsigned)ow * 4u + (unsigned)((j0 / 32 + blk) * 128 + (((lane & 7) ^ (row & 7)) << 4));
+                const int chunk = (lane & 7) ^ (row & 7);
+                const unsigned o = chunk < 4 || g.src_rests ? (unsigned)row * (unsigned)ow * 4u + (unsigned)((j0 / 32 + blk) * 128 + (chunk << 4)) : 0x80000000u;
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(smem + (wave * P + p) * 1024), 16, (int)o, 0, 0, 0);
             }
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -350,32 +363,29 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, int in, int
 #pragma unroll
                 for (int fj = 0; fj < FJ; ++fj)
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
+                    for (int q = 0; q < 4; ++q) {
                         const int row = (H == 1 ? TI * wi : 0) + 32 * fi + l31, blk = (TJ * wj) / 32 + fj;
-                        half4* vp = reinterpret_cast<half4*>(smem + tile_at<T>(row, blk, g) + 8 * hi);
-                        half4* rp = reinterpret_cast<half4*>(smem + tile_at<T>(row, blk, 4 + g) + 8 * hi);
+                        half4* vp = reinterpret_cast<half4*>(smem + tile_at<T>(row, blk, q) + 8 * hi);
+                        half4* rp = reinterpret_cast<half4*>(smem + tile_at<T>(row, blk, 4 + q) + 8 * hi);
                         float v[4];
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) v[r] = acc[fi][fj][4 * g + r] * kInv;
-                        if constexpr (KIND != NS_GRAM) {
+                        for (int r = 0; r < 4; ++r) v[r] = acc[fi][fj][4 * q + r] * g.acc_c;
+                        if constexpr (SRC) {
                             const half4 hv = *vp, lv = *rp;
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                const float old = (float)hv[r] + (float)lv[r];
-                                v[r] = KIND == NS_POLY ? kB * old + kC * v[r] : kA * old + v[r];
-                            }
+                            for (int r = 0; r < 4; ++r) v[r] += g.src_c * ((float)hv[r] + (float)lv[r]);
                         }
-                        if constexpr (KIND == NS_LAST) {               // fp32 in the pair's place: columns 0, 1 | 2, 3 of the four
-                            *reinterpret_cast<float2*>(vp) = make_float2(v[0] * kInv, v[1] * kInv);
-                            *reinterpret_cast<float2*>(rp) = make_float2(v[2] * kInv, v[3] * kInv);
+                        if constexpr (LAST) {                          // fp32 in the pair's place: columns 0, 1 | 2, 3 of the four
+                            *reinterpret_cast<float2*>(vp) = make_float2(v[0], v[1]);
+                            *reinterpret_cast<float2*>(rp) = make_float2(v[2], v[3]);
                         } else {
                             half4 hv, lv;
 #pragma unroll
                             for (int r = 0; r < 4; ++r) {
-                                _Float16 p, q;
-                                split(v[r], p, q);
-                                hv[r] = p;
-                                lv[r] = q;
+                                _Float16 x, y;
+                                split(v[r], x, y);
+                                hv[r] = x;
+                                lv[r] = y;
                             }
                             *vp = hv;
                             *rp = lv;
@@ -383,7 +393,7 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, int in, int
                     }
         }
         __syncthreads();
-        if constexpr (KIND == NS_LAST) {
+        if constexpr (LAST) {
             float* p = a.t.p[b];
             OT* out = reinterpret_cast<OT*>(a.t.out[b]);
             // four entries per thread along the fast axis of the matrix as given, a batch of loads in flight
@@ -437,26 +447,26 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, int in, int
                 }
             }
         } else {
-            _Float16* D = (KIND == NS_GRAM ? a.s : KIND == NS_POLY ? a.pm : a.x) + (long long)b * oh * 2 * ow;
+            _Float16* D = g.D + (long long)b * oh * 2 * ow;
 #pragma unroll 4
             for (int q = tid; q < TR * T / 4; q += NT) {               // 16-byte chunks, whole rows of blocks
                 const int chunk = q & 7, blk = (q >> 3) % (T / 32), row = (q >> 3) / (T / 32);
-                if (r0 + row < oh && j0 + 32 * blk < ow)
+                if (r0 + row < oh && j0 + 32 * blk < ow && (chunk < 4 || g.rests))
                     *reinterpret_cast<u32x4*>(D + (long long)(r0 + row) * 2 * ow + (j0 / 32 + blk) * 64 + chunk * 8) =
                         *reinterpret_cast<const u32x4*>(smem + tile_at<T>(row, blk, chunk));
             }
-            if (KIND == NS_STEP || ti != tj) {                         // the other orientation: rows j, blocks of 32 i
-                _Float16* E = KIND == NS_STEP ? a.xt[in ^ 1] + (long long)b * a.np * 2 * a.mp : D;
+            if (!SYM || ti != tj) {                                    // the other orientation: rows j, blocks of 32 i
+                _Float16* E = SYM ? D : g.E + (long long)b * ow * 2 * oh;
                 const int l15 = lane & 15, grp = lane >> 4;
-                for (int u = wave; u < (T / 16) * (TR / 32) * 2; u += NW) {
-                    const int part = u & 1, ib = (u >> 1) % (TR / 32), c0 = (u >> 1) / (TR / 32) * 16;
+                for (int u = wave; u < (T / 16) * (TR / 32) * (1 + g.rests); u += NW) {
+                    const int part = g.rests ? u & 1 : 0, v = u >> g.rests, ib = v % (TR / 32), c0 = v / (TR / 32) * 16;
                     const int row = 32 * ib + 8 * grp + (l15 >> 2), cc = (c0 & 31) + 4 * (l15 & 3);
                     const char* p0 = smem + tile_at<T>(row, c0 >> 5, (cc >> 3) + 4 * part) + ((cc & 4) << 1);
                     const char* p1 = smem + tile_at<T>(row + 4, c0 >> 5, (cc >> 3) + 4 * part) + ((cc & 4) << 1);
                     const elem4 q0 = dm_ds_read_tr16_b64(p0), q1 = dm_ds_read_tr16_b64(p1);
                     const elem8 o = {q0[0], q0[1], q0[2], q0[3], q1[0], q1[1], q1[2], q1[3]};
                     const int j = j0 + c0 + l15, i = r0 + 32 * ib;
-                    if (j < ow && i < oh) *reinterpret_cast<elem8*>(E + pair_at(j, i, a.mp) + 8 * grp + 32 * part) = o;
+                    if (j < ow && i < oh) *reinterpret_cast<elem8*>(E + pair_at(j, i, oh) + 8 * grp + 32 * part) = o;
                 }
             }
         }
@@ -474,7 +484,7 @@ int gram_splits(int mp, int np, int count) {
     return std::max(1, std::min(kSplitTiles / tiles, np / 32 / 16));
 }
 
-// bytes of one matrix's workspace; of the split's partial sums
+// bytes of one matrix's workspace (x, two x^T, s, p); of the split's partial sums
 long long mat_bytes(long long rows, long long cols) {
     const long long m = pad64(std::min(rows, cols)), n = pad64(std::max(rows, cols));
     return 4 * (3 * m * n + 2 * m * m) + 8 * kNormParts;
@@ -484,15 +494,17 @@ long long part_bytes(long long rows, long long cols) {
     return m >= 128 && gram_splits(m, n, 1) > 1 ? kSplitTiles * 4LL * 128 * 128 : 0;
 }
 
-template <int KIND, int T, int NST, bool PAIR, typename OT>
-int launch_tile(const NsArgs& a, int in, int count, int mode, int splits, hipStream_t stream) {
+template <int T, int NST, bool PAIR, bool SYM, bool SRC, bool LAST, typename OT>
+int launch_tile(const NsArgs& a, Product g, int mode, int splits, hipStream_t stream) {
     constexpr int LDS = std::max(NST * 2 * T * 128, T == 256 ? 2 * T * T : 4 * T * T);
-    static hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_ns_gemm<KIND, T, NST, PAIR, OT>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    static hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_ns_gemm<T, NST, PAIR, SYM, SRC, LAST, OT>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
     if (attr != hipSuccess) return (int)attr;
-    const int ti = (a.mp + T - 1) / T, tj = ((KIND <= NS_POLY ? a.mp : a.np) + T - 1) / T;
-    const long long total = (KIND <= NS_POLY ? (long long)ti * (ti + 1) / 2 : (long long)ti * tj) * count;
-    hipLaunchKernelGGL((k_ns_gemm<KIND, T, NST, PAIR, OT>), dim3((unsigned)((total + 7) / 8 * 8), 1, mode == 1 ? splits : 1), dim3(threads_of(T)), LDS, stream, a, in, ti, tj, count,
-                       mode, splits);
+    g.tiles_i = (g.a_rows + T - 1) / T;
+    g.tiles_j = (g.b_rows + T - 1) / T;
+    g.mode = mode;
+    g.splits = splits;
+    const long long total = (SYM ? (long long)g.tiles_i * (g.tiles_i + 1) / 2 : (long long)g.tiles_i * g.tiles_j) * g.count;
+    hipLaunchKernelGGL((k_ns_gemm<T, NST, PAIR, SYM, SRC, LAST, OT>), dim3((unsigned)((total + 7) / 8 * 8), 1, mode == 1 ? splits : 1), dim3(threads_of(T)), LDS, stream, a, g);
     DM_LAUNCH_CHECK();
     return DM_OK;
 }
@@ -500,47 +512,86 @@ int launch_tile(const NsArgs& a, int in, int count, int mode, int splits, hipStr
 // Tile by the time a launch takes, in rounds of the chip at one 256 tile per CU (measured on 1280^2, paired): a 256 tile needs a third of a
 // 128 tile's LDS and request traffic per product; 128 tiles run two per CU and a round of 512 costs 1.15, half a round 0.6; 64 tiles 0.3
 // per 512, 0.25 where a CU gets one (then with a ring as deep as LDS allows: its loads have nothing else to hide behind).
-template <int KIND, bool PAIR, typename OT>
-int launch_gemm(const NsArgs& a, int in, int count, hipStream_t stream) {
+template <bool PAIR, bool SYM, bool SRC, bool LAST, typename OT>
+int launch_gemm(const NsArgs& a, const Product& g, hipStream_t stream) {
     auto tiles = [&](int T) {
-        const long long t = (a.mp + T - 1) / T, u = ((KIND <= NS_POLY ? a.mp : a.np) + T - 1) / T;
-        return (KIND <= NS_POLY ? t * (t + 1) / 2 : t * u) * count;
+        const long long t = (g.a_rows + T - 1) / T, u = (g.b_rows + T - 1) / T;
+        return (SYM ? t * (t + 1) / 2 : t * u) * g.count;
     };
-    if (KIND == NS_GRAM && a.part && a.mp >= 128) {
-        const int splits = gram_splits(a.mp, a.np, count);
+    if (SYM && !SRC && a.part && g.a_rows >= 128) {
+        const int splits = gram_splits(g.a_rows, g.kw, g.count);
         if (splits > 1) {
-            if (int rc = launch_tile<KIND, 128, 2, PAIR, OT>(a, in, count, 1, splits, stream)) return rc;
-            return launch_tile<KIND, 128, 2, PAIR, OT>(a, in, count, 2, splits, stream);
+            if (int rc = launch_tile<128, 2, PAIR, SYM, SRC, LAST, OT>(a, g, 1, splits, stream)) return rc;
+            return launch_tile<128, 2, PAIR, SYM, SRC, LAST, OT>(a, g, 2, splits, stream);
         }
     }
-    const double c256 = a.mp >= 256 ? (double)((tiles(256) + 255) / 256) : 1e30;
-    const double c128 = a.mp >= 128 ? std::max(0.6, 1.15 * (double)tiles(128) / 512) : 1e30;
+    const double c256 = g.a_rows >= 256 ? (double)((tiles(256) + 255) / 256) : 1e30;
+    const double c128 = g.a_rows >= 128 ? std::max(0.6, 1.15 * (double)tiles(128) / 512) : 1e30;
     const double c64 = tiles(64) <= 256 ? 0.25 : 0.3 * (double)((tiles(64) + 511) / 512);
-    if (c256 <= c128 && c256 <= c64) return launch_tile<KIND, 256, 2, PAIR, OT>(a, in, count, 0, 1, stream);
-    if (c128 <= c64) return launch_tile<KIND, 128, 2, PAIR, OT>(a, in, count, 0, 1, stream);
-    if (tiles(64) <= 256) return launch_tile<KIND, 64, 8, PAIR, OT>(a, in, count, 0, 1, stream);
-    return launch_tile<KIND, 64, 4, PAIR, OT>(a, in, count, 0, 1, stream);
+    if (c256 <= c128 && c256 <= c64) return launch_tile<256, 2, PAIR, SYM, SRC, LAST, OT>(a, g, 0, 1, stream);
+    if (c128 <= c64) return launch_tile<128, 2, PAIR, SYM, SRC, LAST, OT>(a, g, 0, 1, stream);
+    if (tiles(64) <= 256) return launch_tile<64, 8, PAIR, SYM, SRC, LAST, OT>(a, g, 0, 1, stream);
+    return launch_tile<64, 4, PAIR, SYM, SRC, LAST, OT>(a, g, 0, 1, stream);
 }
+
+// the products of the iteration
+struct Iteration {
+    const NsArgs& a;
+    int count;
+    hipStream_t stream;
+    Product make(const _Float16* A, int a_rows, const _Float16* B, int b_rows, int kw, const _Float16* src, float src_c, float acc_c, _Float16* D, _Float16* E) const {
+        Product g{};
+        g.A = A; g.B = B; g.src = src; g.D = D; g.E = E;
+        g.a_rows = a_rows; g.b_rows = b_rows; g.kw = kw; g.src_c = src_c; g.acc_c = acc_c; g.count = count;
+        return g;
+    }
+    // S = X X^T
+    template <bool PAIR> int gram() const {
+        Product g = make(a.x, a.mp, a.x, a.mp, a.np, nullptr, 0.f, kInv, a.s, nullptr);
+        g.rests = PAIR;
+        return launch_gemm<PAIR, true, false, false, float>(a, g, stream);
+    }
+    // P = b S + c S S
+    template <bool PAIR> int poly() const {
+        Product g = make(a.s, a.mp, a.s, a.mp, a.mp, a.s, kB, kC * kInv, a.pm, nullptr);
+        g.src_rests = g.rests = PAIR;
+        return launch_gemm<PAIR, true, true, false, float>(a, g, stream);
+    }
+    // X <- a X + P X, in both orientations; rests: the next iteration takes pairs
+    template <bool PAIR> int step(int in, bool rests) const {
+        Product g = make(a.pm, a.mp, a.xt[in], a.np, a.mp, a.x, kA, kInv, a.x, a.xt[in ^ 1]);
+        g.src_rests = PAIR;
+        g.rests = rests;
+        return launch_gemm<PAIR, false, true, false, float>(a, g, stream);
+    }
+    // the result a X + P X
+    template <bool PAIR, typename T> int last(int in) const {
+        Product g = make(a.pm, a.mp, a.xt[in], a.np, a.mp, a.x, kA * kInv, kInv * kInv, nullptr, nullptr);
+        g.src_rests = PAIR;
+        return launch_gemm<PAIR, false, true, true, T>(a, g, stream);
+    }
+};
+
+#define NS_TRY(call) if (int rc_ = (call)) return rc_
 
 template <typename T>
 int run_group(NsArgs& a, int count, int steps, hipStream_t stream) {
     hipLaunchKernelGGL((k_ns_norm<T>), dim3(a.parts, count), dim3(256), 0, stream, a);
     hipLaunchKernelGGL((k_ns_pack<T>), dim3(a.np / 64, a.mp / 64, count), dim3(256), 0, stream, a);
     DM_LAUNCH_CHECK();
+    const Iteration it{a, count, stream};
     constexpr bool SHORT = std::is_same<T, __bf16>::value;       // bf16: the last two iterations without the rests, see the head of the file
     const int plain_from = SHORT ? std::max(1, steps - 2) : steps;
     for (int k = 0; k < steps; ++k) {
-        int rc;
         if (k < plain_from) {
-            if ((rc = launch_gemm<NS_GRAM, true, float>(a, k & 1, count, stream)) || (rc = launch_gemm<NS_POLY, true, float>(a, k & 1, count, stream))) return rc;
-            rc = k + 1 < steps ? launch_gemm<NS_STEP, true, float>(a, k & 1, count, stream) : launch_gemm<NS_LAST, true, T>(a, k & 1, count, stream);
+            NS_TRY(it.gram<true>());
+            NS_TRY(it.poly<true>());
+            NS_TRY(k + 1 < steps ? it.step<true>(k & 1, k + 1 < plain_from) : (it.last<true, T>(k & 1)));
         } else if constexpr (SHORT) {
-            if ((rc = launch_gemm<NS_GRAM, false, float>(a, k & 1, count, stream)) || (rc = launch_gemm<NS_POLY, false, float>(a, k & 1, count, stream))) return rc;
-            rc = k + 1 < steps ? launch_gemm<NS_STEP, false, float>(a, k & 1, count, stream) : launch_gemm<NS_LAST, false, T>(a, k & 1, count, stream);
-        } else {
-            rc = DM_OK;
+            NS_TRY(it.gram<false>());
+            NS_TRY(it.poly<false>());
+            NS_TRY(k + 1 < steps ? it.step<false>(k & 1, false) : (it.last<false, T>(k & 1)));
         }
-        if (rc) return rc;
     }
     return DM_OK;
 }

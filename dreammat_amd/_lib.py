@@ -167,7 +167,8 @@ _SIGS = {
                                    + [c_int] * 4 + [c_void_p]),
     "dm_orthogonalize_workspace_bytes": (c_size_t, [c_int] * 3),
     "dm_orthogonalize": (c_int, [c_void_p, c_void_p] + [c_int] * 5 + [c_float, c_void_p, c_size_t, c_void_p]),
-    "dm_muon_step": (c_int, [c_void_p] * 3 + [c_int] * 5 + [c_float, c_int, c_float, c_float, c_float, c_void_p, c_size_t, c_void_p]),
+    "dm_muon_step_workspace_bytes": (c_size_t, [c_void_p, c_void_p, c_int]),
+    "dm_muon_step": (c_int, [c_void_p] * 6 + [c_int] * 3 + [c_float, c_int, c_float, c_float, c_void_p, c_size_t, c_void_p]),
     "dm_adam_step": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, _LL, c_int, c_float, c_float, c_float, c_float,
                              c_float, c_int, c_void_p]),
 }

@@ -25,6 +25,11 @@
 #include "dm_common.h"
 #include "dm_elem.h"
 
+#include <algorithm>
+#include <new>
+#include <type_traits>
+#include <vector>
+
 namespace {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -36,29 +41,32 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int kGroup = 16;                                   // matrices of one launch
 constexpr int kNormParts = 512;                              // most partial sums of a squared norm
 
-// One group of same-shaped matrices [rows, cols] (row-major, contiguous)
-struct Mats {
-    const void* g[kGroup];
-    float* mom[kGroup];      // momentum, or NULL
-    float* p[kGroup];        // parameter, or NULL
-    void* out[kGroup];       // orthogonalised matrix, or NULL
+// One matrix [rows, cols] (row-major, contiguous).  The iteration takes it as m x n, m <= n (transposed if rows > cols); mp, np: padded to
+// multiples of 64.
+struct Mat {
+    const void* g;
+    float* mom;              // momentum, or NULL
+    float* p;                // parameter, or NULL
+    void* out;               // orthogonalised matrix, or NULL
+    _Float16* x;             // pairs: X [mp][np], X^T [np][mp] twice (ping-pong), S [mp][mp], P [mp][mp]
+    int rows, cols;
+    float step;
+    short parts;             // workgroups of the norm pass
+    short whole;             // rows and pointers of the norm pass are whole 16-byte chunks
+    __host__ __device__ int m() const { return rows < cols ? rows : cols; }
+    __host__ __device__ int n() const { return rows < cols ? cols : rows; }
+    __host__ __device__ int mp() const { return (m() + 63) & ~63; }
+    __host__ __device__ int np() const { return (n() + 63) & ~63; }
+    __device__ bool flip() const { return rows > cols; }
+    __device__ _Float16* xt(int k) const { return x + (long long)(1 + k) * mp() * 2 * np(); }
+    __device__ _Float16* s() const { return xt(2); }
+    __device__ _Float16* pm() const { return xt(2) + (long long)mp() * 2 * mp(); }
 };
 
 struct NsArgs {
-    Mats t;
-    int rows, cols;          // as given
-    int m, n;                // m <= n: the iteration's orientation
-    int mp, np;              // padded to multiples of 64
-    int flip;                // rows > cols
-    int whole;               // rows and pointers of the norm pass are whole 16-byte chunks
-    int parts;               // workgroups per matrix of the norm pass
+    Mat t[kGroup];           // same-shaped ones side by side
     double* norm;            // [count][kNormParts]
-    float* part;             // partial sums of a split contraction
-    _Float16* x;             // pairs [count][mp][np]
-    _Float16* xt[2];         // pairs [count][np][mp], ping-pong
-    _Float16* s;             // pairs [count][mp][mp]
-    _Float16* pm;            // pairs [count][mp][mp]
-    float mu, eps, decay, step;
+    float mu, eps, decay;
     int nesterov;
 };
 
@@ -72,26 +80,28 @@ __device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
 
 // the update direction of element i
 template <typename T>
-__device__ __forceinline__ float direction(const NsArgs& a, int b, long long i) {
-    const float g = (float)reinterpret_cast<const T*>(a.t.g[b])[i];
-    if (!a.t.mom[b]) return g;
-    const float m = a.t.mom[b][i];
+__device__ __forceinline__ float direction(const NsArgs& a, const Mat& t, long long i) {
+    const float g = (float)reinterpret_cast<const T*>(t.g)[i];
+    if (!t.mom) return g;
+    const float m = t.mom[i];
     return a.nesterov ? g + a.mu * m : m;
 }
 
-// momentum update and the squared norm of the direction: a.parts workgroups per matrix, four elements per thread, sums in 64 bits
+// momentum update and the squared norm of the direction: parts workgroups per matrix, four elements per thread, sums in 64 bits
 template <typename T>
 __global__ __launch_bounds__(256) void k_ns_norm(NsArgs a) {
     __shared__ double red[4];
     const int b = blockIdx.y;
-    const long long total = (long long)a.rows * a.cols;
-    const T* g = reinterpret_cast<const T*>(a.t.g[b]);
-    float* mom = a.t.mom[b];
+    const Mat& t = a.t[b];
+    if ((int)blockIdx.x >= t.parts) return;
+    const long long total = (long long)t.rows * t.cols;
+    const T* g = reinterpret_cast<const T*>(t.g);
+    float* mom = t.mom;
     double s = 0.0;
     auto add = [&](float u) { s += (double)u * (double)u; };
-    if (a.whole) {
+    if (t.whole) {
         typedef T vec __attribute__((ext_vector_type(4)));
-        for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < total; i += 1024LL * a.parts) {
+        for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < total; i += 1024LL * t.parts) {
             const vec gv = *reinterpret_cast<const vec*>(g + i);
             if (mom) {
                 float4 m = *reinterpret_cast<const float4*>(mom + i);
@@ -107,9 +117,9 @@ __global__ __launch_bounds__(256) void k_ns_norm(NsArgs a) {
             }
         }
     } else {
-        for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += 256LL * a.parts) {
+        for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += 256LL * t.parts) {
             if (mom) mom[i] = a.mu * mom[i] + (float)g[i];
-            add(direction<T>(a, b, i));
+            add(direction<T>(a, t, i));
         }
     }
 #pragma unroll
@@ -126,14 +136,18 @@ __global__ __launch_bounds__(256) void k_ns_pack(NsArgs a) {
     __shared__ double red[4];
     const int b = blockIdx.z, i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;       // rows / columns of X
     const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+    const Mat& t = a.t[b];
+    const int m = t.m(), n = t.n(), mp = t.mp(), np = t.np();
+    const bool flip = t.flip();
+    if (i0 >= mp || j0 >= np) return;
     float v[16];
 #pragma unroll
     for (int q = 0; q < 16; ++q) {                                              // read along the rows as given
-        const int r = ty + 4 * q, i = a.flip ? i0 + tx : i0 + r, j = a.flip ? j0 + r : j0 + tx;
-        v[q] = i < a.m && j < a.n ? direction<T>(a, b, a.flip ? (long long)j * a.cols + i : (long long)i * a.cols + j) : 0.f;
+        const int r = ty + 4 * q, i = flip ? i0 + tx : i0 + r, j = flip ? j0 + r : j0 + tx;
+        v[q] = i < m && j < n ? direction<T>(a, t, flip ? (long long)j * t.cols + i : (long long)i * t.cols + j) : 0.f;
     }
     double s = 0.0;
-    for (int k = threadIdx.x; k < a.parts; k += 256) s += a.norm[(long long)b * kNormParts + k];
+    for (int k = threadIdx.x; k < t.parts; k += 256) s += a.norm[(long long)b * kNormParts + k];
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     if (tx == 0) red[ty] = s;
@@ -142,12 +156,11 @@ __global__ __launch_bounds__(256) void k_ns_pack(NsArgs a) {
 #pragma unroll
     for (int q = 0; q < 16; ++q) {
         const int r = ty + 4 * q;
-        if (a.flip) tile[tx][r] = v[q] * inv;
+        if (flip) tile[tx][r] = v[q] * inv;
         else tile[r][tx] = v[q] * inv;
     }
     __syncthreads();
-    _Float16* x = a.x + (long long)b * a.mp * 2 * a.np;
-    _Float16* xt = a.xt[0] + (long long)b * a.np * 2 * a.mp;
+    _Float16 *x = t.x, *xt = t.xt(0);
 #pragma unroll
     for (int q = 0; q < 2; ++q) {                                               // eight entries of a row per thread: 16-byte stores
         const int r = (threadIdx.x >> 3) + 32 * q, c = (threadIdx.x & 7) * 8;
@@ -159,7 +172,7 @@ __global__ __launch_bounds__(256) void k_ns_pack(NsArgs a) {
             h[k] = p;
             l[k] = w;
         }
-        const long long at = pair_at(i0 + r, j0 + c, a.np);
+        const long long at = pair_at(i0 + r, j0 + c, np);
         *reinterpret_cast<half8*>(x + at) = h;
         *reinterpret_cast<half8*>(x + at + 32) = l;
 #pragma unroll
@@ -169,7 +182,7 @@ __global__ __launch_bounds__(256) void k_ns_pack(NsArgs a) {
             h[k] = p;
             l[k] = w;
         }
-        const long long to = pair_at(j0 + r, i0 + c, a.mp);
+        const long long to = pair_at(j0 + r, i0 + c, mp);
         *reinterpret_cast<half8*>(xt + to) = h;
         *reinterpret_cast<half8*>(xt + to + 32) = l;
     }
@@ -182,75 +195,83 @@ __device__ __forceinline__ int tile_at(int row, int blk, int chunk) {
     return (row * (T / 32) + (blk ^ ((row >> 3) & 1))) * 128 + ((chunk ^ (row & 7)) << 4);
 }
 
-// One launch: D = src_c * src + acc_c * (A B^T) for `count` matrices
-struct Product {
-    const _Float16 *A, *B;           // [a_rows][kw], [b_rows][kw] pairs
-    const _Float16* src;             // [a_rows][b_rows] pairs (SRC)
-    _Float16* D;                     // the result as pairs [a_rows][b_rows]; symmetric: both halves of it
-    _Float16* E;                     // not symmetric: the result transposed [b_rows][a_rows]
-    int a_rows, b_rows, kw;          // padded
-    float src_c, acc_c;
-    int src_rests, rests;            // whether the source has rests, whether the result needs them (its readers take pairs)
-    int tiles_i, tiles_j, count;
-    int mode, splits;
+// The products of the iteration, all C = A B^T over pair matrices:
+//   GRAM  A = B = X,         S = C
+//   POLY  A = B = S,         P = b S + c C
+//   STEP  A = P, B = X^T,    X <- a X + C  in both orientations (X in place: a tile is read and written by its own workgroup only)
+//   LAST  the same, into the parameter or the output
+enum { NS_GRAM = 0, NS_POLY = 1, NS_STEP = 2, NS_LAST = 3 };
+
+// One launch over a group: same-shaped matrices are a class; a class's units are tiles, each split into `splits` shares of K
+struct Class {
+    int first;               // its first workgroup, a multiple of 8
+    int mat, count;          // matrices mat .. mat + count
+    int tiles_i, tiles_j, per_mat;
+    int splits, part;        // shares per tile (1: none); its first share among all shares
+};
+struct Launch {
+    Class c[kGroup];
+    float* part;             // fp32 partial sums [share][T * T]
+    int classes, in, rests;  // which X^T is read; whether the result's readers take its rests
 };
 
-// Tile T x T, two rows of WJ waves of T/2 x T/WJ.  K goes in blocks of 128 bytes per row through a ring of NST LDS stages filled by
-// buffer_load ... lds (chunks XOR-swizzled by (row >> 1) & 7), NST - 1 of them in flight: 32 pairs (PAIR: three products per block) or the
-// values of 64.
-//   SYM   A B^T is symmetric: tiles i >= j, stored twice
-//   SRC   the result adds src_c src (SYM: another matrix; else the matrix that D replaces, read and written by its own workgroup only)
-//   LAST  the result goes into the parameter or the output instead of pairs
-// The epilogue goes through LDS: the source tile arrives as whole lines, every lane replaces its own entries, and whole lines leave in both
-// orientations (the transposed one by ds_read_b64_tr_b16); a 256 tile does that half by half.
-// mode 0: the whole product.  1: this workgroup's share (blockIdx.z) of a split contraction, fp32 sums to a.part.  2: joins those shares.
-template <int T, int NST, bool PAIR, bool SYM, bool SRC, bool LAST, typename OT>
-__global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Product g) {
-    [[maybe_unused]] constexpr int NT = threads_of(T), NW = NT / 64, WJ = NW / 2, ROWB = 128, STAGE = 2 * T * ROWB, TI = T / 2, TJ = T / WJ, FI = TI / 32, FJ = TJ / 32,
-                                   PIECES = T / 8 / NW, H = T == 256 ? 2 : 1, TR = T / H;       // TR rows per epilogue pass
-    extern __shared__ __attribute__((aligned(16))) char smem[];      // max(NST * STAGE, 4 TR T)
-#if defined(__HIP_DEVICE_COMPILE__)
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, hi = lane >> 5, l31 = lane & 31;
-    const int wi = wave / WJ, wj = wave % WJ;
-    const int mode = g.mode, splits = g.splits;
-    // XCD-contiguous tile order (block b runs on XCD b % 8), matrix by matrix
-    const int per_mat = SYM ? g.tiles_i * (g.tiles_i + 1) / 2 : g.tiles_i * g.tiles_j;
-    const int total = per_mat * g.count, per = (total + 7) / 8;
-    const int id = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
-    if ((int)(blockIdx.x >> 3) >= per || id >= total) return;
-    const int b = id / per_mat, rem = id - b * per_mat;
-    int ti, tj;
+// block -> class, unit.  Block b runs on XCD b % 8: every XCD gets an eighth of each class's units, neighbours of a matrix together; the odd
+// units go to other XCDs class by class.  False: nothing to do.
+__device__ __forceinline__ bool locate(const Launch& l, int bid, int& c, int& id) {
+    c = 0;
+    while (c + 1 < l.classes && bid >= l.c[c + 1].first) ++c;
+    const int units = l.c[c].per_mat * l.c[c].count * l.c[c].splits, local = bid - l.c[c].first, x = ((local & 7) + 3 * c) & 7;
+    id = (int)((long long)units * x / 8) + (local >> 3);
+    return id < (int)((long long)units * (x + 1) / 8);
+}
+
+// tile of a matrix: SYM: on or below the diagonal
+template <bool SYM>
+__device__ __forceinline__ void tile_of(const Class& c, int rem, int& ti, int& tj) {
     if constexpr (SYM) {
         ti = (int)((sqrtf(8.f * (float)rem + 1.f) - 1.f) * 0.5f);
         while ((ti + 1) * (ti + 2) / 2 <= rem) ++ti;
         while (ti * (ti + 1) / 2 > rem) --ti;
         tj = rem - ti * (ti + 1) / 2;
     } else {
-        ti = rem % g.tiles_i;                   // the row tiles of one panel of B side by side
-        tj = rem / g.tiles_i;
+        ti = rem % c.tiles_i;                   // the row tiles of one panel of B side by side
+        tj = rem / c.tiles_i;
     }
+}
+
+// Tile T x T, two rows of WJ waves of T/2 x T/WJ.  K goes in blocks of 128 bytes per row through a ring of NST LDS stages filled by
+// buffer_load ... lds (chunks XOR-swizzled by (row >> 1) & 7), NST - 1 of them in flight: 32 pairs (PAIR: three products per block) or the
+// values of 64.
+// GRAM and POLY are symmetric: tiles i >= j, stored twice.
+// The epilogue goes through LDS: the tile of S or X arrives as whole lines, every lane replaces its own entries, and whole lines leave in both
+// orientations (the transposed one by ds_read_b64_tr_b16); a 256 tile does that half by half.  A share of a split contraction leaves its fp32
+// sums in l.part instead, for k_ns_join.
+template <int KIND, int T, int NST, bool PAIR, typename OT>
+__global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
+    [[maybe_unused]] constexpr int NT = threads_of(T), NW = NT / 64, WJ = NW / 2, ROWB = 128, STAGE = 2 * T * ROWB, TI = T / 2, TJ = T / WJ, FI = TI / 32, FJ = TJ / 32,
+                                   PIECES = T / 8 / NW, H = T == 256 ? 2 : 1, TR = T / H;       // TR rows per epilogue pass
+    [[maybe_unused]] constexpr bool SYM = KIND <= NS_POLY, SRC = KIND != NS_GRAM, LAST = KIND == NS_LAST;
+    // the result in units of 2^13 (LAST: 1) from products in units of 2^26
+    [[maybe_unused]] constexpr float ACC = LAST ? kInv * kInv : KIND == NS_POLY ? kC * kInv : kInv, OLD = LAST ? kA * kInv : KIND == NS_POLY ? kB : kA;
+    extern __shared__ __attribute__((aligned(16))) char smem[];      // max(NST * STAGE, 4 TR T)
+#if defined(__HIP_DEVICE_COMPILE__)
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, hi = lane >> 5, l31 = lane & 31;
+    const int wi = wave / WJ, wj = wave % WJ;
+    int cls, id;
+    if (!locate(l, blockIdx.x, cls, id)) return;
+    const Class& c = l.c[cls];
+    const int tiles = c.per_mat * c.count, z = id / tiles, tile = id - z * tiles, rel = tile / c.per_mat, splits = c.splits;
+    int ti, tj;
+    tile_of<SYM>(c, tile - rel * c.per_mat, ti, tj);
+    const Mat& t = a.t[c.mat + rel];
+    const int mp = t.mp(), np = t.np();
     const int i0 = ti * T, j0 = tj * T;
+    const int kw = KIND == NS_GRAM ? np : mp, ow = SYM ? mp : np, oh = mp;      // contraction; the result's columns and rows
     f32x16 acc[FI][FJ];
-    if (mode == 2) {
-#pragma unroll
-        for (int i = 0; i < FI; ++i)
-#pragma unroll
-            for (int j = 0; j < FJ; ++j)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const float4* p = reinterpret_cast<const float4*>(a.part) + ((long long)id * splits * FI * FJ * 4 + (i * FJ + j) * 4 + q) * NT + tid;
-                    float4 v = p[0];
-                    for (int z = 1; z < splits; ++z) {
-                        const float4 o = p[(long long)z * FI * FJ * 4 * NT];
-                        v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
-                    }
-                    acc[i][j][4 * q] = v.x; acc[i][j][4 * q + 1] = v.y; acc[i][j][4 * q + 2] = v.z; acc[i][j][4 * q + 3] = v.w;
-                }
-    } else {
-        const int kw = g.kw;
-        const _Float16* A = g.A + (long long)b * g.a_rows * 2 * kw;
-        const _Float16* B = g.B + (long long)b * g.b_rows * 2 * kw;
-        const int arows = min(T, g.a_rows - i0), brows = min(T, g.b_rows - j0);
+    {
+        const _Float16* A = KIND == NS_GRAM ? t.x : KIND == NS_POLY ? t.s() : t.pm();
+        const _Float16* B = SYM ? A : t.xt(l.in);
+        const int arows = min(T, oh - i0), brows = min(T, ow - j0);
         const __amdgpu_buffer_rsrc_t ars = __builtin_amdgcn_make_buffer_rsrc((void*)(A + (long long)i0 * 2 * kw), 0, arows * kw * 4, 0x00020000);
         const __amdgpu_buffer_rsrc_t brs = __builtin_amdgcn_make_buffer_rsrc((void*)(B + (long long)j0 * 2 * kw), 0, brows * kw * 4, 0x00020000);
         unsigned off[PIECES];                                      // rows past the matrix lie past the descriptor: zeros
@@ -279,7 +300,7 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Product g) 
             return *reinterpret_cast<const half8*>(base + row * ROWB + ((chunk ^ ((row >> 1) & 7)) << 4));
         };
         const int all = kw / (PAIR ? 32 : 64);
-        const int s_lo = mode == 1 ? (int)((long long)all * blockIdx.z / splits) : 0, s_hi = mode == 1 ? (int)((long long)all * (blockIdx.z + 1) / splits) : all;
+        const int s_lo = (int)((long long)all * z / splits), s_hi = (int)((long long)all * (z + 1) / splits);
 #pragma unroll
         for (int q = 0; q < NST - 1; ++q)
             if (s_lo + q < s_hi) issue(s_lo + q, q);
@@ -323,14 +344,15 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Product g) 
             }
             st = st + 1 == NST ? 0 : st + 1;
         }
-        if (mode == 1) {
+        if (KIND == NS_GRAM && splits > 1) {
+            float4* part = reinterpret_cast<float4*>(l.part) + (long long)(c.part + tile * splits + z) * (T * T / 4);
 #pragma unroll
             for (int i = 0; i < FI; ++i)
 #pragma unroll
                 for (int j = 0; j < FJ; ++j)
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
-                        reinterpret_cast<float4*>(a.part)[(((long long)id * splits + blockIdx.z) * FI * FJ * 4 + (i * FJ + j) * 4 + q) * NT + tid] =
+                        part[((wave * FI + i) * FJ + j) * 256 + 64 * q + lane] =
                             make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
             return;
         }
@@ -338,20 +360,19 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Product g) 
 
     // ---- epilogue.  lane: row i = l31 of the fragment, registers 4 g + r: columns 8 g + 4 hi + r
     typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-    const int ow = g.b_rows, oh = g.a_rows;
     for (int h = 0; h < H; ++h) {
         const int r0 = i0 + h * TR;                                    // first row of this pass
         if (h && r0 >= oh) break;
         __syncthreads();                                               // every wave has read its last fragments (its share of the last pass)
         if constexpr (SRC) {
             constexpr int P = TR * T / 256 / NW;                       // 1 KB = 8 blocks per wave and request
-            const _Float16* src = g.src + (long long)b * oh * 2 * ow;
+            const _Float16* src = KIND == NS_POLY ? t.s() : t.x;
             const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(src + (long long)r0 * 2 * ow), 0, min(TR, oh - r0) * ow * 4, 0x00020000);
 #pragma unroll
             for (int p = 0; p < P; ++p) {
                 const int q = (wave * P + p) * 8 + (lane >> 3), row = q / (T / 32), blk = (q % (T / 32)) ^ ((row >> 3) & 1);
                 const int chunk = (lane & 7) ^ (row & 7);
-                const unsigned o = chunk < 4 || g.src_rests ? (unsigned)row * (unsigned)ow * 4u + (unsigned)((j0 / 32 + blk) * 128 + (chunk << 4)) : 0x80000000u;
+                const unsigned o = PAIR || chunk < 4 ? (unsigned)row * (unsigned)ow * 4u + (unsigned)((j0 / 32 + blk) * 128 + (chunk << 4)) : 0x80000000u;
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(smem + (wave * P + p) * 1024), 16, (int)o, 0, 0, 0);
             }
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -369,11 +390,11 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Product g) 
                         half4* rp = reinterpret_cast<half4*>(smem + tile_at<T>(row, blk, 4 + q) + 8 * hi);
                         float v[4];
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) v[r] = acc[fi][fj][4 * q + r] * g.acc_c;
+                        for (int r = 0; r < 4; ++r) v[r] = acc[fi][fj][4 * q + r] * ACC;
                         if constexpr (SRC) {
                             const half4 hv = *vp, lv = *rp;
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) v[r] += g.src_c * ((float)hv[r] + (float)lv[r]);
+                            for (int r = 0; r < 4; ++r) v[r] += OLD * ((float)hv[r] + (float)lv[r]);
                         }
                         if constexpr (LAST) {                          // fp32 in the pair's place: columns 0, 1 | 2, 3 of the four
                             *reinterpret_cast<float2*>(vp) = make_float2(v[0], v[1]);
@@ -394,12 +415,13 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Product g) 
         }
         __syncthreads();
         if constexpr (LAST) {
-            float* p = a.t.p[b];
-            OT* out = reinterpret_cast<OT*>(a.t.out[b]);
+            const bool flip = t.flip();
+            float* p = t.p;
+            OT* out = reinterpret_cast<OT*>(t.out);
             // four entries per thread along the fast axis of the matrix as given, a batch of loads in flight
             constexpr int Q = TR * T / 4 / NT, U = T == 256 ? 4 : Q < 8 ? Q : 8;
             static_assert(Q % U == 0, "whole batches");
-            const bool four = (a.flip ? a.m : a.n) % 4 == 0 && !((uintptr_t)(p ? (void*)p : (void*)out) & 15);
+            const bool four = (flip ? t.m() : t.n()) % 4 == 0 && !((uintptr_t)(p ? (void*)p : (void*)out) & 15);
             for (int k0 = 0; k0 < Q; k0 += U) {
                 float4 old[U];
                 long long to[U];
@@ -407,10 +429,10 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Product g) 
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     const int k = tid + (k0 + u) * NT;
-                    const int row = a.flip ? k % (TR / 4) * 4 : k / (T / 4), col = a.flip ? k / (TR / 4) : k % (T / 4) * 4, i = r0 + row, j = j0 + col;
-                    const int fast = a.flip ? a.m - i : a.n - j, slow = a.flip ? a.n - j : a.m - i;
+                    const int row = flip ? k % (TR / 4) * 4 : k / (T / 4), col = flip ? k / (TR / 4) : k % (T / 4) * 4, i = r0 + row, j = j0 + col;
+                    const int fast = flip ? t.m() - i : t.n() - j, slow = flip ? t.n() - j : t.m() - i;
                     ok[u] = slow > 0 ? max(0, min(4, fast)) : 0;
-                    to[u] = a.flip ? (long long)j * a.cols + i : (long long)i * a.cols + j;
+                    to[u] = flip ? (long long)j * t.cols + i : (long long)i * t.cols + j;
                     if (p && ok[u]) {
                         if (four) old[u] = *reinterpret_cast<const float4*>(p + to[u]);
                         else {
@@ -425,16 +447,16 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Product g) 
                 for (int u = 0; u < U; ++u) {
                     if (!ok[u]) continue;
                     const int k = tid + (k0 + u) * NT;
-                    const int row = a.flip ? k % (TR / 4) * 4 : k / (T / 4), col = a.flip ? k / (TR / 4) : k % (T / 4) * 4;
+                    const int row = flip ? k % (TR / 4) * 4 : k / (T / 4), col = flip ? k / (TR / 4) : k % (T / 4) * 4;
                     float o[4];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const int rr = a.flip ? row + r : row, cc = a.flip ? col : col + r;
+                        const int rr = flip ? row + r : row, cc = flip ? col : col + r;
                         o[r] = *reinterpret_cast<const float*>(smem + tile_at<T>(rr, cc >> 5, ((cc & 31) >> 3) + ((cc & 2) << 1)) + ((cc & 4) << 1) + ((cc & 1) << 2));
                     }
                     if (p) {
-                        const float w[4] = {old[u].x * a.decay - a.step * o[0], old[u].y * a.decay - a.step * o[1], old[u].z * a.decay - a.step * o[2],
-                                            old[u].w * a.decay - a.step * o[3]};
+                        const float w[4] = {old[u].x * a.decay - t.step * o[0], old[u].y * a.decay - t.step * o[1], old[u].z * a.decay - t.step * o[2],
+                                            old[u].w * a.decay - t.step * o[3]};
                         if (four) *reinterpret_cast<float4*>(p + to[u]) = make_float4(w[0], w[1], w[2], w[3]);
                         else
                             for (int r = 0; r < ok[u]; ++r) p[to[u] + r] = w[r];
@@ -447,19 +469,20 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Product g) 
                 }
             }
         } else {
-            _Float16* D = g.D + (long long)b * oh * 2 * ow;
+            _Float16* D = KIND == NS_GRAM ? t.s() : KIND == NS_POLY ? t.pm() : t.x;
+            const bool rests = KIND == NS_STEP ? l.rests : PAIR;
 #pragma unroll 4
             for (int q = tid; q < TR * T / 4; q += NT) {               // 16-byte chunks, whole rows of blocks
                 const int chunk = q & 7, blk = (q >> 3) % (T / 32), row = (q >> 3) / (T / 32);
-                if (r0 + row < oh && j0 + 32 * blk < ow && (chunk < 4 || g.rests))
+                if (r0 + row < oh && j0 + 32 * blk < ow && (chunk < 4 || rests))
                     *reinterpret_cast<u32x4*>(D + (long long)(r0 + row) * 2 * ow + (j0 / 32 + blk) * 64 + chunk * 8) =
                         *reinterpret_cast<const u32x4*>(smem + tile_at<T>(row, blk, chunk));
             }
             if (!SYM || ti != tj) {                                    // the other orientation: rows j, blocks of 32 i
-                _Float16* E = SYM ? D : g.E + (long long)b * ow * 2 * oh;
+                _Float16* E = SYM ? D : t.xt(l.in ^ 1);
                 const int l15 = lane & 15, grp = lane >> 4;
-                for (int u = wave; u < (T / 16) * (TR / 32) * (1 + g.rests); u += NW) {
-                    const int part = g.rests ? u & 1 : 0, v = u >> g.rests, ib = v % (TR / 32), c0 = v / (TR / 32) * 16;
+                for (int u = wave; u < (T / 16) * (TR / 32) * (1 + rests); u += NW) {
+                    const int part = rests ? u & 1 : 0, v = u >> (int)rests, ib = v % (TR / 32), c0 = v / (TR / 32) * 16;
                     const int row = 32 * ib + 8 * grp + (l15 >> 2), cc = (c0 & 31) + 4 * (l15 & 3);
                     const char* p0 = smem + tile_at<T>(row, c0 >> 5, (cc >> 3) + 4 * part) + ((cc & 4) << 1);
                     const char* p1 = smem + tile_at<T>(row + 4, c0 >> 5, (cc >> 3) + 4 * part) + ((cc & 4) << 1);
@@ -474,195 +497,330 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Product g) 
 #endif
 }
 
-long long pad64(long long v) { return (v + 63) / 64 * 64; }
-
-// Split of the Gram contraction: a wide X (n much larger than m) has few tiles with a long K each.  Shares of at least 16 steps, at most
-// two workgroups per CU in all.  1: no split.
-constexpr int kSplitTiles = 512;
-int gram_splits(int mp, int np, int count) {
-    const int t = (mp + 127) / 128, tiles = t * (t + 1) / 2 * count;
-    return std::max(1, std::min(kSplitTiles / tiles, np / 32 / 16));
+// S from the shares of a split Gram contraction, in both orientations: a wave per 32 x 32 block of a tile, summed in the shares' order
+template <int T>
+__global__ __launch_bounds__(256) void k_ns_join(NsArgs a, Launch l) {
+    __shared__ float sums[4][32][33];
+    constexpr int FI = T / 64, FJ = T == 256 ? 2 : T / 64, WJ = threads_of(T) / 128, BLOCKS = (T / 32) * (T / 32) / 4;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, hi = lane >> 5, l31 = lane & 31;
+    int cls = 0;
+    while (cls + 1 < l.classes && (int)blockIdx.x >= l.c[cls + 1].first) ++cls;
+    const Class& c = l.c[cls];
+    const int local = blockIdx.x - c.first, tile = local / BLOCKS, f = (local - tile * BLOCKS) * 4 + wave;      // f = (wave of the product, i, j)
+    const int rel = tile / c.per_mat;
+    int ti, tj;
+    tile_of<true>(c, tile - rel * c.per_mat, ti, tj);
+    const Mat& t = a.t[c.mat + rel];
+    const int mp = t.mp(), w = f / (FI * FJ), i = f / FJ % FI, j = f % FJ;
+    const int i0 = ti * T + T / 2 * (w / WJ) + 32 * i, j0 = tj * T + T / WJ * (w % WJ) + 32 * j;
+    const float4* part = reinterpret_cast<const float4*>(l.part) + (long long)(c.part + tile * c.splits) * (T * T / 4) + f * 256 + lane;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        float4 v = part[64 * q];
+        for (int z = 1; z < c.splits; ++z) {
+            const float4 o = part[(long long)z * (T * T / 4) + 64 * q];
+            v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+        }
+        float* d = &sums[wave][l31][8 * q + 4 * hi];
+        d[0] = v.x * kInv; d[1] = v.y * kInv; d[2] = v.z * kInv; d[3] = v.w * kInv;
+    }
+    __syncthreads();
+    if (i0 >= mp || j0 >= mp) return;                                  // (mp is a multiple of 64)
+    const int r = lane >> 1, c0 = (lane & 1) * 16;
+    auto store = [&](int row0, int col0, bool turned) {
+        _Float16* to = t.s() + pair_at(row0 + r, col0 + c0, mp);
+#pragma unroll
+        for (int o = 0; o < 16; o += 8) {
+            half8 h, e;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                _Float16 x, y;
+                split(turned ? sums[wave][c0 + o + k][r] : sums[wave][r][c0 + o + k], x, y);
+                h[k] = x;
+                e[k] = y;
+            }
+            *reinterpret_cast<half8*>(to + o) = h;
+            *reinterpret_cast<half8*>(to + 32 + o) = e;
+        }
+    };
+    store(i0, j0, false);
+    if (ti != tj) store(j0, i0, true);
 }
 
-// bytes of one matrix's workspace (x, two x^T, s, p); of the split's partial sums
-long long mat_bytes(long long rows, long long cols) {
-    const long long m = pad64(std::min(rows, cols)), n = pad64(std::max(rows, cols));
-    return 4 * (3 * m * n + 2 * m * m) + 8 * kNormParts;
-}
-long long part_bytes(long long rows, long long cols) {
-    const int m = (int)pad64(std::min(rows, cols)), n = (int)pad64(std::max(rows, cols));
-    return m >= 128 && gram_splits(m, n, 1) > 1 ? kSplitTiles * 4LL * 128 * 128 : 0;
+// A launch of one kind over a group, and what it should take, in K steps of 32 pairs on one CU with a 256 tile (2.8 us).
+// Measured on 1280^2, paired: a 256 tile needs a third of a 128 tile's LDS and request traffic per product; 128 tiles run two per CU and a
+// round of 512 costs 1.15, half a round 0.6; 64 tiles 0.3 per 512, 0.25 where a CU gets one (then with a ring as deep as LDS allows: its
+// loads have nothing else to hide behind).  Rounds: of equal units, whole ones; of unequal ones (longest first) the longest, or a tenth more
+// than their mean over the CUs.
+struct Plan {
+    Launch l;
+    int tile, blocks, units, shares;
+    double cost;
+};
+
+constexpr int kShareBytes = 128 << 20;          // most memory of partial sums
+
+// length > 0: the contraction is split into shares of at most so many steps (and no fewer than 16)
+Plan plan_tile(const Mat* t, int count, int kind, int T, int length) {
+    Plan p{};
+    p.tile = T;
+    struct Item { Class c; int steps; } items[kGroup];
+    int n = 0, longest = 0, shortest = 1 << 30, top = 0;
+    double work = 0;
+    for (int at = 0, end; at < count; at = end) {
+        for (end = at + 1; end < count && t[end].mp() == t[at].mp() && t[end].np() == t[at].np();) ++end;
+        Item& q = items[n++];
+        const int mp = t[at].mp(), np = t[at].np(), all = (kind == NS_GRAM ? np : mp) / 32;
+        q.c = {};
+        q.c.mat = at;
+        q.c.count = end - at;
+        q.c.tiles_i = (mp + T - 1) / T;
+        q.c.tiles_j = ((kind <= NS_POLY ? mp : np) + T - 1) / T;
+        q.c.per_mat = kind <= NS_POLY ? q.c.tiles_i * (q.c.tiles_i + 1) / 2 : q.c.tiles_i * q.c.tiles_j;
+        q.c.splits = length > 0 ? std::max(1, std::min((all + length - 1) / length, all / 16)) : 1;
+        q.steps = (all + q.c.splits - 1) / q.c.splits;
+        const int units = q.c.per_mat * q.c.count * q.c.splits;
+        if (q.c.splits > 1) {
+            q.c.part = p.shares;
+            p.shares += units;
+        }
+        p.units += units;
+        work += (double)units * q.steps;
+        longest = std::max(longest, q.steps);
+        shortest = std::min(shortest, q.steps);
+        top = std::max(top, mp);
+    }
+    std::stable_sort(items, items + n, [](const Item& x, const Item& y) { return x.steps > y.steps; });
+    for (int i = 0; i < n; ++i) {
+        p.l.c[i] = items[i].c;
+        p.l.c[i].first = p.blocks;
+        p.blocks += (items[i].c.per_mat * items[i].c.count * items[i].c.splits + 7) / 8 * 8;
+    }
+    p.l.classes = n;
+    auto rounds = [&](int slots) {
+        return longest == shortest ? (double)longest * ((p.units + slots - 1) / slots) : std::max((double)longest, 1.1 * work / slots);
+    };
+    if (T == 256) p.cost = rounds(256);
+    else if (T == 128) p.cost = std::max(0.6 * longest, 1.15 * work / 512);
+    else p.cost = p.units <= 256 ? 0.25 * longest : 0.3 * rounds(512);
+    if (p.shares) p.cost += 2 + 0.05 * p.shares * (T * T) / 65536;       // the join: a launch, 256 KB written and read per share of a 256 tile
+    if (top < T || (long long)p.shares * T * T * 4 > kShareBytes) p.cost = 1e30;
+    return p;
 }
 
-template <int T, int NST, bool PAIR, bool SYM, bool SRC, bool LAST, typename OT>
-int launch_tile(const NsArgs& a, Product g, int mode, int splits, hipStream_t stream) {
+Plan plan(const Mat* t, int count, int kind) {
+    Plan best = plan_tile(t, count, kind, 64, 0);
+    int most = 0;
+    for (int i = 0; i < count; ++i) most = std::max(most, t[i].np() / 32);
+    for (int T = 128; T <= 256; T *= 2)
+        for (int d = 0; d <= (kind == NS_GRAM ? 16 : 0); ++d) {          // shares of a d-th of the longest contraction
+            if (d && most / d < 16) break;
+            const Plan p = plan_tile(t, count, kind, T, d ? (most + d - 1) / d : 0);
+            if (p.cost < best.cost) best = p;
+        }
+    return best;
+}
+
+template <int KIND, int T, int NST, bool PAIR, typename OT>
+int launch_tile(const NsArgs& a, const Plan& p, int in, bool rests, float* part, hipStream_t stream) {
     constexpr int LDS = std::max(NST * 2 * T * 128, T == 256 ? 2 * T * T : 4 * T * T);
-    static hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_ns_gemm<T, NST, PAIR, SYM, SRC, LAST, OT>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    static hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_ns_gemm<KIND, T, NST, PAIR, OT>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
     if (attr != hipSuccess) return (int)attr;
-    g.tiles_i = (g.a_rows + T - 1) / T;
-    g.tiles_j = (g.b_rows + T - 1) / T;
-    g.mode = mode;
-    g.splits = splits;
-    const long long total = (SYM ? (long long)g.tiles_i * (g.tiles_i + 1) / 2 : (long long)g.tiles_i * g.tiles_j) * g.count;
-    hipLaunchKernelGGL((k_ns_gemm<T, NST, PAIR, SYM, SRC, LAST, OT>), dim3((unsigned)((total + 7) / 8 * 8), 1, mode == 1 ? splits : 1), dim3(threads_of(T)), LDS, stream, a, g);
+    Launch l = p.l;
+    l.in = in;
+    l.rests = rests;
+    l.part = part;
+    hipLaunchKernelGGL((k_ns_gemm<KIND, T, NST, PAIR, OT>), dim3(p.blocks), dim3(threads_of(T)), LDS, stream, a, l);
     DM_LAUNCH_CHECK();
+    if constexpr (KIND == NS_GRAM && T >= 128) {
+        if (!p.shares) return DM_OK;
+        int n = 0, blocks = 0;
+        for (int c = 0; c < p.l.classes; ++c) {
+            if (p.l.c[c].splits < 2) continue;
+            l.c[n] = p.l.c[c];
+            l.c[n++].first = blocks;
+            blocks += p.l.c[c].per_mat * p.l.c[c].count * ((T / 32) * (T / 32) / 4);
+        }
+        l.classes = n;
+        hipLaunchKernelGGL((k_ns_join<T>), dim3(blocks), dim3(256), 0, stream, a, l);
+        DM_LAUNCH_CHECK();
+    }
     return DM_OK;
 }
 
-// Tile by the time a launch takes, in rounds of the chip at one 256 tile per CU (measured on 1280^2, paired): a 256 tile needs a third of a
-// 128 tile's LDS and request traffic per product; 128 tiles run two per CU and a round of 512 costs 1.15, half a round 0.6; 64 tiles 0.3
-// per 512, 0.25 where a CU gets one (then with a ring as deep as LDS allows: its loads have nothing else to hide behind).
-template <bool PAIR, bool SYM, bool SRC, bool LAST, typename OT>
-int launch_gemm(const NsArgs& a, const Product& g, hipStream_t stream) {
-    auto tiles = [&](int T) {
-        const long long t = (g.a_rows + T - 1) / T, u = (g.b_rows + T - 1) / T;
-        return (SYM ? t * (t + 1) / 2 : t * u) * g.count;
-    };
-    if (SYM && !SRC && a.part && g.a_rows >= 128) {
-        const int splits = gram_splits(g.a_rows, g.kw, g.count);
-        if (splits > 1) {
-            if (int rc = launch_tile<128, 2, PAIR, SYM, SRC, LAST, OT>(a, g, 1, splits, stream)) return rc;
-            return launch_tile<128, 2, PAIR, SYM, SRC, LAST, OT>(a, g, 2, splits, stream);
-        }
-    }
-    const double c256 = g.a_rows >= 256 ? (double)((tiles(256) + 255) / 256) : 1e30;
-    const double c128 = g.a_rows >= 128 ? std::max(0.6, 1.15 * (double)tiles(128) / 512) : 1e30;
-    const double c64 = tiles(64) <= 256 ? 0.25 : 0.3 * (double)((tiles(64) + 511) / 512);
-    if (c256 <= c128 && c256 <= c64) return launch_tile<256, 2, PAIR, SYM, SRC, LAST, OT>(a, g, 0, 1, stream);
-    if (c128 <= c64) return launch_tile<128, 2, PAIR, SYM, SRC, LAST, OT>(a, g, 0, 1, stream);
-    if (tiles(64) <= 256) return launch_tile<64, 8, PAIR, SYM, SRC, LAST, OT>(a, g, 0, 1, stream);
-    return launch_tile<64, 4, PAIR, SYM, SRC, LAST, OT>(a, g, 0, 1, stream);
+template <int KIND, bool PAIR, typename OT>
+int launch_gemm(const NsArgs& a, const Plan& p, int in, bool rests, float* part, hipStream_t stream) {
+    if (p.tile == 256) return launch_tile<KIND, 256, 2, PAIR, OT>(a, p, in, rests, part, stream);
+    if (p.tile == 128) return launch_tile<KIND, 128, 2, PAIR, OT>(a, p, in, rests, part, stream);
+    if (p.units <= 256) return launch_tile<KIND, 64, 8, PAIR, OT>(a, p, in, rests, part, stream);
+    return launch_tile<KIND, 64, 4, PAIR, OT>(a, p, in, rests, part, stream);
 }
 
-// the products of the iteration
-struct Iteration {
-    const NsArgs& a;
-    int count;
-    hipStream_t stream;
-    Product make(const _Float16* A, int a_rows, const _Float16* B, int b_rows, int kw, const _Float16* src, float src_c, float acc_c, _Float16* D, _Float16* E) const {
-        Product g{};
-        g.A = A; g.B = B; g.src = src; g.D = D; g.E = E;
-        g.a_rows = a_rows; g.b_rows = b_rows; g.kw = kw; g.src_c = src_c; g.acc_c = acc_c; g.count = count;
-        return g;
-    }
-    // S = X X^T
-    template <bool PAIR> int gram() const {
-        Product g = make(a.x, a.mp, a.x, a.mp, a.np, nullptr, 0.f, kInv, a.s, nullptr);
-        g.rests = PAIR;
-        return launch_gemm<PAIR, true, false, false, float>(a, g, stream);
-    }
-    // P = b S + c S S
-    template <bool PAIR> int poly() const {
-        Product g = make(a.s, a.mp, a.s, a.mp, a.mp, a.s, kB, kC * kInv, a.pm, nullptr);
-        g.src_rests = g.rests = PAIR;
-        return launch_gemm<PAIR, true, true, false, float>(a, g, stream);
-    }
-    // X <- a X + P X, in both orientations; rests: the next iteration takes pairs
-    template <bool PAIR> int step(int in, bool rests) const {
-        Product g = make(a.pm, a.mp, a.xt[in], a.np, a.mp, a.x, kA, kInv, a.x, a.xt[in ^ 1]);
-        g.src_rests = PAIR;
-        g.rests = rests;
-        return launch_gemm<PAIR, false, true, false, float>(a, g, stream);
-    }
-    // the result a X + P X
-    template <bool PAIR, typename T> int last(int in) const {
-        Product g = make(a.pm, a.mp, a.xt[in], a.np, a.mp, a.x, kA * kInv, kInv * kInv, nullptr, nullptr);
-        g.src_rests = PAIR;
-        return launch_gemm<PAIR, false, true, true, T>(a, g, stream);
-    }
-};
-
-#define NS_TRY(call) if (int rc_ = (call)) return rc_
+#define NS_TRY(call) do { if (int rc_ = (call)) return rc_; } while (0)
 
 template <typename T>
-int run_group(NsArgs& a, int count, int steps, hipStream_t stream) {
-    hipLaunchKernelGGL((k_ns_norm<T>), dim3(a.parts, count), dim3(256), 0, stream, a);
-    hipLaunchKernelGGL((k_ns_pack<T>), dim3(a.np / 64, a.mp / 64, count), dim3(256), 0, stream, a);
+int run_group(const NsArgs& a, int count, int steps, float* part, hipStream_t stream) {
+    int parts = 1, mp = 0, np = 0;
+    for (int i = 0; i < count; ++i) {
+        parts = std::max<int>(parts, a.t[i].parts);
+        mp = std::max(mp, a.t[i].mp());
+        np = std::max(np, a.t[i].np());
+    }
+    hipLaunchKernelGGL((k_ns_norm<T>), dim3(parts, count), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((k_ns_pack<T>), dim3(np / 64, mp / 64, count), dim3(256), 0, stream, a);
     DM_LAUNCH_CHECK();
-    const Iteration it{a, count, stream};
+    const Plan gram = plan(a.t, count, NS_GRAM), poly = plan(a.t, count, NS_POLY), step = plan(a.t, count, NS_STEP);
     constexpr bool SHORT = std::is_same<T, __bf16>::value;       // bf16: the last two iterations without the rests, see the head of the file
     const int plain_from = SHORT ? std::max(1, steps - 2) : steps;
     for (int k = 0; k < steps; ++k) {
         if (k < plain_from) {
-            NS_TRY(it.gram<true>());
-            NS_TRY(it.poly<true>());
-            NS_TRY(k + 1 < steps ? it.step<true>(k & 1, k + 1 < plain_from) : (it.last<true, T>(k & 1)));
+            NS_TRY((launch_gemm<NS_GRAM, true, float>(a, gram, 0, true, part, stream)));
+            NS_TRY((launch_gemm<NS_POLY, true, float>(a, poly, 0, true, part, stream)));
+            if (k + 1 < steps) NS_TRY((launch_gemm<NS_STEP, true, float>(a, step, k & 1, k + 1 < plain_from, part, stream)));
+            else NS_TRY((launch_gemm<NS_LAST, true, T>(a, step, k & 1, false, part, stream)));
         } else if constexpr (SHORT) {
-            NS_TRY(it.gram<false>());
-            NS_TRY(it.poly<false>());
-            NS_TRY(k + 1 < steps ? it.step<false>(k & 1, false) : (it.last<false, T>(k & 1)));
+            NS_TRY((launch_gemm<NS_GRAM, false, float>(a, gram, 0, false, part, stream)));
+            NS_TRY((launch_gemm<NS_POLY, false, float>(a, poly, 0, false, part, stream)));
+            if (k + 1 < steps) NS_TRY((launch_gemm<NS_STEP, false, float>(a, step, k & 1, false, part, stream)));
+            else NS_TRY((launch_gemm<NS_LAST, false, T>(a, step, k & 1, false, part, stream)));
         }
     }
     return DM_OK;
 }
 
+// workspace of one matrix (x, two x^T, s, p, norm) and of a group
+long long mat_bytes(const Mat& t) { return 4LL * t.mp() * (3LL * t.np() + 2LL * t.mp()) + 8 * kNormParts; }
+long long group_bytes(const Mat* t, int count) {
+    const Plan gram = plan(t, count, NS_GRAM);
+    long long b = 4LL * gram.shares * gram.tile * gram.tile;
+    for (int i = 0; i < count; ++i) b += mat_bytes(t[i]);
+    return b;
+}
+// the most that groups of `fit` need
+long long need_bytes(const std::vector<Mat>& t, int fit) {
+    long long b = 0;
+    for (size_t at = 0; at < t.size(); at += fit) b = std::max(b, group_bytes(t.data() + at, (int)std::min<size_t>(fit, t.size() - at)));
+    return b;
+}
+
+bool sizes_ok(int rows, int cols) { return (long long)rows * cols <= (1LL << 31) && std::min(rows, cols) <= 32768 && std::max(rows, cols) <= (1 << 20); }
+
+// largest first, equal shapes side by side
+void order(std::vector<Mat>& t) {
+    std::stable_sort(t.begin(), t.end(), [](const Mat& x, const Mat& y) {
+        const long long a = (long long)x.mp() * x.np(), b = (long long)y.mp() * y.np();
+        return a != b ? a > b : x.mp() > y.mp();
+    });
+}
+
 // dtype of the gradients / outputs: 0 bf16, 1 half, 2 fp32
-int run(const void* const* g, float* const* mom, float* const* p, void* const* out, int count, int rows, int cols, int dtype, int steps, float mu,
-        int nesterov, float eps, float decay, float step, void* ws, size_t ws_bytes, hipStream_t stream) {
-    if (count < 0 || rows <= 0 || cols <= 0 || steps < 1 || steps > 64 || dtype < 0 || dtype > 2 || !ws) return DM_ERR_ARG;
-    if ((long long)rows * cols > (1LL << 31) || std::min(rows, cols) > 32768 || std::max(rows, cols) > (1 << 20)) return DM_ERR_UNSUPPORTED;
-    if ((uintptr_t)ws & 255) return DM_ERR_ARG;
-    const long long one = mat_bytes(rows, cols), extra = part_bytes(rows, cols);
-    const int fit = (int)std::min<long long>(kGroup, std::max<long long>(0, (long long)ws_bytes - extra) / one);
-    if (count && fit < 1) return DM_ERR_WORKSPACE;
-    NsArgs a{};
-    a.rows = rows; a.cols = cols; a.flip = rows > cols;
-    a.m = std::min(rows, cols); a.n = std::max(rows, cols);
-    a.mp = (int)pad64(a.m); a.np = (int)pad64(a.n);
-    a.mu = mu; a.nesterov = nesterov; a.eps = eps; a.decay = decay; a.step = step;
-    a.parts = (int)std::max<long long>(1, std::min<long long>(kNormParts, (long long)rows * cols / (256 * 8)));
+int run(std::vector<Mat>& t, NsArgs& a, int dtype, int steps, void* ws, size_t ws_bytes, hipStream_t stream) {
+    if (steps < 1 || steps > 64 || dtype < 0 || dtype > 2 || !ws || ((uintptr_t)ws & 255)) return DM_ERR_ARG;
+    for (Mat& m : t) {
+        if (!m.g || (m.p ? !m.mom : !m.out) || m.rows <= 0 || m.cols <= 0) return DM_ERR_ARG;
+        if (!sizes_ok(m.rows, m.cols)) return DM_ERR_UNSUPPORTED;
+        m.parts = (short)std::max<long long>(1, std::min<long long>(kNormParts, (long long)m.rows * m.cols / (256 * 8)));
+        m.whole = m.cols % 4 == 0 && !(((uintptr_t)m.g | (uintptr_t)m.mom) & 15);      // rows of 16-byte (8-byte) chunks in every operand of the norm pass
+    }
+    order(t);
+    int fit = kGroup;
+    while (fit && need_bytes(t, fit) > (long long)ws_bytes) --fit;
+    if (!fit) return DM_ERR_WORKSPACE;
     DM_ENTER();
-    for (int at = 0; at < count; at += fit) {
-        const int c = std::min(fit, count - at);
-        bool whole = cols % 4 == 0;                                // rows of 16-byte (8-byte) chunks in every operand of the norm pass
-        for (int i = 0; i < c; ++i) {
-            a.t.g[i] = g[at + i];
-            a.t.mom[i] = mom ? mom[at + i] : nullptr;
-            a.t.p[i] = p ? p[at + i] : nullptr;
-            a.t.out[i] = out ? out[at + i] : nullptr;
-            if (!a.t.g[i] || (mom && !a.t.mom[i]) || (p ? !a.t.p[i] : !a.t.out[i])) return DM_ERR_ARG;
-            whole = whole && !(((uintptr_t)a.t.g[i] | (uintptr_t)a.t.mom[i]) & 15);
-        }
-        a.whole = whole;
+    for (size_t at = 0; at < t.size(); at += fit) {
+        const int c = (int)std::min<size_t>(fit, t.size() - at);
         char* w = (char*)ws;
-        a.part = extra ? (float*)w : nullptr;
-        w += extra;
-        auto take = [&](long long bytes) { char* q = w; w += bytes * c; return q; };
-        a.norm = (double*)take(8 * kNormParts);
-        a.x = (_Float16*)take(4LL * a.mp * a.np);
-        a.xt[0] = (_Float16*)take(4LL * a.mp * a.np);
-        a.xt[1] = (_Float16*)take(4LL * a.mp * a.np);
-        a.s = (_Float16*)take(4LL * a.mp * a.mp);
-        a.pm = (_Float16*)take(4LL * a.mp * a.mp);
-        const int rc = dtype == 0 ? run_group<__bf16>(a, c, steps, stream) : dtype == 1 ? run_group<_Float16>(a, c, steps, stream) : run_group<float>(a, c, steps, stream);
+        a.norm = (double*)w;
+        w += 8LL * kNormParts * c;
+        for (int i = 0; i < c; ++i) {
+            a.t[i] = t[at + i];
+            a.t[i].x = (_Float16*)w;
+            w += mat_bytes(a.t[i]) - 8 * kNormParts;
+        }
+        float* part = (float*)w;
+        const int rc = dtype == 0 ? run_group<__bf16>(a, c, steps, part, stream) : dtype == 1 ? run_group<_Float16>(a, c, steps, part, stream) : run_group<float>(a, c, steps, part, stream);
         if (rc) return rc;
     }
     return DM_OK;
+}
+
+// host memory for the matrices' list: an allocation that fails is an error code, not an exception
+template <typename F>
+int with_mats(int count, F f) {
+    try {
+        std::vector<Mat> t((size_t)count);
+        return f(t);
+    } catch (const std::bad_alloc&) {
+        return DM_ERR_WORKSPACE;
+    }
 }
 
 }  // namespace
 
 extern "C" {
 
-// workspace bytes that take `count` [rows, cols] matrices in one launch (at most 16 at once; less memory means more launches)
+// workspace bytes that take `count` [rows, cols] matrices in groups of 16 (less memory, down to one matrix's: smaller groups); 0: sizes out of range
 size_t dm_orthogonalize_workspace_bytes(int count, int rows, int cols) {
-    if (count <= 0 || rows <= 0 || cols <= 0) return 0;
-    return (size_t)(std::min(count, kGroup) * mat_bytes(rows, cols) + part_bytes(rows, cols));
+    if (count <= 0 || rows <= 0 || cols <= 0 || !sizes_ok(rows, cols)) return 0;
+    Mat t[kGroup] = {};
+    for (Mat& m : t) { m.rows = rows; m.cols = cols; }
+    return (size_t)std::max(group_bytes(t, std::min(count, kGroup)), count > kGroup && count % kGroup ? group_bytes(t, count % kGroup) : 0);
 }
 
-// out[i] = five-step Newton-Schulz of g[i]: `count` same-shaped matrices [rows, cols] behind HOST arrays of device pointers; dtype 0 bf16 |
+// the same for matrices of their own sizes
+size_t dm_muon_step_workspace_bytes(const int* rows_host, const int* cols_host, int count) {
+    if (count <= 0 || !rows_host || !cols_host) return 0;
+    size_t bytes = 0;
+    with_mats(count, [&](std::vector<Mat>& t) {
+        for (int i = 0; i < count; ++i) {
+            t[i].rows = rows_host[i];
+            t[i].cols = cols_host[i];
+            if (rows_host[i] <= 0 || cols_host[i] <= 0 || !sizes_ok(rows_host[i], cols_host[i])) return DM_ERR_ARG;
+        }
+        order(t);
+        bytes = (size_t)need_bytes(t, kGroup);
+        return DM_OK;
+    });
+    return bytes;
+}
+
+// out[i] = Newton-Schulz of g[i]: `count` same-shaped matrices [rows, cols] behind HOST arrays of device pointers; dtype 0 bf16 |
 // 1 half | 2 fp32 of both; ws 256-byte aligned
 int dm_orthogonalize(const void* const* g_host, void* const* out_host, int count, int rows, int cols, int dtype, int steps, float eps, void* ws,
                      size_t ws_bytes, hipStream_t stream) {
-    if (count && (!g_host || !out_host)) return DM_ERR_ARG;
-    return run(g_host, nullptr, nullptr, out_host, count, rows, cols, dtype, steps, 0.f, 0, eps, 1.f, 0.f, ws, ws_bytes, stream);
+    if (count < 0 || rows <= 0 || cols <= 0 || (count && (!g_host || !out_host))) return DM_ERR_ARG;
+    return with_mats(count, [&](std::vector<Mat>& t) {
+        for (int i = 0; i < count; ++i) {
+            t[i].g = g_host[i];
+            t[i].out = out_host[i];
+            t[i].rows = rows;
+            t[i].cols = cols;
+        }
+        NsArgs a{};
+        a.eps = eps;
+        return run(t, a, dtype, steps, ws, ws_bytes, stream);
+    });
 }
 
-// momentum step on fp32 masters: mom <- mu mom + g;  u = g + mu mom or mom;  p <- p decay - step orth(u).  g of `dtype`, mom / p fp32
-int dm_muon_step(const void* const* g_host, float* const* mom_host, float* const* p_host, int count, int rows, int cols, int dtype, int steps, float mu,
-                 int nesterov, float eps, float decay, float step, void* ws, size_t ws_bytes, hipStream_t stream) {
-    if (count && (!g_host || !mom_host || !p_host)) return DM_ERR_ARG;
-    return run(g_host, mom_host, p_host, nullptr, count, rows, cols, dtype, steps, mu, nesterov, eps, decay, step, ws, ws_bytes, stream);
+// momentum step on fp32 masters of their own sizes: mom <- mu mom + g;  u = g + mu mom or mom;  p <- p decay - step[i] orth(u).  g of `dtype`,
+// mom / p fp32; all arrays on the HOST
+int dm_muon_step(const void* const* g_host, float* const* mom_host, float* const* p_host, const int* rows_host, const int* cols_host,
+                 const float* step_host, int count, int dtype, int steps, float mu, int nesterov, float eps, float decay, void* ws, size_t ws_bytes,
+                 hipStream_t stream) {
+    if (count < 0 || (count && (!g_host || !mom_host || !p_host || !rows_host || !cols_host || !step_host))) return DM_ERR_ARG;
+    return with_mats(count, [&](std::vector<Mat>& t) {
+        for (int i = 0; i < count; ++i) {
+            t[i].g = g_host[i];
+            t[i].mom = mom_host[i];
+            t[i].p = p_host[i];
+            t[i].rows = rows_host[i];
+            t[i].cols = cols_host[i];
+            t[i].step = step_host[i];
+        }
+        NsArgs a{};
+        a.mu = mu; a.nesterov = nesterov; a.eps = eps; a.decay = decay;
+        return run(t, a, dtype, steps, ws, ws_bytes, stream);
+    });
 }
 
 }  // extern "C"

@@ -1997,7 +1997,6 @@ def gated_add_norm(x, h, gate=None, post=None, pre=None, scale=1.0, eps=1e-5, ki
 # ------------------------------------------------------------------------------------------ fine-tuning: orthogonalised updates
 _NS_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_NS_SIDE = 32768                     # of the shorter side; the longer one up to 2^20
-NS_GROUP = 16                           # matrices of one launch (csrc/newton_schulz.hip)
 
 
 def _ns_shape(rows, cols, what):
@@ -2009,8 +2008,15 @@ def _ptr_array(ts):
     return (ctypes.c_void_p * len(ts))(*[t.data_ptr() for t in ts])
 
 
-def _ns_workspace(count, rows, cols, device):
-    return torch.empty(int(_lib.lib().dm_orthogonalize_workspace_bytes(count, rows, cols)), device=device, dtype=torch.uint8)
+def _overlap(written, read):
+    """whether a tensor of `written` shares memory with another one of it or with one of `read` (all contiguous)"""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), w) for ts, w in ((written, True), (read, False)) for t in ts)
+    end = {True: 0, False: 0}           # how far the written / the read ones so far reach
+    for lo, hi, w in spans:
+        if lo < end[True] or (w and lo < end[False]):
+            return True
+        end[w] = max(end[w], hi)
+    return False
 
 
 def orthogonalize(g, steps=5, eps=1e-7):
@@ -2030,7 +2036,7 @@ def orthogonalize(g, steps=5, eps=1e-7):
     out = torch.empty_like(g)
     gs, outs = g.view(-1, rows, cols), out.view(-1, rows, cols)
     with _guard(g.device):
-        ws = _ns_workspace(gs.shape[0], rows, cols, g.device)
+        ws = torch.empty(int(_lib.lib().dm_orthogonalize_workspace_bytes(gs.shape[0], rows, cols)), device=g.device, dtype=torch.uint8)
         check(_lib.lib().dm_orthogonalize(_ptr_array(list(gs)), _ptr_array(list(outs)), gs.shape[0], rows, cols, _NS_DTYPES[g.dtype], int(steps), float(eps),
                                           ws.data_ptr(), ws.numel(), _stream_of(g.device)), "dm_orthogonalize")
     return out
@@ -2043,7 +2049,7 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
         m <- momentum m + g;  u = g + momentum m (nesterov) or m;  p <- p (1 - lr weight_decay) - lr s orthogonalize(u)
 
     s = 0.2 sqrt(max(rows, cols)) for scale = "rms" (updates as large as Adam's, so its learning rate and decay carry over),
-    sqrt(max(1, rows / cols)) for "spectral", or the given number.  Matrices of one shape share their launches."""
+    sqrt(max(1, rows / cols)) for "spectral", or the given number.  The matrices share their launches in groups of 16, largest first."""
     params, grads, momenta = list(params), list(grads), list(momenta)
     if not len(params) == len(grads) == len(momenta):
         raise ValueError("muon_step: one gradient and one momentum buffer per parameter")
@@ -2065,20 +2071,24 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
             continue
         rows, cols = p.shape[0], p.numel() // p.shape[0]
         _ns_shape(rows, cols, "muon_step")
-        groups.setdefault((rows, cols, g.dtype, p.device), []).append((p, g, m))
-    live = [t for v in groups.values() for q in v for t in (q[0], q[2])]
-    if len({t.data_ptr() for t in live}) != len(live):
-        raise ValueError("muon_step: a parameter or momentum buffer occurs twice")
-    for (rows, cols, dtype, device), v in groups.items():
-        for p, g, m in v:
-            _on_one_gpu(p, g, m)
-    for (rows, cols, dtype, device), v in groups.items():
-        s = 0.2 * max(rows, cols) ** 0.5 if scale == "rms" else max(1.0, rows / cols) ** 0.5 if scale == "spectral" else float(scale)
-        gs = [g.detach().contiguous() for _, g, _ in v]
+        if g.device == p.device == m.device:
+            g = g.detach().contiguous()
+        groups.setdefault((g.dtype, p.device), []).append((p, g, m, rows, cols))
+    live = [t for v in groups.values() for p, _, m, _, _ in v for t in (p, m)]
+    if _overlap(live, [q[1] for v in groups.values() for q in v]):
+        raise ValueError("muon_step: parameters and momentum buffers share memory with each other or with a gradient")
+    for v in groups.values():
+        for q in v:
+            _on_one_gpu(*q[:3])
+    for (dtype, device), v in groups.items():
+        n = len(v)
+        rows, cols = ((ctypes.c_int * n)(*[q[i] for q in v]) for i in (3, 4))
+        size = (lambda r, c: 0.2 * max(r, c) ** 0.5) if scale == "rms" else (lambda r, c: max(1.0, r / c) ** 0.5) if scale == "spectral" else (lambda r, c: float(scale))
+        lengths = (ctypes.c_float * n)(*[lr * size(q[3], q[4]) for q in v])
         with _guard(device):
-            ws = _ns_workspace(len(v), rows, cols, device)
-            check(_lib.lib().dm_muon_step(_ptr_array(gs), _ptr_array([m for _, _, m in v]), _ptr_array([p for p, _, _ in v]), len(v), rows, cols,
-                                          _NS_DTYPES[dtype], int(steps), float(momentum), int(bool(nesterov)), float(eps), float(1.0 - lr * weight_decay),
-                                          float(lr * s), ws.data_ptr(), ws.numel(), _stream_of(device)), "dm_muon_step")
+            ws = torch.empty(int(_lib.lib().dm_muon_step_workspace_bytes(rows, cols, n)), device=device, dtype=torch.uint8)
+            check(_lib.lib().dm_muon_step(*[_ptr_array([q[i] for q in v]) for i in (1, 2, 0)], rows, cols, lengths, n, _NS_DTYPES[dtype], int(steps),
+                                          float(momentum), int(bool(nesterov)), float(eps), float(1.0 - lr * weight_decay), ws.data_ptr(), ws.numel(),
+                                          _stream_of(device)), "dm_muon_step")
     if live:
         torch.autograd.graph.increment_version(live)      # caches keyed on a parameter's version see the update

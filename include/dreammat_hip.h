@@ -572,14 +572,17 @@ int dm_linear_adapted_bwd_f16(const void* x, const void* dy, const void* w_t, co
                               const int32_t* offsets, long long n, float scale, const void* u, void* ws, size_t ws_bytes, void* dx, void* da, void* db,
                               long long M, int K, int N, int R, int E, dm_stream_t stream);
 
-/* Orthogonalised updates by Newton-Schulz products (csrc/newton_schulz.hip).  `count` matrices [rows, cols], contiguous, behind HOST arrays
- * of device pointers; dtype of g and out: 0 bf16 | 1 half | 2 fp32.  dm_muon_step (mom, p fp32): mom <- mu mom + g; u = g + mu mom (nesterov)
- * or mom; p <- p decay - step orth(u).  ws: 256-byte aligned, dm_orthogonalize_workspace_bytes (less, down to one matrix's: more launches). */
+/* Orthogonalised updates by Newton-Schulz products (csrc/newton_schulz.hip): `count` contiguous matrices [rows, cols], the device pointers (and
+ * for dm_muon_step every matrix's sizes and step) in HOST arrays; dtype of g and out: 0 bf16 | 1 half | 2 fp32.  dm_muon_step (mom, p fp32):
+ * mom <- mu mom + g; u = g + mu mom (nesterov) or mom; p <- p decay - step[i] orth(u).  ws: 256-byte aligned, ..._workspace_bytes (less, down to
+ * the largest matrix's alone: smaller groups, more launches). */
 size_t dm_orthogonalize_workspace_bytes(int count, int rows, int cols);
+size_t dm_muon_step_workspace_bytes(const int* rows_host, const int* cols_host, int count);
 int dm_orthogonalize(const void* const* g_host, void* const* out_host, int count, int rows, int cols, int dtype, int steps, float eps, void* ws,
                      size_t ws_bytes, dm_stream_t stream);
-int dm_muon_step(const void* const* g_host, float* const* mom_host, float* const* p_host, int count, int rows, int cols, int dtype, int steps,
-                 float mu, int nesterov, float eps, float decay, float step, void* ws, size_t ws_bytes, dm_stream_t stream);
+int dm_muon_step(const void* const* g_host, float* const* mom_host, float* const* p_host, const int* rows_host, const int* cols_host,
+                 const float* step_host, int count, int dtype, int steps, float mu, int nesterov, float eps, float decay, void* ws, size_t ws_bytes,
+                 dm_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -113,6 +113,18 @@ def test_muon_step_refuses():
     hipops.muon_step([], [], [], lr=0.1)                                              # nothing to do
 
 
+def test_muon_step_refuses_shared_memory():
+    both, g = torch.zeros(80), torch.zeros(4, 6)
+    view = lambda lo, *shape: both[lo:lo + 24].view(*(shape or (4, 6)))
+    for params, grads, momenta in [([view(0)], [view(0)], [view(40)]), ([view(0)], [view(40)], [view(40)]), ([view(0)], [view(20)], [view(50)]),
+                                   ([view(0), view(23, 2, 12)], [g, g.view(2, 12)], [view(50), torch.zeros(2, 12)]), ([view(30)], [g], [view(53)])]:
+        with pytest.raises(ValueError, match="share memory"):
+            hipops.muon_step(params, grads, momenta, lr=0.1)
+    for grads in ([g, g], [view(30), g]):                           # neighbours, and one gradient twice, are fine as far as memory goes
+        with pytest.raises(_lib.DmError):
+            hipops.muon_step([view(0), torch.zeros(4, 6)], grads, [view(54), torch.zeros(4, 6)], lr=0.1)
+
+
 def test_c_entries_refuse_before_any_launch():
     L = _lib.lib()
     ARG, WS, UNS = -1, -2, -3
@@ -152,7 +164,14 @@ def test_c_entries_refuse_before_any_launch():
                    (dict(ws=P + 16), ARG), (dict(ws=None), ARG), (dict(wb=need - 1), WS), (dict(rows=40000, cols=40000), UNS)]:
         assert ns(**kw) == rc, kw
     assert ns(count=0) == 0
-    assert L.dm_muon_step(ptrs, null, ptrs, 1, 8, 8, 2, 5, 0.9, 1, 1e-7, 1.0, 0.1, P, need, None) == ARG
+    eight, length = (ctypes.c_int * 1)(8), (ctypes.c_float * 1)(0.1)
+    mu = lambda g=ptrs, m=ptrs, p=ptrs, rows=eight, cols=eight, count=1, wb=need: L.dm_muon_step(g, m, p, rows, cols, length, count, 2, 5, 0.9, 1, 1e-7, 1.0, P, wb, None)
+    zero, huge = (ctypes.c_int * 1)(0), (ctypes.c_int * 1)(40000)
+    for kw, rc in [(dict(m=null), ARG), (dict(p=null), ARG), (dict(g=null), ARG), (dict(m=None), ARG), (dict(rows=None), ARG), (dict(rows=zero), ARG),
+                   (dict(rows=huge, cols=huge), UNS), (dict(count=-1), ARG), (dict(wb=need - 1), WS)]:
+        assert mu(**kw) == rc, kw
+    assert mu(count=0) == 0
+    assert L.dm_muon_step_workspace_bytes(eight, eight, 1) == need and L.dm_muon_step_workspace_bytes(zero, eight, 1) == 0
 
 
 def test_size_queries():

@@ -217,10 +217,13 @@ struct Launch {
 
 // block -> class, unit.  Block b runs on XCD b % 8: every XCD gets an eighth of each class's units, neighbours of a matrix together; the odd
 // units go to other XCDs class by class.  False: nothing to do.
-__device__ __forceinline__ bool locate(const Launch& l, int bid, int& c, int& id) {
-    c = 0;
-    while (c + 1 < l.classes && bid >= l.c[c + 1].first) ++c;
-    const int units = l.c[c].per_mat * l.c[c].count * l.c[c].splits, local = bid - l.c[c].first, x = ((local & 7) + 3 * c) & 7;
+__device__ __forceinline__ bool locate(const Launch& l, int bid, Class& c, int& id) {
+    int k = 0;
+    if (l.classes > 1) {
+        while (k + 1 < l.classes && bid >= l.c[k + 1].first) ++k;
+        c = l.c[k];
+    }
+    const int units = c.per_mat * c.count * c.splits, local = bid - c.first, x = ((local & 7) + 3 * k) & 7;
     id = (int)((long long)units * x / 8) + (local >> 3);
     return id < (int)((long long)units * (x + 1) / 8);
 }
@@ -253,20 +256,38 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
     [[maybe_unused]] constexpr bool SYM = KIND <= NS_POLY, SRC = KIND != NS_GRAM, LAST = KIND == NS_LAST;
     // the result in units of 2^13 (LAST: 1) from products in units of 2^26
     [[maybe_unused]] constexpr float ACC = LAST ? kInv * kInv : KIND == NS_POLY ? kC * kInv : kInv, OLD = LAST ? kA * kInv : KIND == NS_POLY ? kB : kA;
-    extern __shared__ __attribute__((aligned(16))) char smem[];      // max(NST * STAGE, 4 TR T)
+    // A 64 tile has LDS to spare for its source tile: requested before the products instead of waited for behind them
+    [[maybe_unused]] constexpr bool EARLY = SRC && T == 64;
+    extern __shared__ __attribute__((aligned(16))) char smem[];      // EARLY: NST * STAGE + 4 TR T, else the larger of the two
 #if defined(__HIP_DEVICE_COMPILE__)
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, hi = lane >> 5, l31 = lane & 31;
     const int wi = wave / WJ, wj = wave % WJ;
-    int cls, id;
-    if (!locate(l, blockIdx.x, cls, id)) return;
-    const Class& c = l.c[cls];
+    // the arguments come from memory: the first class and matrix are requested at once, so that one matrix waits for them once, not three times
+    Mat t = a.t[0];
+    Class c = l.c[0];
+    int id;
+    if (!locate(l, blockIdx.x, c, id)) return;
     const int tiles = c.per_mat * c.count, z = id / tiles, tile = id - z * tiles, rel = tile / c.per_mat, splits = c.splits;
     int ti, tj;
     tile_of<SYM>(c, tile - rel * c.per_mat, ti, tj);
-    const Mat& t = a.t[c.mat + rel];
+    if (c.mat + rel) t = a.t[c.mat + rel];
     const int mp = t.mp(), np = t.np();
     const int i0 = ti * T, j0 = tj * T;
     const int kw = KIND == NS_GRAM ? np : mp, ow = SYM ? mp : np, oh = mp;      // contraction; the result's columns and rows
+    char* const pane = smem + (EARLY ? NST * STAGE : 0);
+    auto source = [&](int r0) __attribute__((always_inline)) {         // rows r0 .. r0 + TR of the source tile
+        constexpr int P = TR * T / 256 / NW;                           // 1 KB = 8 blocks per wave and request
+        const _Float16* src = KIND == NS_POLY ? t.s() : t.x;
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(src + (long long)r0 * 2 * ow), 0, min(TR, oh - r0) * ow * 4, 0x00020000);
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int q = (wave * P + p) * 8 + (lane >> 3), row = q / (T / 32), blk = (q % (T / 32)) ^ ((row >> 3) & 1);
+            const int chunk = (lane & 7) ^ (row & 7);
+            const unsigned o = PAIR || chunk < 4 ? (unsigned)row * (unsigned)ow * 4u + (unsigned)((j0 / 32 + blk) * 128 + (chunk << 4)) : 0x80000000u;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(pane + (wave * P + p) * 1024), 16, (int)o, 0, 0, 0);
+        }
+    };
+    if constexpr (EARLY) source(i0);
     f32x16 acc[FI][FJ];
     {
         const _Float16* A = KIND == NS_GRAM ? t.x : KIND == NS_POLY ? t.s() : t.pm();
@@ -364,17 +385,8 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
         const int r0 = i0 + h * TR;                                    // first row of this pass
         if (h && r0 >= oh) break;
         __syncthreads();                                               // every wave has read its last fragments (its share of the last pass)
-        if constexpr (SRC) {
-            constexpr int P = TR * T / 256 / NW;                       // 1 KB = 8 blocks per wave and request
-            const _Float16* src = KIND == NS_POLY ? t.s() : t.x;
-            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(src + (long long)r0 * 2 * ow), 0, min(TR, oh - r0) * ow * 4, 0x00020000);
-#pragma unroll
-            for (int p = 0; p < P; ++p) {
-                const int q = (wave * P + p) * 8 + (lane >> 3), row = q / (T / 32), blk = (q % (T / 32)) ^ ((row >> 3) & 1);
-                const int chunk = (lane & 7) ^ (row & 7);
-                const unsigned o = PAIR || chunk < 4 ? (unsigned)row * (unsigned)ow * 4u + (unsigned)((j0 / 32 + blk) * 128 + (chunk << 4)) : 0x80000000u;
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(smem + (wave * P + p) * 1024), 16, (int)o, 0, 0, 0);
-            }
+        if constexpr (SRC && !EARLY) {
+            source(r0);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
         }
@@ -386,8 +398,8 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         const int row = (H == 1 ? TI * wi : 0) + 32 * fi + l31, blk = (TJ * wj) / 32 + fj;
-                        half4* vp = reinterpret_cast<half4*>(smem + tile_at<T>(row, blk, q) + 8 * hi);
-                        half4* rp = reinterpret_cast<half4*>(smem + tile_at<T>(row, blk, 4 + q) + 8 * hi);
+                        half4* vp = reinterpret_cast<half4*>(pane + tile_at<T>(row, blk, q) + 8 * hi);
+                        half4* rp = reinterpret_cast<half4*>(pane + tile_at<T>(row, blk, 4 + q) + 8 * hi);
                         float v[4];
 #pragma unroll
                         for (int r = 0; r < 4; ++r) v[r] = acc[fi][fj][4 * q + r] * ACC;
@@ -452,7 +464,7 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int rr = flip ? row + r : row, cc = flip ? col : col + r;
-                        o[r] = *reinterpret_cast<const float*>(smem + tile_at<T>(rr, cc >> 5, ((cc & 31) >> 3) + ((cc & 2) << 1)) + ((cc & 4) << 1) + ((cc & 1) << 2));
+                        o[r] = *reinterpret_cast<const float*>(pane + tile_at<T>(rr, cc >> 5, ((cc & 31) >> 3) + ((cc & 2) << 1)) + ((cc & 4) << 1) + ((cc & 1) << 2));
                     }
                     if (p) {
                         const float w[4] = {old[u].x * a.decay - t.step * o[0], old[u].y * a.decay - t.step * o[1], old[u].z * a.decay - t.step * o[2],
@@ -476,7 +488,7 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
                 const int chunk = q & 7, blk = (q >> 3) % (T / 32), row = (q >> 3) / (T / 32);
                 if (r0 + row < oh && j0 + 32 * blk < ow && (chunk < 4 || rests))
                     *reinterpret_cast<u32x4*>(D + (long long)(r0 + row) * 2 * ow + (j0 / 32 + blk) * 64 + chunk * 8) =
-                        *reinterpret_cast<const u32x4*>(smem + tile_at<T>(row, blk, chunk));
+                        *reinterpret_cast<const u32x4*>(pane + tile_at<T>(row, blk, chunk));
             }
             if (!SYM || ti != tj) {                                    // the other orientation: rows j, blocks of 32 i
                 _Float16* E = SYM ? D : t.xt(l.in ^ 1);
@@ -484,8 +496,8 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
                 for (int u = wave; u < (T / 16) * (TR / 32) * (1 + rests); u += NW) {
                     const int part = rests ? u & 1 : 0, v = u >> (int)rests, ib = v % (TR / 32), c0 = v / (TR / 32) * 16;
                     const int row = 32 * ib + 8 * grp + (l15 >> 2), cc = (c0 & 31) + 4 * (l15 & 3);
-                    const char* p0 = smem + tile_at<T>(row, c0 >> 5, (cc >> 3) + 4 * part) + ((cc & 4) << 1);
-                    const char* p1 = smem + tile_at<T>(row + 4, c0 >> 5, (cc >> 3) + 4 * part) + ((cc & 4) << 1);
+                    const char* p0 = pane + tile_at<T>(row, c0 >> 5, (cc >> 3) + 4 * part) + ((cc & 4) << 1);
+                    const char* p1 = pane + tile_at<T>(row + 4, c0 >> 5, (cc >> 3) + 4 * part) + ((cc & 4) << 1);
                     const elem4 q0 = dm_ds_read_tr16_b64(p0), q1 = dm_ds_read_tr16_b64(p1);
                     const elem8 o = {q0[0], q0[1], q0[2], q0[3], q1[0], q1[1], q1[2], q1[3]};
                     const int j = j0 + c0 + l15, i = r0 + 32 * ib;
@@ -623,7 +635,7 @@ Plan plan(const Mat* t, int count, int kind) {
 
 template <int KIND, int T, int NST, bool PAIR, typename OT>
 int launch_tile(const NsArgs& a, const Plan& p, int in, bool rests, float* part, hipStream_t stream) {
-    constexpr int LDS = std::max(NST * 2 * T * 128, T == 256 ? 2 * T * T : 4 * T * T);
+    constexpr int RING = NST * 2 * T * 128, TILE = T == 256 ? 2 * T * T : 4 * T * T, LDS = T == 64 && KIND != NS_GRAM ? RING + TILE : std::max(RING, TILE);
     static hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_ns_gemm<KIND, T, NST, PAIR, OT>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
     if (attr != hipSuccess) return (int)attr;
     Launch l = p.l;

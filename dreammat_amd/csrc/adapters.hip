@@ -277,38 +277,40 @@ __global__ __launch_bounds__(256) void k_shrink_ring(const elem_t* __restrict__ 
 #endif
 }
 
-// One row per blockIdx.x, one rank row per wave: requests of a few rows each, where a tile would hold many adapters.  Every row reads
+// One row per workgroup, one rank row per wave: requests of a few rows each, where a tile would hold many adapters.  Every row reads
 // its own adapter (R K 2 bytes).  f32out: plain fp32 [M][Rp] for the skinny product, else the pair format.
 __global__ __launch_bounds__(1024) void k_shrink_rows(const elem_t* __restrict__ x, const elem_t* __restrict__ A, Rows rows, int K, int R, float scale,
                                                       elem_t* __restrict__ u, float* __restrict__ us, float* __restrict__ f32out) {
     __shared__ float row[kMaxRank];
-    const long long m = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, Rp = rank_pad(R);
-    const int e = adapter_of(rows, m);
-    if (e == kNone) return;
-    const elem_t* xr = x + m * K;
-    for (int r = tid >> 6; r < R; r += blockDim.x >> 6) {
-        const elem_t* ar = A + ((long long)e * R + r) * K;
-        float s = 0.f;
-        for (int k = lane * 8; k < K; k += 512) {
-            const elem8 xv = *reinterpret_cast<const elem8*>(xr + k), av = *reinterpret_cast<const elem8*>(ar + k);
+    for (long long m = blockIdx.x; m < rows.M; m += gridDim.x) {
+        const int e = adapter_of(rows, m);
+        if (e == kNone) continue;
+        const elem_t* xr = x + m * K;
+        for (int r = tid >> 6; r < R; r += blockDim.x >> 6) {
+            const elem_t* ar = A + ((long long)e * R + r) * K;
+            float s = 0.f;
+            for (int k = lane * 8; k < K; k += 512) {
+                const elem8 xv = *reinterpret_cast<const elem8*>(xr + k), av = *reinterpret_cast<const elem8*>(ar + k);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s += (float)xv[i] * (float)av[i];
+                for (int i = 0; i < 8; ++i) s += (float)xv[i] * (float)av[i];
+            }
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+            if (lane == 0) row[r] = scale * s;
         }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-        if (lane == 0) row[r] = scale * s;
+        __syncthreads();
+        if (f32out) {
+            for (int r = tid; r < Rp; r += blockDim.x) f32out[m * Rp + r] = r < R ? row[r] : 0.f;
+        } else {
+            float big = 0.f;
+            for (int r = 0; r < R; ++r) big = fmaxf(big, fabsf(row[r]));
+            const float p = pow2_scale(big);
+            for (int r = tid; r < Rp; r += blockDim.x) store_pair(u + m * 2 * Rp, Rp, r, r < R ? row[r] / p : 0.f);
+            if (tid == 0) us[m] = p;
+        }
+        __syncthreads();
     }
-    __syncthreads();
-    if (f32out) {
-        for (int r = tid; r < Rp; r += blockDim.x) f32out[m * Rp + r] = r < R ? row[r] : 0.f;
-        return;
-    }
-    float big = 0.f;
-    for (int r = 0; r < R; ++r) big = fmaxf(big, fabsf(row[r]));
-    const float p = pow2_scale(big);
-    for (int r = tid; r < Rp; r += blockDim.x) store_pair(u + m * 2 * Rp, Rp, r, r < R ? row[r] / p : 0.f);
-    if (tid == 0) us[m] = p;
 }
 
 // ------------------------------------------------------------------------------------------------ expand
@@ -621,11 +623,11 @@ __global__ __launch_bounds__(512) void k_expand_skinny(ExpandArgs a, const float
 // ------------------------------------------------------------------------------------------------ layouts of the adapters
 // 32 x 32 tiles through LDS.  pad: dst[e][c][0 .. Rp) = src[e][c][0 .. R), zeros behind (B whose rank rows are not whole 16-byte chunks)
 __global__ __launch_bounds__(256) void k_adapter_pad(const elem_t* __restrict__ src, elem_t* __restrict__ dst, long long rows, int R, int Rp) {
-    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (at >= rows * Rp) return;
-    const long long c = at / Rp;
-    const int r = (int)(at - c * Rp);
-    dst[at] = r < R ? src[c * R + r] : (elem_t)0.f;
+    for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < rows * Rp; at += 256LL * gridDim.x) {
+        const long long c = at / Rp;
+        const int r = (int)(at - c * Rp);
+        dst[at] = r < R ? src[c * R + r] : (elem_t)0.f;
+    }
 }
 
 // The operands of the data gradient: at [E, K, Rp] = A^T with zeros past R (from A [E, R, K]) and bt [E, R, N] = B^T (from B [E, N, R]).
@@ -927,6 +929,8 @@ Rows make_rows(const int* ids, const int* offsets, long long n, long long M, int
     return r;
 }
 
+constexpr long long kMostBlocks = 1 << 20;      // of a grid whose workgroups loop (a grid holds fewer than 2^32 threads)
+
 // requests shorter than this share a tile with many others: one row at a time then
 bool few_rows_each(long long M, long long n) { return M < 8 * n; }
 
@@ -938,8 +942,8 @@ void launch_shrink(const elem_t* x, const elem_t* A, const Rows& rows, int K, in
 template <int NR>
 int launch_ring(const elem_t* x, const elem_t* A, const Rows& rows, int K, int R, float scale, elem_t* u, float* us, hipStream_t stream) {
     constexpr int LDS = 4 * (64 + 16 * NR) * 128 + 64 * 4;
-    static hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_shrink_ring<NR>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-    if (attr != hipSuccess) return (int)attr;
+    static unsigned long long devices = 0;
+    DM_HIP(dm_dynamic_lds(reinterpret_cast<const void*>(&k_shrink_ring<NR>), LDS, devices));
     hipLaunchKernelGGL((k_shrink_ring<NR>), dim3((unsigned)((rows.M + 63) / 64)), dim3(256), LDS, stream, x, A, rows, K, R, scale, u, us);
     DM_LAUNCH_CHECK();
     return DM_OK;
@@ -948,7 +952,7 @@ int launch_ring(const elem_t* x, const elem_t* A, const Rows& rows, int K, int R
 // Many rows: 64-row tiles through LDS; few: 32 or 16 rows per workgroup, whose waves share K; requests of a few rows: one row each.
 int shrink(const elem_t* x, const elem_t* A, const Rows& rows, int K, int R, float scale, elem_t* u, float* us, hipStream_t stream) {
     if (few_rows_each(rows.M, rows.n)) {
-        hipLaunchKernelGGL(k_shrink_rows, dim3((unsigned)rows.M), dim3(std::min(1024, 64 * R)), 0, stream, x, A, rows, K, R, scale, u, us, (float*)nullptr);
+        hipLaunchKernelGGL(k_shrink_rows, dim3((unsigned)std::min(rows.M, kMostBlocks)), dim3(std::min(1024, 64 * R)), 0, stream, x, A, rows, K, R, scale, u, us, (float*)nullptr);
         DM_LAUNCH_CHECK();
         return DM_OK;
     }
@@ -984,8 +988,8 @@ int launch_expand(ExpandArgs a, hipStream_t stream) {
     if (n_mt * a.n_nt > (1LL << 30)) return DM_ERR_UNSUPPORTED;
     a.n_mt = (int)n_mt;
     a.tiles = (int)(n_mt * a.n_nt);
-    static hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_expand<BM, BN, WM, WN, NST>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-    if (attr != hipSuccess) return (int)attr;
+    static unsigned long long devices = 0;
+    DM_HIP(dm_dynamic_lds(reinterpret_cast<const void*>(&k_expand<BM, BN, WM, WN, NST>), LDS, devices));
     hipLaunchKernelGGL((k_expand<BM, BN, WM, WN, NST>), dim3((unsigned)((a.tiles + 7) / 8 * 8)), dim3(WM * WN * 64), LDS, stream, a);
     DM_LAUNCH_CHECK();
     return DM_OK;
@@ -1058,7 +1062,7 @@ int DM_T(dm_linear_adapted_, )(const void* x, const void* w, const void* bias, c
     DM_ENTER();
     if (R % 8) {
         elem_t* padded = (elem_t*)((char*)ws + u_bytes(M, R));
-        hipLaunchKernelGGL(k_adapter_pad, dim3((unsigned)(((long long)E * N * Rp + 255) / 256)), dim3(256), 0, stream, a.B, padded, (long long)E * N, R, Rp);
+        hipLaunchKernelGGL(k_adapter_pad, dim3((unsigned)std::min(((long long)E * N * Rp + 255) / 256, kMostBlocks)), dim3(256), 0, stream, a.B, padded, (long long)E * N, R, Rp);
         a.B = padded;
         a.ldb = Rp;
     }

@@ -28,4 +28,15 @@
         if (e__ != hipSuccess) return (int)e__;    \
     } while (0)
 
+// More than 64 KB of dynamic LDS for a kernel: asked for once per device (`devices`: the kernel's static record of them, one bit each).
+static inline hipError_t dm_dynamic_lds(const void* kernel, int bytes, unsigned long long& devices) {
+    int dev = 0;
+    if (hipError_t e = hipGetDevice(&dev); e != hipSuccess) return e;
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (__atomic_load_n(&devices, __ATOMIC_RELAXED) & bit) return hipSuccess;
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess) __atomic_fetch_or(&devices, bit, __ATOMIC_RELAXED);
+    return e;
+}
+
 static inline int dm_div_up(long long a, long long b) { return (int)((a + b - 1) / b); }

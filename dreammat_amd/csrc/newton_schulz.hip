@@ -636,8 +636,8 @@ Plan plan(const Mat* t, int count, int kind) {
 template <int KIND, int T, int NST, bool PAIR, typename OT>
 int launch_tile(const NsArgs& a, const Plan& p, int in, bool rests, float* part, hipStream_t stream) {
     constexpr int RING = NST * 2 * T * 128, TILE = T == 256 ? 2 * T * T : 4 * T * T, LDS = T == 64 && KIND != NS_GRAM ? RING + TILE : std::max(RING, TILE);
-    static hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_ns_gemm<KIND, T, NST, PAIR, OT>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-    if (attr != hipSuccess) return (int)attr;
+    static unsigned long long devices = 0;
+    DM_HIP(dm_dynamic_lds(reinterpret_cast<const void*>(&k_ns_gemm<KIND, T, NST, PAIR, OT>), LDS, devices));
     Launch l = p.l;
     l.in = in;
     l.rests = rests;

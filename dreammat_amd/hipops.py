@@ -1772,6 +1772,7 @@ def _ptr(t):
 
 
 MAX_ADAPTER_RANK = 128
+MAX_TRAINED_ADAPTERS = 60000            # row ranges of the weight gradients are one dimension of a grid: one per adapter and up to 1024 more
 _ADAPTER_FN = {}        # element type -> forward, backward entry points
 
 
@@ -1885,6 +1886,8 @@ def linear_adapted_autograd(x, w, w_t, bias, lora_a, lora_b, ids, scale=1.0, res
         raise ValueError("linear_adapted_autograd: the projection is frozen (w or bias requires a gradient)")
     if w_t.shape != w.shape[::-1] or w_t.dtype != w.dtype or w_t.device != w.device:
         raise ValueError("linear_adapted_autograd: w_t is w transposed, of its type and on its device")
+    if lora_a.dim() == 3 and lora_a.shape[0] > MAX_TRAINED_ADAPTERS:
+        raise ValueError(f"linear_adapted_autograd: {lora_a.shape[0]} adapters: at most {MAX_TRAINED_ADAPTERS} can be trained together")
     return _LinearAdapted.apply(x, w, w_t, bias, lora_a, lora_b, ids, float(scale), residual, offsets)
 
 

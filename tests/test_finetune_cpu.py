@@ -58,6 +58,8 @@ def test_linear_adapted_autograd_refuses_a_trainable_projection_and_a_foreign_tr
         hipops.linear_adapted_autograd(w_t=v["w"].t().contiguous(), **adapter(w=torch.zeros(72, 64, dtype=BF, requires_grad=True)))
     with pytest.raises(ValueError):
         hipops.linear_adapted_autograd(w_t=v["w"].t().contiguous(), **adapter(bias=torch.zeros(72, dtype=BF, requires_grad=True)))
+    with pytest.raises(ValueError, match="trained together"):
+        hipops.linear_adapted_autograd(w_t=v["w"].t().contiguous(), **adapter(lora_a=torch.zeros(60001, 1, 64, dtype=BF), lora_b=torch.zeros(60001, 72, 1, dtype=BF)))
 
 
 ONE = torch.ones(64)

@@ -152,6 +152,21 @@ def test_linear_adapted_keeps_other_adapters_infinities_out():
         assert not torch.isfinite(got[q:2 * q].float()).any()
 
 
+def test_linear_adapted_of_millions_of_single_rows():
+    """more rows with an adapter each than one grid has workgroups"""
+    from dreammat_amd import hipops
+    M = (1 << 22) + 77
+    g = gen(11)
+    x, w, a, b = rand(g, M, 8, dtype=BF), rand(g, 8, 8, dtype=BF), rand(g, 5, 16, 8, dtype=BF), rand(g, 5, 8, 16, dtype=BF)
+    ids = torch.randint(-1, 5, (M,), generator=g, device=DEV, dtype=torch.int32)
+    y = hipops.linear_adapted(x, w, None, a, b, ids)
+    at = torch.cat([torch.arange(0, 300), torch.arange((1 << 20) - 100, (1 << 20) + 100), torch.arange((1 << 21) - 5, (1 << 21) + 200), torch.arange(M - 300, M)]).to(DEV)
+    xs, e = x[at].double(), ids[at].long()
+    low = [torch.where((e >= 0)[:, None], torch.matmul(torch.matmul(v.unsqueeze(1), p[e.clamp(min=0)].mT.contiguous()), q[e.clamp(min=0)].mT.contiguous())[:, 0], 0.0)
+           for v, p, q in ((xs, a.double(), b.double()), (xs.abs(), a.double().abs(), b.double().abs()))]
+    near(y[at], xs @ w.double().T + low[0], xs.abs() @ w.double().abs().T + low[1], 8 + 16 + 16, 2.0 ** -17)
+
+
 @pytest.mark.parametrize("size", [1e-6, 1e4])
 def test_linear_adapted_half_range_of_the_low_rank_factor(size):
     """u = x A^T far outside and far below half's range, B the other way round: the pair keeps its bits (row scales)"""
@@ -462,6 +477,41 @@ def test_muon_step_groups_of_many_matrices_equal_single_ones():
     for a, b, c in zip(p2, gr, m2):
         hipops.muon_step([a], [b], [c], lr=0.1, scale="spectral")
     assert all(torch.equal(a, b) for a, b in zip(p + m, p2 + m2))
+
+
+@pytest.mark.parametrize("shapes", [
+    [(192, 5000), (130, 2100), (64, 64)],                                                                # few tiles: the Gram contraction in shares
+    [(1024, 1100), (640, 5120), (2560, 300), (1024, 1100), (70, 9000), (1024, 1100), (33, 33)],          # classes of one and of three
+    [(320 + 64 * (i % 5), 200 + 37 * i) for i in range(19)],                                             # two groups
+    [(1280, 1280)] * 9 + [(1280, 4000)]])                                                                # whole rounds of the largest tiles
+def test_muon_step_of_many_shapes_at_once_against_64_bits(shapes):
+    from dreammat_amd import hipops
+    g = gen(len(shapes))
+    p, m = ([rand(g, *q, scale=c) for q in shapes] for c in (0.02, 1e-3))
+    gr = [rand(g, *q, scale=1e-3) for q in shapes]
+    want = []
+    for a, b, c in zip(p, m, gr):
+        mm = 0.9 * b.double() + c.double()
+        up = 0.1 * 0.2 * max(a.shape) ** 0.5 * ns_formula(c.double() + 0.9 * mm)
+        want.append((a.double() * (1 - 0.1 * 0.02) - up, mm, up))
+    state = [q.clone() for q in p + m]
+    hipops.muon_step(p, gr, m, lr=0.1, momentum=0.9, weight_decay=0.02)
+    for a, b, (pa, mm, up) in zip(p, m, want):
+        assert (b.double() - mm).abs().max() <= 3 * 2.0 ** -24 * 8e-3
+        assert (a.double() - pa).norm() <= NS_TOL[FP] * up.norm() + 3 * 2.0 ** -24 * pa.norm()
+    n = len(shapes)
+    hipops.muon_step(state[:n], gr, state[n:], lr=0.1, momentum=0.9, weight_decay=0.02)
+    assert all(torch.equal(a, b) for a, b in zip(p + m, state))                  # no atomics: the same bits
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("shape", [(128, 320), (640, 320)])
+def test_orthogonalize_of_a_few_strong_directions(shape, dtype):
+    """three directions a thousand times the others, as gradients have them: the weak ones are what the iteration amplifies most"""
+    from dreammat_amd import hipops
+    g = gen(9)
+    u = (rand(g, shape[0], 3) @ rand(g, 3, shape[1]) + 1e-3 * rand(g, *shape)).to(dtype)
+    assert rel(hipops.orthogonalize(u), ns_formula(u)) <= NS_TOL[dtype]
 
 
 # ------------------------------------------------------------------------------------------------ together

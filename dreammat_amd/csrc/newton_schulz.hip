@@ -6,8 +6,7 @@
 // (a, b, c) = (3.4445, -4.7750, 2.0315): every singular value s in (0, 1] runs through s <- a s + b s^3 + c s^5 and lands near 1.
 //
 // Bound by the matrix pipe: m^2 n + m^3 + 2 m^2 n flops per iteration (S and S S are symmetric: only the tiles on and below the diagonal
-// are computed and stored twice).  All products are row-by-row (both operands contiguous along the contraction): X is kept in both
-// orientations, S and P are symmetric, and an epilogue writes its tile both ways.
+// are computed and stored twice).  X X^T and S S take both operands row by row; P X takes X along its rows, turned by the transposing LDS read.
 //
 // Precision.  The iteration multiplies a small singular value -- and every rounding error next to it -- by a^5 = 485, so 8 bits (bf16
 // storage) leave 1e-2 of error in the result and 11 bits (half) 1e-3, 1e-2 where a few directions dominate the matrix.  Numbers are
@@ -48,7 +47,7 @@ struct Mat {
     float* mom;              // momentum, or NULL
     float* p;                // parameter, or NULL
     void* out;               // orthogonalised matrix, or NULL
-    _Float16* x;             // pairs: X [mp][np], X^T [np][mp] twice (ping-pong), S [mp][mp], P [mp][mp]
+    _Float16* work;          // pairs: X [mp][np] twice (ping-pong), S [mp][mp], P [mp][mp]
     int rows, cols;
     float step;
     short parts;             // workgroups of the norm pass
@@ -58,9 +57,9 @@ struct Mat {
     __host__ __device__ int mp() const { return (m() + 63) & ~63; }
     __host__ __device__ int np() const { return (n() + 63) & ~63; }
     __device__ bool flip() const { return rows > cols; }
-    __device__ _Float16* xt(int k) const { return x + (long long)(1 + k) * mp() * 2 * np(); }
-    __device__ _Float16* s() const { return xt(2); }
-    __device__ _Float16* pm() const { return xt(2) + (long long)mp() * 2 * mp(); }
+    __device__ _Float16* x(int k) const { return work + (long long)k * mp() * 2 * np(); }
+    __device__ _Float16* s() const { return x(2); }
+    __device__ _Float16* pm() const { return x(2) + (long long)mp() * 2 * mp(); }
 };
 
 struct NsArgs {
@@ -129,7 +128,7 @@ __global__ __launch_bounds__(256) void k_ns_norm(NsArgs a) {
     if (threadIdx.x == 0) a.norm[(long long)b * kNormParts + blockIdx.x] = red[0] + red[1] + red[2] + red[3];
 }
 
-// X0 and X0^T as pairs, zero past m and n; a 64 x 64 tile through LDS per workgroup
+// X0 as pairs, zero past m and n; a 64 x 64 tile through LDS per workgroup
 template <typename T>
 __global__ __launch_bounds__(256) void k_ns_pack(NsArgs a) {
     __shared__ float tile[64][65];
@@ -160,7 +159,7 @@ __global__ __launch_bounds__(256) void k_ns_pack(NsArgs a) {
         else tile[r][tx] = v[q] * inv;
     }
     __syncthreads();
-    _Float16 *x = t.x, *xt = t.xt(0);
+    _Float16* x = t.x(0);
 #pragma unroll
     for (int q = 0; q < 2; ++q) {                                               // eight entries of a row per thread: 16-byte stores
         const int r = (threadIdx.x >> 3) + 32 * q, c = (threadIdx.x & 7) * 8;
@@ -175,16 +174,6 @@ __global__ __launch_bounds__(256) void k_ns_pack(NsArgs a) {
         const long long at = pair_at(i0 + r, j0 + c, np);
         *reinterpret_cast<half8*>(x + at) = h;
         *reinterpret_cast<half8*>(x + at + 32) = l;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            _Float16 p, w;
-            split(tile[c + k][r], p, w);
-            h[k] = p;
-            l[k] = w;
-        }
-        const long long to = pair_at(j0 + r, i0 + c, mp);
-        *reinterpret_cast<half8*>(xt + to) = h;
-        *reinterpret_cast<half8*>(xt + to + 32) = l;
     }
 }
 
@@ -195,10 +184,10 @@ __device__ __forceinline__ int tile_at(int row, int blk, int chunk) {
     return (row * (T / 32) + (blk ^ ((row >> 3) & 1))) * 128 + ((chunk ^ (row & 7)) << 4);
 }
 
-// The products of the iteration, all C = A B^T over pair matrices:
-//   GRAM  A = B = X,         S = C
-//   POLY  A = B = S,         P = b S + c C
-//   STEP  A = P, B = X^T,    X <- a X + C  in both orientations (X in place: a tile is read and written by its own workgroup only)
+// The products of the iteration over pair matrices:
+//   GRAM  S = X X^T
+//   POLY  P = b S + c S S^T
+//   STEP  X' = a X + P X, from one copy of X into the other
 //   LAST  the same, into the parameter or the output
 enum { NS_GRAM = 0, NS_POLY = 1, NS_STEP = 2, NS_LAST = 3 };
 
@@ -212,7 +201,7 @@ struct Class {
 struct Launch {
     Class c[kGroup];
     float* part;             // fp32 partial sums [share][T * T]
-    int classes, in, rests;  // which X^T is read; whether the result's readers take its rests
+    int classes, in, rests;  // which copy of X is read; whether the result's readers take its rests
 };
 
 // block -> class, unit.  Block b runs on XCD b % 8: every XCD gets an eighth of each class's units, neighbours of a matrix together; the odd
@@ -242,13 +231,14 @@ __device__ __forceinline__ void tile_of(const Class& c, int rem, int& ti, int& t
     }
 }
 
-// Tile T x T, two rows of WJ waves of T/2 x T/WJ.  K goes in blocks of 128 bytes per row through a ring of NST LDS stages filled by
-// buffer_load ... lds (chunks XOR-swizzled by (row >> 1) & 7), NST - 1 of them in flight: 32 pairs (PAIR: three products per block) or the
-// values of 64.
+// Tile T x T, two rows of WJ waves of T/2 x T/WJ.  K goes in steps of 32 pairs (PAIR: three products) or the values of 64, through a ring of
+// NST LDS stages filled by buffer_load ... lds, NST - 1 of them in flight.  A stage holds T rows of the left operand, 128 bytes of K each
+// (chunks XOR-swizzled by (row >> 1) & 7), and of the right one, S or X^T, the same -- or, in P X, the 32 or 64 rows of X along K,
+// T columns each, which the transposing LDS read turns (chunks XOR-swizzled by 4 (row & 3): its four rows meet different banks).
 // GRAM and POLY are symmetric: tiles i >= j, stored twice.
-// The epilogue goes through LDS: the tile of S or X arrives as whole lines, every lane replaces its own entries, and whole lines leave in both
-// orientations (the transposed one by ds_read_b64_tr_b16); a 256 tile does that half by half.  A share of a split contraction leaves its fp32
-// sums in l.part instead, for k_ns_join.
+// The epilogue goes through LDS: the tile of S or X arrives as whole lines, every lane replaces its own entries, and whole lines leave (GRAM,
+// POLY: in both orientations, the transposed one by the transposing read); a 256 tile does that half by half.  A share of a split
+// contraction leaves its fp32 sums in l.part instead, for k_ns_join.
 template <int KIND, int T, int NST, bool PAIR, typename OT>
 __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
     [[maybe_unused]] constexpr int NT = threads_of(T), NW = NT / 64, WJ = NW / 2, ROWB = 128, STAGE = 2 * T * ROWB, TI = T / 2, TJ = T / WJ, FI = TI / 32, FJ = TJ / 32,
@@ -274,10 +264,13 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
     const int mp = t.mp(), np = t.np();
     const int i0 = ti * T, j0 = tj * T;
     const int kw = KIND == NS_GRAM ? np : mp, ow = SYM ? mp : np, oh = mp;      // contraction; the result's columns and rows
+    // rows of X of a stage (P X), their bytes and 16-byte chunks; the swizzle of row's chunks (64 values of a row are half the banks wide)
+    [[maybe_unused]] constexpr int KR = PAIR ? 32 : 64, RB = PAIR ? 4 * T : 2 * T, CPR = RB / 16;
+    [[maybe_unused]] auto turn = [](int row) __attribute__((always_inline)) { return CPR == 8 ? (row & 2) << 1 : (row & 3) << 2; };
     char* const pane = smem + (EARLY ? NST * STAGE : 0);
     auto source = [&](int r0) __attribute__((always_inline)) {         // rows r0 .. r0 + TR of the source tile
         constexpr int P = TR * T / 256 / NW;                           // 1 KB = 8 blocks per wave and request
-        const _Float16* src = KIND == NS_POLY ? t.s() : t.x;
+        const _Float16* src = KIND == NS_POLY ? t.s() : t.x(l.in);
         const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(src + (long long)r0 * 2 * ow), 0, min(TR, oh - r0) * ow * 4, 0x00020000);
 #pragma unroll
         for (int p = 0; p < P; ++p) {
@@ -290,11 +283,10 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
     if constexpr (EARLY) source(i0);
     f32x16 acc[FI][FJ];
     {
-        const _Float16* A = KIND == NS_GRAM ? t.x : KIND == NS_POLY ? t.s() : t.pm();
-        const _Float16* B = SYM ? A : t.xt(l.in);
+        const _Float16* A = KIND == NS_GRAM ? t.x(l.in) : KIND == NS_POLY ? t.s() : t.pm();
         const int arows = min(T, oh - i0), brows = min(T, ow - j0);
         const __amdgpu_buffer_rsrc_t ars = __builtin_amdgcn_make_buffer_rsrc((void*)(A + (long long)i0 * 2 * kw), 0, arows * kw * 4, 0x00020000);
-        const __amdgpu_buffer_rsrc_t brs = __builtin_amdgcn_make_buffer_rsrc((void*)(B + (long long)j0 * 2 * kw), 0, brows * kw * 4, 0x00020000);
+        const __amdgpu_buffer_rsrc_t brs = __builtin_amdgcn_make_buffer_rsrc((void*)(A + (long long)j0 * 2 * kw), 0, brows * kw * 4, 0x00020000);      // (SYM)
         unsigned off[PIECES];                                      // rows past the matrix lie past the descriptor: zeros
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
@@ -302,14 +294,29 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
             const int chunk = (lane & 7) ^ ((row >> 1) & 7);       // (values only: chunks 4 .. 7 are the next block's values)
             off[p] = (unsigned)row * (unsigned)kw * 4u + (unsigned)(PAIR ? chunk * 16 : (chunk >> 2) * 128 + (chunk & 3) * 16);
         }
+        [[maybe_unused]] unsigned xoff[PIECES];                    // P X: rows along K of X, columns past it out of range
+        if constexpr (!SYM) {
+#pragma unroll
+            for (int p = 0; p < PIECES; ++p) {
+                const int q = (wave * PIECES + p) * 64 + lane, row = q / CPR, chunk = (q % CPR) ^ turn(row), blk = chunk >> (PAIR ? 3 : 2);
+                xoff[p] = j0 + 32 * blk < ow ? (unsigned)row * (unsigned)ow * 4u + (unsigned)((j0 / 32 + blk) * 128 + (chunk & (PAIR ? 7 : 3)) * 16) : 0x80000000u;
+            }
+        }
         auto issue = [&](int s, int stage) __attribute__((always_inline)) {
             char* base = smem + stage * STAGE;
 #pragma unroll
             for (int p = 0; p < PIECES; ++p)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(ars, (__attribute__((address_space(3))) void*)(base + (wave * (T / NW) + 8 * p) * ROWB), 16, (int)off[p], s * (PAIR ? 128 : 256), 0, 0);
+            if constexpr (SYM) {
 #pragma unroll
-            for (int p = 0; p < PIECES; ++p)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(brs, (__attribute__((address_space(3))) void*)(base + T * ROWB + (wave * (T / NW) + 8 * p) * ROWB), 16, (int)off[p], s * (PAIR ? 128 : 256), 0, 0);
+                for (int p = 0; p < PIECES; ++p)
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(brs, (__attribute__((address_space(3))) void*)(base + T * ROWB + (wave * (T / NW) + 8 * p) * ROWB), 16, (int)off[p], s * (PAIR ? 128 : 256), 0, 0);
+            } else {
+                const __amdgpu_buffer_rsrc_t xrs = __builtin_amdgcn_make_buffer_rsrc((void*)(t.x(l.in) + (long long)s * KR * 2 * ow), 0, KR * ow * 4, 0x00020000);
+#pragma unroll
+                for (int p = 0; p < PIECES; ++p)
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(xrs, (__attribute__((address_space(3))) void*)(base + T * ROWB + (wave * PIECES + p) * 1024), 16, (int)xoff[p], 0, 0, 0);
+            }
         };
 #pragma unroll
         for (int i = 0; i < FI; ++i)
@@ -319,6 +326,63 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
                 for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
         auto frag = [&](const char* base, int row, int chunk) __attribute__((always_inline)) {
             return *reinterpret_cast<const half8*>(base + row * ROWB + ((chunk ^ ((row >> 1) & 7)) << 4));
+        };
+        // eight k of one column of X per lane: two transposing reads of four rows each
+        [[maybe_unused]] const int l15 = lane & 15, col = 16 * ((lane >> 4) & 1) + 4 * (l15 & 3), first = 8 * hi + (l15 >> 2);
+        [[maybe_unused]] int at[FJ][2];                            // (turn has period 4: the steps along K are constants)
+        if constexpr (!SYM) {
+#pragma unroll
+            for (int j = 0; j < FJ; ++j)
+#pragma unroll
+                for (int part = 0; part < 2; ++part) {
+                    const int blk = TJ / 32 * wj + j, chunk = (PAIR ? 8 * blk + 4 * part : 4 * blk) + (col >> 3);
+                    at[j][part] = T * ROWB + first * RB + ((chunk ^ turn(first)) << 4) + ((col & 4) << 1);
+                }
+        }
+        // All of a stage's fragments of X before the next stage is requested: the compiler lets a transposing read wait for every request in flight,
+        // which costs nothing while there is none.  The deeper ring of 64 tiles always has some: there the reads bring their own wait.
+        [[maybe_unused]] half8 xt[PAIR ? 2 : 4][FJ][PAIR ? 2 : 1];
+        auto turned = [&](const char* base) __attribute__((always_inline)) {
+            constexpr int KK = PAIR ? 2 : 4, PARTS = PAIR ? 2 : 1;
+            elem4 q[KK][FJ][PARTS][2];
+            if constexpr (T == 64) {
+                const unsigned p0 = (unsigned)(uintptr_t)(base + at[0][0]), p1 = (unsigned)(uintptr_t)(base + at[0][PARTS - 1]);
+                if constexpr (PAIR)
+                    asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%10\n\t"
+                                 "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%10\n\t"
+                                 "ds_read_b64_tr_b16 %4, %8 offset:%11\n\tds_read_b64_tr_b16 %5, %8 offset:%12\n\t"
+                                 "ds_read_b64_tr_b16 %6, %9 offset:%11\n\tds_read_b64_tr_b16 %7, %9 offset:%12\n\ts_waitcnt lgkmcnt(0)"
+                                 : "=&v"(q[0][0][0][0]), "=&v"(q[0][0][0][1]), "=&v"(q[0][0][1][0]), "=&v"(q[0][0][1][1]), "=&v"(q[1][0][0][0]),
+                                   "=&v"(q[1][0][0][1]), "=&v"(q[1][0][1][0]), "=&v"(q[1][0][1][1])
+                                 : "v"(p0), "v"(p1), "n"(4 * RB), "n"(16 * RB), "n"(20 * RB) : "memory");
+                else
+                    asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%9\n\t"
+                                 "ds_read_b64_tr_b16 %2, %8 offset:%10\n\tds_read_b64_tr_b16 %3, %8 offset:%11\n\t"
+                                 "ds_read_b64_tr_b16 %4, %8 offset:%12\n\tds_read_b64_tr_b16 %5, %8 offset:%13\n\t"
+                                 "ds_read_b64_tr_b16 %6, %8 offset:%14\n\tds_read_b64_tr_b16 %7, %8 offset:%15\n\ts_waitcnt lgkmcnt(0)"
+                                 : "=&v"(q[0][0][0][0]), "=&v"(q[0][0][0][1]), "=&v"(q[1][0][0][0]), "=&v"(q[1][0][0][1]), "=&v"(q[KK - 2][0][0][0]),
+                                   "=&v"(q[KK - 2][0][0][1]), "=&v"(q[KK - 1][0][0][0]), "=&v"(q[KK - 1][0][0][1])
+                                 : "v"(p0), "n"(4 * RB), "n"(16 * RB), "n"(20 * RB), "n"(32 * RB), "n"(36 * RB), "n"(48 * RB), "n"(52 * RB) : "memory");
+            } else {
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+                    for (int j = 0; j < FJ; ++j)
+#pragma unroll
+                        for (int part = 0; part < PARTS; ++part) {
+                            q[kk][j][part][0] = dm_ds_read_tr16_b64(base + at[j][part] + 16 * kk * RB);
+                            q[kk][j][part][1] = dm_ds_read_tr16_b64(base + at[j][part] + (16 * kk + 4) * RB);
+                        }
+            }
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+                for (int j = 0; j < FJ; ++j)
+#pragma unroll
+                    for (int part = 0; part < PARTS; ++part) {
+                        const elem4 u = q[kk][j][part][0], v = q[kk][j][part][1];
+                        xt[kk][j][part] = __builtin_bit_cast(half8, elem8{u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]});
+                    }
         };
         const int all = kw / (PAIR ? 32 : 64);
         const int s_lo = (int)((long long)all * z / splits), s_hi = (int)((long long)all * (z + 1) / splits);
@@ -332,9 +396,10 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
             else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
+            const char* ab = smem + st * STAGE;
+            if constexpr (!SYM) turned(ab);
             const int fill = st == 0 ? NST - 1 : st - 1;           // the stage read one step ago
             if (s + NST - 1 < s_hi) issue(s + NST - 1, fill);
-            const char* ab = smem + st * STAGE;
             const char* bb = ab + T * ROWB;
 #pragma unroll
             for (int kk = 0; kk < (PAIR ? 2 : 4); ++kk) {
@@ -347,9 +412,14 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
                 }
 #pragma unroll
                 for (int j = 0; j < FJ; ++j) {
-                    const int row = TJ * wj + 32 * j + l31;
-                    bh[j] = frag(bb, row, 2 * kk + hi);
-                    if constexpr (PAIR) bl[j] = frag(bb, row, 4 + 2 * kk + hi);
+                    if constexpr (SYM) {
+                        const int row = TJ * wj + 32 * j + l31;
+                        bh[j] = frag(bb, row, 2 * kk + hi);
+                        if constexpr (PAIR) bl[j] = frag(bb, row, 4 + 2 * kk + hi);
+                    } else {
+                        bh[j] = xt[kk][j][0];
+                        if constexpr (PAIR) bl[j] = xt[kk][j][1];
+                    }
                 }
                 // B as the matrix instruction's first operand: a lane holds one row i and four consecutive columns j per group
 #pragma unroll
@@ -481,7 +551,7 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
                 }
             }
         } else {
-            _Float16* D = KIND == NS_GRAM ? t.s() : KIND == NS_POLY ? t.pm() : t.x;
+            _Float16* D = KIND == NS_GRAM ? t.s() : KIND == NS_POLY ? t.pm() : t.x(l.in ^ 1);
             const bool rests = KIND == NS_STEP ? l.rests : PAIR;
 #pragma unroll 4
             for (int q = tid; q < TR * T / 4; q += NT) {               // 16-byte chunks, whole rows of blocks
@@ -490,8 +560,7 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
                     *reinterpret_cast<u32x4*>(D + (long long)(r0 + row) * 2 * ow + (j0 / 32 + blk) * 64 + chunk * 8) =
                         *reinterpret_cast<const u32x4*>(pane + tile_at<T>(row, blk, chunk));
             }
-            if (!SYM || ti != tj) {                                    // the other orientation: rows j, blocks of 32 i
-                _Float16* E = SYM ? D : t.xt(l.in ^ 1);
+            if (SYM && ti != tj) {                                     // the other half: rows j, blocks of 32 i
                 const int l15 = lane & 15, grp = lane >> 4;
                 for (int u = wave; u < (T / 16) * (TR / 32) * (1 + rests); u += NW) {
                     const int part = rests ? u & 1 : 0, v = u >> (int)rests, ib = v % (TR / 32), c0 = v / (TR / 32) * 16;
@@ -501,7 +570,7 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
                     const elem4 q0 = dm_ds_read_tr16_b64(p0), q1 = dm_ds_read_tr16_b64(p1);
                     const elem8 o = {q0[0], q0[1], q0[2], q0[3], q1[0], q1[1], q1[2], q1[3]};
                     const int j = j0 + c0 + l15, i = r0 + 32 * ib;
-                    if (j < ow && i < oh) *reinterpret_cast<elem8*>(E + pair_at(j, i, oh) + 8 * grp + 32 * part) = o;
+                    if (j < ow && i < oh) *reinterpret_cast<elem8*>(D + pair_at(j, i, oh) + 8 * grp + 32 * part) = o;
                 }
             }
         }
@@ -686,12 +755,12 @@ int run_group(const NsArgs& a, int count, int steps, float* part, hipStream_t st
     const int plain_from = SHORT ? std::max(1, steps - 2) : steps;
     for (int k = 0; k < steps; ++k) {
         if (k < plain_from) {
-            NS_TRY((launch_gemm<NS_GRAM, true, float>(a, gram, 0, true, part, stream)));
+            NS_TRY((launch_gemm<NS_GRAM, true, float>(a, gram, k & 1, true, part, stream)));
             NS_TRY((launch_gemm<NS_POLY, true, float>(a, poly, 0, true, part, stream)));
             if (k + 1 < steps) NS_TRY((launch_gemm<NS_STEP, true, float>(a, step, k & 1, k + 1 < plain_from, part, stream)));
             else NS_TRY((launch_gemm<NS_LAST, true, T>(a, step, k & 1, false, part, stream)));
         } else if constexpr (SHORT) {
-            NS_TRY((launch_gemm<NS_GRAM, false, float>(a, gram, 0, false, part, stream)));
+            NS_TRY((launch_gemm<NS_GRAM, false, float>(a, gram, k & 1, false, part, stream)));
             NS_TRY((launch_gemm<NS_POLY, false, float>(a, poly, 0, false, part, stream)));
             if (k + 1 < steps) NS_TRY((launch_gemm<NS_STEP, false, float>(a, step, k & 1, false, part, stream)));
             else NS_TRY((launch_gemm<NS_LAST, false, T>(a, step, k & 1, false, part, stream)));
@@ -700,8 +769,8 @@ int run_group(const NsArgs& a, int count, int steps, float* part, hipStream_t st
     return DM_OK;
 }
 
-// workspace of one matrix (x, two x^T, s, p, norm) and of a group
-long long mat_bytes(const Mat& t) { return 4LL * t.mp() * (3LL * t.np() + 2LL * t.mp()) + 8 * kNormParts; }
+// workspace of one matrix (X twice, S, P, norm) and of a group
+long long mat_bytes(const Mat& t) { return 4LL * t.mp() * (2LL * t.np() + 2LL * t.mp()) + 8 * kNormParts; }
 long long group_bytes(const Mat* t, int count) {
     const Plan gram = plan(t, count, NS_GRAM);
     long long b = 4LL * gram.shares * gram.tile * gram.tile;
@@ -746,7 +815,7 @@ int run(std::vector<Mat>& t, NsArgs& a, int dtype, int steps, void* ws, size_t w
         w += 8LL * kNormParts * c;
         for (int i = 0; i < c; ++i) {
             a.t[i] = t[at + i];
-            a.t[i].x = (_Float16*)w;
+            a.t[i].work = (_Float16*)w;
             w += mat_bytes(a.t[i]) - 8 * kNormParts;
         }
         float* part = (float*)w;

@@ -11,7 +11,7 @@
 // Precision.  The iteration multiplies a small singular value -- and every rounding error next to it -- by a^5 = 485, so 8 bits (bf16
 // storage) leave 1e-2 of error in the result and 11 bits (half) 1e-3, 1e-2 where a few directions dominate the matrix.  Numbers are
 // therefore kept as a PAIR of halves, value + rest (22 bits; scaled by 2^13, so that neither leaves half's range: |X| <= 1.2, |S| <=
-// 1.5, |P| <= 2.9), and a product is value value + value rest + rest value with fp32 sums: the result agrees with fp32 arithmetic to its
+// 1.5, |P + a| <= 3.5), and a product is value value + value rest + rest value with fp32 sums: the result agrees with fp32 arithmetic to its
 // own rounding (1.7e-6 against 1.7e-6 of the fp32 form on a 1024^2 Gaussian).  For bf16 input the last two iterations, whose
 // errors are hardly amplified any more, take (and are given) the values only: 1e-3 of error under the 1.7e-3 of the rounding to bf16.
 // (Taking the polynomials of S = X X^T alone and multiplying X0 once saves half the products of a wide matrix, but S holds squared singular
@@ -186,8 +186,8 @@ __device__ __forceinline__ int tile_at(int row, int blk, int chunk) {
 
 // The products of the iteration over pair matrices:
 //   GRAM  S = X X^T
-//   POLY  P = b S + c S S^T
-//   STEP  X' = a X + P X, from one copy of X into the other
+//   POLY  P = b S + c S S^T (pairs: + a on the diagonal)
+//   STEP  X' = a X + P X (pairs: P X), from one copy of X into the other
 //   LAST  the same, into the parameter or the output
 enum { NS_GRAM = 0, NS_POLY = 1, NS_STEP = 2, NS_LAST = 3 };
 
@@ -243,7 +243,9 @@ template <int KIND, int T, int NST, bool PAIR, typename OT>
 __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
     [[maybe_unused]] constexpr int NT = threads_of(T), NW = NT / 64, WJ = NW / 2, ROWB = 128, STAGE = 2 * T * ROWB, TI = T / 2, TJ = T / WJ, FI = TI / 32, FJ = TJ / 32,
                                    PIECES = T / 8 / NW, H = T == 256 ? 2 : 1, TR = T / H;       // TR rows per epilogue pass
-    [[maybe_unused]] constexpr bool SYM = KIND <= NS_POLY, SRC = KIND != NS_GRAM, LAST = KIND == NS_LAST;
+    [[maybe_unused]] constexpr bool SYM = KIND <= NS_POLY, LAST = KIND == NS_LAST;
+    // pairs: the a of a X sits on the diagonal of P, so X is not read again; values alone would round it to 11 bits
+    [[maybe_unused]] constexpr bool DIAG = KIND == NS_POLY && PAIR, SRC = KIND == NS_POLY || (!SYM && !PAIR);
     // the result in units of 2^13 (LAST: 1) from products in units of 2^26
     [[maybe_unused]] constexpr float ACC = LAST ? kInv * kInv : KIND == NS_POLY ? kC * kInv : kInv, OLD = LAST ? kA * kInv : KIND == NS_POLY ? kB : kA;
     // A 64 tile has LDS to spare for its source tile: requested before the products instead of waited for behind them
@@ -477,6 +479,10 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
                             const half4 hv = *vp, lv = *rp;
 #pragma unroll
                             for (int r = 0; r < 4; ++r) v[r] += OLD * ((float)hv[r] + (float)lv[r]);
+                            if constexpr (DIAG) {
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) v[r] += r0 + row == j0 + 32 * blk + 8 * q + 4 * hi + r ? kA * kScale : 0.f;
+                            }
                         }
                         if constexpr (LAST) {                          // fp32 in the pair's place: columns 0, 1 | 2, 3 of the four
                             *reinterpret_cast<float2*>(vp) = make_float2(v[0], v[1]);
@@ -704,7 +710,7 @@ Plan plan(const Mat* t, int count, int kind) {
 
 template <int KIND, int T, int NST, bool PAIR, typename OT>
 int launch_tile(const NsArgs& a, const Plan& p, int in, bool rests, float* part, hipStream_t stream) {
-    constexpr int RING = NST * 2 * T * 128, TILE = T == 256 ? 2 * T * T : 4 * T * T, LDS = T == 64 && KIND != NS_GRAM ? RING + TILE : std::max(RING, TILE);
+    constexpr int RING = NST * 2 * T * 128, TILE = T == 256 ? 2 * T * T : 4 * T * T, LDS = T == 64 && (KIND == NS_POLY || (KIND >= NS_STEP && !PAIR)) ? RING + TILE : std::max(RING, TILE);
     static unsigned long long devices = 0;
     DM_HIP(dm_dynamic_lds(reinterpret_cast<const void*>(&k_ns_gemm<KIND, T, NST, PAIR, OT>), LDS, devices));
     Launch l = p.l;

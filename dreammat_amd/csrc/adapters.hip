@@ -68,7 +68,8 @@ __device__ __forceinline__ float pow2_scale(float biggest) {
 }
 
 // ------------------------------------------------------------------------------------------------ shrink
-// u rows are stored [value: Rp | rest: Rp] elem_t (Rp = rank_pad(R), columns past R zero) with us[m] = the row's power of two.
+// u rows are stored [value: Rp | rest: Rp] elem_t (Rp = rank_pad(R), columns past R zero) with us[m] = the row's power of two and who[m] = the
+// row's adapter, which the big product then reads instead of searching for it.
 __device__ __forceinline__ void store_pair(elem_t* u, int Rp, int r, float v) {
     const elem_t hi = (elem_t)v;
     u[r] = hi;
@@ -95,13 +96,16 @@ __device__ __forceinline__ int next_adapter(const int* aid, int cur) {
 // that occurs in the tile.  Bound by the x read.
 template <int RT, int NR>
 __global__ __launch_bounds__(256) void k_shrink(const elem_t* __restrict__ x, const elem_t* __restrict__ A, Rows rows, int K, int R, float scale,
-                                                elem_t* __restrict__ u, float* __restrict__ us) {
+                                                elem_t* __restrict__ u, float* __restrict__ us, int* __restrict__ who) {
     constexpr int TR = 16 * RT, Rp = 16 * NR;
     __shared__ float part[4][TR][Rp + 1];
     __shared__ int aid[TR];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l15 = lane & 15, kq = lane >> 4;
     const long long m0 = (long long)blockIdx.x * TR;
-    if (tid < TR) aid[tid] = adapter_of(rows, m0 + tid);
+    if (tid < TR) {
+        aid[tid] = adapter_of(rows, m0 + tid);
+        if (m0 + tid < rows.M) who[m0 + tid] = aid[tid];
+    }
     __syncthreads();
     const elem_t* xr[RT];
 #pragma unroll
@@ -189,7 +193,7 @@ __global__ __launch_bounds__(256) void k_shrink(const elem_t* __restrict__ x, co
 // [24576, 5120] 187 -> 66 us.
 template <int NR>
 __global__ __launch_bounds__(256) void k_shrink_ring(const elem_t* __restrict__ x, const elem_t* __restrict__ A, Rows rows, int K, int R, float scale,
-                                                     elem_t* __restrict__ u, float* __restrict__ us) {
+                                                     elem_t* __restrict__ u, float* __restrict__ us, int* __restrict__ who) {
     [[maybe_unused]] constexpr int Rp = 16 * NR, ROWB = 128, STAGE = (64 + Rp) * ROWB, NST = 4, PA = Rp >= 32 ? Rp / 32 : 1;
     extern __shared__ __attribute__((aligned(16))) char smem[];      // NST STAGE | int aid[64]
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -201,7 +205,10 @@ __global__ __launch_bounds__(256) void k_shrink_ring(const elem_t* __restrict__ 
     const __amdgpu_buffer_rsrc_t xrs = __builtin_amdgcn_make_buffer_rsrc((void*)(x + m0 * K), 0, mrows * K * 2, 0x00020000);
     // x pieces: rows 16 wave + 8 i; rank pieces: rows 8 p of A (with 16 ranks two waves fetch each piece)
     auto chunk_of = [&](int row) __attribute__((always_inline)) { return (unsigned)(((lane & 7) ^ ((row >> 1) & 7)) * 8); };
-    if (tid < 64) aid[tid] = adapter_of(rows, m0 + tid);
+    if (tid < 64) {
+        aid[tid] = adapter_of(rows, m0 + tid);
+        if (tid < mrows) who[m0 + tid] = aid[tid];
+    }
     __syncthreads();
     int cur = kNone;
     for (;;) {
@@ -280,11 +287,12 @@ __global__ __launch_bounds__(256) void k_shrink_ring(const elem_t* __restrict__ 
 // One row per workgroup, one rank row per wave: requests of a few rows each, where a tile would hold many adapters.  Every row reads
 // its own adapter (R K 2 bytes).  f32out: plain fp32 [M][Rp] for the skinny product, else the pair format.
 __global__ __launch_bounds__(1024) void k_shrink_rows(const elem_t* __restrict__ x, const elem_t* __restrict__ A, Rows rows, int K, int R, float scale,
-                                                      elem_t* __restrict__ u, float* __restrict__ us, float* __restrict__ f32out) {
+                                                      elem_t* __restrict__ u, float* __restrict__ us, int* __restrict__ who, float* __restrict__ f32out) {
     __shared__ float row[kMaxRank];
     const int tid = threadIdx.x, lane = tid & 63, Rp = rank_pad(R);
     for (long long m = blockIdx.x; m < rows.M; m += gridDim.x) {
         const int e = adapter_of(rows, m);
+        if (!f32out && tid == 0) who[m] = e;
         if (e == kNone) continue;
         const elem_t* xr = x + m * K;
         for (int r = tid >> 6; r < R; r += blockDim.x >> 6) {
@@ -317,6 +325,7 @@ __global__ __launch_bounds__(1024) void k_shrink_rows(const elem_t* __restrict__
 struct ExpandArgs {
     const elem_t *x, *w, *bias, *res, *u, *B;
     const float* us;
+    const int* who;
     elem_t* y;
     Rows rows;
     int K, N, R, ldb;      // ldb: elements between the rows of B (a multiple of 8)
@@ -431,9 +440,10 @@ __global__ __launch_bounds__(WM * WN * 64) void k_expand(ExpandArgs a) {
     issue();                                                         // (the first step of K)
     int ahead = 1, plain = 1;
     for (int t = tid; t < BM; t += NW * 64) {
-        const int e = adapter_of(a.rows, m0 + t);
+        const int e = t < mrows ? a.who[m0 + t] : kNone;
+        const float scale = t < mrows ? a.us[m0 + t] : 1.f;
         aid[t] = e;
-        scale_of[t] = e != kNone ? a.us[m0 + t] : 1.f;
+        scale_of[t] = e != kNone ? scale : 1.f;
         if (scale_of[t] != 1.f) plain = 0;
     }
     for (int t = tid; t < BN; t += NW * 64) bias_of[t] = a.bias && n0 + t < a.N ? (float)a.bias[n0 + t] : 0.f;
@@ -683,7 +693,11 @@ __global__ __launch_bounds__(1024) void k_wgrad_plan(Rows rows, int chunk, int* 
             }
             __syncthreads();
             const int n = min(1024, rows.n - b);
-            for (int i = 0; i < n; ++i) count = (int)min(rows.M, (long long)count + (id[i] == e0 + tid ? len[i] : 0));
+            {
+                const unsigned most = (unsigned)rows.M;              // (sums of two stay below 2^32)
+#pragma unroll 8
+                for (int i = 0; i < n; ++i) count = (int)min(most, (unsigned)count + (id[i] == e0 + tid ? (unsigned)len[i] : 0u));
+            }
         }
         if (e0 + tid < E) first[e0 + tid + 1] = count;
     }
@@ -712,8 +726,9 @@ __global__ __launch_bounds__(1024) void k_wgrad_plan(Rows rows, int chunk, int* 
             }
             __syncthreads();
             const int n = min(1024, rows.n - b);
+#pragma unroll 8
             for (int i = 0; i < n; ++i)
-                if (id[i] == e0 + tid) { start[b + i] = at; at = (int)min(rows.M, (long long)at + len[i]); }
+                if (id[i] == e0 + tid) { start[b + i] = at; at = (int)min((unsigned)rows.M, (unsigned)at + (unsigned)len[i]); }
         }
     }
 }
@@ -935,43 +950,43 @@ constexpr long long kMostBlocks = 1 << 20;      // of a grid whose workgroups lo
 bool few_rows_each(long long M, long long n) { return M < 8 * n; }
 
 template <int RT, int NR>
-void launch_shrink(const elem_t* x, const elem_t* A, const Rows& rows, int K, int R, float scale, elem_t* u, float* us, hipStream_t stream) {
-    hipLaunchKernelGGL((k_shrink<RT, NR>), dim3((unsigned)((rows.M + 16 * RT - 1) / (16 * RT))), dim3(256), 0, stream, x, A, rows, K, R, scale, u, us);
+void launch_shrink(const elem_t* x, const elem_t* A, const Rows& rows, int K, int R, float scale, elem_t* u, float* us, int* who, hipStream_t stream) {
+    hipLaunchKernelGGL((k_shrink<RT, NR>), dim3((unsigned)((rows.M + 16 * RT - 1) / (16 * RT))), dim3(256), 0, stream, x, A, rows, K, R, scale, u, us, who);
 }
 
 template <int NR>
-int launch_ring(const elem_t* x, const elem_t* A, const Rows& rows, int K, int R, float scale, elem_t* u, float* us, hipStream_t stream) {
+int launch_ring(const elem_t* x, const elem_t* A, const Rows& rows, int K, int R, float scale, elem_t* u, float* us, int* who, hipStream_t stream) {
     constexpr int LDS = 4 * (64 + 16 * NR) * 128 + 64 * 4;
     static unsigned long long devices = 0;
     DM_HIP(dm_dynamic_lds(reinterpret_cast<const void*>(&k_shrink_ring<NR>), LDS, devices));
-    hipLaunchKernelGGL((k_shrink_ring<NR>), dim3((unsigned)((rows.M + 63) / 64)), dim3(256), LDS, stream, x, A, rows, K, R, scale, u, us);
+    hipLaunchKernelGGL((k_shrink_ring<NR>), dim3((unsigned)((rows.M + 63) / 64)), dim3(256), LDS, stream, x, A, rows, K, R, scale, u, us, who);
     DM_LAUNCH_CHECK();
     return DM_OK;
 }
 
 // Many rows: 64-row tiles through LDS; few: 32 or 16 rows per workgroup, whose waves share K; requests of a few rows: one row each.
-int shrink(const elem_t* x, const elem_t* A, const Rows& rows, int K, int R, float scale, elem_t* u, float* us, hipStream_t stream) {
+int shrink(const elem_t* x, const elem_t* A, const Rows& rows, int K, int R, float scale, elem_t* u, float* us, int* who, hipStream_t stream) {
     if (few_rows_each(rows.M, rows.n)) {
-        hipLaunchKernelGGL(k_shrink_rows, dim3((unsigned)std::min(rows.M, kMostBlocks)), dim3(std::min(1024, 64 * R)), 0, stream, x, A, rows, K, R, scale, u, us, (float*)nullptr);
+        hipLaunchKernelGGL(k_shrink_rows, dim3((unsigned)std::min(rows.M, kMostBlocks)), dim3(std::min(1024, 64 * R)), 0, stream, x, A, rows, K, R, scale, u, us, who, (float*)nullptr);
         DM_LAUNCH_CHECK();
         return DM_OK;
     }
     const int Rp = rank_pad(R);
     if (rows.M >= 64 * 192) {                                        // (tiles for three quarters of the CUs)
         switch (Rp) {
-            case 16: return launch_ring<1>(x, A, rows, K, R, scale, u, us, stream);
-            case 32: return launch_ring<2>(x, A, rows, K, R, scale, u, us, stream);
-            case 64: return launch_ring<4>(x, A, rows, K, R, scale, u, us, stream);
-            default: return launch_ring<8>(x, A, rows, K, R, scale, u, us, stream);
+            case 16: return launch_ring<1>(x, A, rows, K, R, scale, u, us, who, stream);
+            case 32: return launch_ring<2>(x, A, rows, K, R, scale, u, us, who, stream);
+            case 64: return launch_ring<4>(x, A, rows, K, R, scale, u, us, who, stream);
+            default: return launch_ring<8>(x, A, rows, K, R, scale, u, us, who, stream);
         }
     }
     auto go = [&](auto rt_tag) {
         constexpr int RT = decltype(rt_tag)::value;
         switch (Rp) {
-            case 16: launch_shrink<RT, 1>(x, A, rows, K, R, scale, u, us, stream); break;
-            case 32: launch_shrink<RT, 2>(x, A, rows, K, R, scale, u, us, stream); break;
-            case 64: launch_shrink<RT, 4>(x, A, rows, K, R, scale, u, us, stream); break;
-            default: launch_shrink<RT, 8>(x, A, rows, K, R, scale, u, us, stream); break;
+            case 16: launch_shrink<RT, 1>(x, A, rows, K, R, scale, u, us, who, stream); break;
+            case 32: launch_shrink<RT, 2>(x, A, rows, K, R, scale, u, us, who, stream); break;
+            case 64: launch_shrink<RT, 4>(x, A, rows, K, R, scale, u, us, who, stream); break;
+            default: launch_shrink<RT, 8>(x, A, rows, K, R, scale, u, us, who, stream); break;
         }
     };
     if (rows.M >= 32 * 256) go(std::integral_constant<int, 2>{});
@@ -996,18 +1011,20 @@ int launch_expand(ExpandArgs a, hipStream_t stream) {
 }
 
 // Tile by the rounds a launch takes: a round of 768 tiles of 64 x 64 (three per CU) takes 0.34 / 0.6 of one of 512 tiles of 128 x 128 (two per
-// CU) for 0.37 of the work.  (256 x 256 tiles are 6-14 % faster on the bare product, but their accumulators leave no registers for rows
+// CU) for 0.37 of the work.  Where every CU gets at most one 64 tile its ring is as deep as LDS allows (both directions of [382, 976, 728]
+// 21.6 -> 19.7 us).  (256 x 256 tiles are 6-14 % faster on the bare product, but their accumulators leave no registers for rows
 // of several adapters: with spills 850 against 500 us on [24576, 1280, 5120].)
 int expand(const ExpandArgs& a, hipStream_t stream) {
     auto rounds = [&](long long t, long long per) { return (double)(((a.rows.M + t - 1) / t * ((a.N + t - 1) / t) + per - 1) / per); };
     if (0.6 * rounds(128, 512) <= 0.34 * rounds(64, 768)) return launch_expand<128, 128, 2, 2, 2>(a, stream);
+    if ((a.rows.M + 63) / 64 * ((a.N + 63) / 64) <= 256) return launch_expand<64, 64, 2, 2, 8>(a, stream);
     return launch_expand<64, 64, 2, 2, 3>(a, stream);
 }
 
 constexpr long long kSkinny = 32;
 
 long long align256(long long v) { return (v + 255) / 256 * 256; }
-long long u_bytes(long long M, int R) { return align256(M * (4LL * rank_pad(R) + 4)); }
+long long u_bytes(long long M, int R) { return align256(M * (4LL * rank_pad(R) + 8)); }
 
 int check_product(const Rows& r, const void* x, const void* w, const void* lora_a, const void* lora_b, int K, int N, int R) {
     if (!x || !lora_a || !lora_b || K <= 0 || N <= 0 || R <= 0) return DM_ERR_ARG;
@@ -1026,7 +1043,7 @@ long long wgrad_items(long long M, int E, int chunk) { return std::min<long long
 extern "C" {
 
 #if !defined(DM_F16)
-// bytes of the forward's workspace: u as pairs of 16-bit columns and one fp32 scale per row, then B with padded rank rows where R % 8 != 0
+// bytes of the forward's workspace: u as pairs of 16-bit columns, one fp32 scale and one adapter per row, then B with padded rank rows where R % 8 != 0
 size_t dm_linear_adapted_workspace_bytes(long long M, int N, int R, int E) {
     if (M <= 0 || N <= 0 || R <= 0 || R > kMaxRank || E <= 0) return 0;
     return (size_t)(u_bytes(M, R) + (R % 8 ? 2LL * E * N * rank_pad(R) : 0));
@@ -1056,7 +1073,7 @@ int DM_T(dm_linear_adapted_, )(const void* x, const void* w, const void* bias, c
     if ((long long)ws_bytes < u_bytes(M, R) + (R % 8 ? 2LL * E * N * Rp : 0)) return DM_ERR_WORKSPACE;
     ExpandArgs a{};
     a.x = (const elem_t*)x; a.w = (const elem_t*)w; a.bias = (const elem_t*)bias; a.res = (const elem_t*)residual;
-    a.u = (const elem_t*)ws; a.us = (const float*)((const elem_t*)ws + M * 2 * Rp); a.B = (const elem_t*)lora_b; a.y = (elem_t*)y;
+    a.u = (const elem_t*)ws; a.us = (const float*)((const elem_t*)ws + M * 2 * Rp); a.who = (const int*)(a.us + M); a.B = (const elem_t*)lora_b; a.y = (elem_t*)y;
     a.rows = rows;
     a.K = K; a.N = N; a.R = R; a.ldb = R;
     DM_ENTER();
@@ -1069,14 +1086,14 @@ int DM_T(dm_linear_adapted_, )(const void* x, const void* w, const void* bias, c
     if (M <= kSkinny && !keep_u) {
         float* uf = (float*)ws;
         hipLaunchKernelGGL(k_shrink_rows, dim3((unsigned)M), dim3(std::min(1024, 64 * R)), 0, stream, a.x, (const elem_t*)lora_a, a.rows, K, R, scale,
-                           (elem_t*)nullptr, (float*)nullptr, uf);
+                           (elem_t*)nullptr, (float*)nullptr, (int*)nullptr, uf);
         const dim3 grid((unsigned)((N + 15) / 16));
         if (M <= 16) hipLaunchKernelGGL(k_expand_skinny<1>, grid, dim3(512), 0, stream, a, uf);
         else hipLaunchKernelGGL(k_expand_skinny<2>, grid, dim3(512), 0, stream, a, uf);
         DM_LAUNCH_CHECK();
         return DM_OK;
     }
-    if (int rc = shrink(a.x, (const elem_t*)lora_a, a.rows, K, R, scale, (elem_t*)ws, const_cast<float*>(a.us), stream)) return rc;
+    if (int rc = shrink(a.x, (const elem_t*)lora_a, a.rows, K, R, scale, (elem_t*)ws, const_cast<float*>(a.us), const_cast<int*>(a.who), stream)) return rc;
     return expand(a, stream);
 }
 
@@ -1107,11 +1124,11 @@ int DM_T(dm_linear_adapted_bwd_, )(const void* x, const void* dy, const void* w_
         const int at_tiles = dx ? (K + 31) / 32 : 0;
         hipLaunchKernelGGL(k_adapter_transpose, dim3((unsigned)(at_tiles + (N + 31) / 32), (unsigned)((Rp + 31) / 32), (unsigned)E), dim3(256), 0, stream,
                            (const elem_t*)lora_a, (const elem_t*)lora_b, at, bt, K, N, R, Rp, at_tiles);
-        if (int rc = shrink((const elem_t*)dy, bt, rows, N, R, scale, du, dus, stream)) return rc;
+        if (int rc = shrink((const elem_t*)dy, bt, rows, N, R, scale, du, dus, (int*)(dus + M), stream)) return rc;
     }
     if (dx) {
         ExpandArgs a{};
-        a.x = (const elem_t*)dy; a.w = (const elem_t*)w_t; a.u = du; a.us = dus; a.B = at; a.y = (elem_t*)dx; a.rows = rows;
+        a.x = (const elem_t*)dy; a.w = (const elem_t*)w_t; a.u = du; a.us = dus; a.who = (const int*)(dus + M); a.B = at; a.y = (elem_t*)dx; a.rows = rows;
         a.K = N; a.N = K; a.R = R; a.ldb = Rp;
         if (int rc = expand(a, stream)) return rc;
     }

@@ -179,7 +179,7 @@ def test_c_entries_refuse_before_any_launch():
 def test_size_queries():
     L = _lib.lib()
     up = lambda v: (v + 255) // 256 * 256
-    u = lambda M, r: up(M * (4 * r + 4))                                             # pairs of 16-bit columns (padded rank), a scale per row
+    u = lambda M, r: up(M * (4 * r + 8))                                             # pairs of 16-bit columns (padded rank), a scale and an adapter per row
     assert [L.dm_linear_adapted_workspace_bytes(10, 64, r, 3) for r in (16, 24, 64, 128)] == [u(10, p) for p in (16, 32, 64, 128)]
     assert [L.dm_linear_adapted_workspace_bytes(10, 64, r, 3) for r in (1, 33)] == [u(10, p) + 2 * 3 * 64 * p for p in (16, 64)]      # + B in padded rows
     assert L.dm_linear_adapted_workspace_bytes(0, 64, 16, 1) == L.dm_linear_adapted_workspace_bytes(4, 64, 129, 1) == 0

@@ -636,7 +636,7 @@ __global__ __launch_bounds__(256) void k_ns_join(NsArgs a, Launch l) {
 
 // A launch of one kind over a group, and what it should take, in K steps of 32 pairs on one CU with a 256 tile (2.8 us).
 // Measured on 1280^2, paired: a 256 tile needs a third of a 128 tile's LDS and request traffic per product; 128 tiles run two per CU and a
-// round of 512 costs 1.15, half a round 0.6; 64 tiles 0.3 per 512, 0.25 where a CU gets one (then with a ring as deep as LDS allows: its
+// round of 512 costs 1.15, half a round 0.6; 64 tiles 0.3 per 512, 0.18 where a CU gets one (then with a ring as deep as LDS allows: its
 // loads have nothing else to hide behind).  Rounds: of equal units, whole ones; of unequal ones (longest first) the longest, or a tenth more
 // than their mean over the CUs.
 struct Plan {
@@ -689,17 +689,18 @@ Plan plan_tile(const Mat* t, int count, int kind, int T, int length) {
     };
     if (T == 256) p.cost = rounds(256);
     else if (T == 128) p.cost = std::max(0.6 * longest, 1.15 * work / 512);
-    else p.cost = p.units <= 256 ? 0.25 * longest : 0.3 * rounds(512);
+    else p.cost = p.units <= 256 ? 0.18 * longest : 0.3 * rounds(512);
     if (p.shares) p.cost += 2 + 0.05 * p.shares * (T * T) / 65536;       // the join: a launch, 256 KB written and read per share of a 256 tile
     if (top < T || (long long)p.shares * T * T * 4 > kShareBytes) p.cost = 1e30;
     return p;
 }
 
 Plan plan(const Mat* t, int count, int kind) {
-    Plan best = plan_tile(t, count, kind, 64, 0);
+    Plan best{};
+    best.cost = 2e30;
     int most = 0;
     for (int i = 0; i < count; ++i) most = std::max(most, t[i].np() / 32);
-    for (int T = 128; T <= 256; T *= 2)
+    for (int T = 64; T <= 256; T *= 2)
         for (int d = 0; d <= (kind == NS_GRAM ? 16 : 0); ++d) {          // shares of a d-th of the longest contraction
             if (d && most / d < 16) break;
             const Plan p = plan_tile(t, count, kind, T, d ? (most + d - 1) / d : 0);
@@ -719,7 +720,7 @@ int launch_tile(const NsArgs& a, const Plan& p, int in, bool rests, float* part,
     l.part = part;
     hipLaunchKernelGGL((k_ns_gemm<KIND, T, NST, PAIR, OT>), dim3(p.blocks), dim3(threads_of(T)), LDS, stream, a, l);
     DM_LAUNCH_CHECK();
-    if constexpr (KIND == NS_GRAM && T >= 128) {
+    if constexpr (KIND == NS_GRAM) {
         if (!p.shares) return DM_OK;
         int n = 0, blocks = 0;
         for (int c = 0; c < p.l.classes; ++c) {

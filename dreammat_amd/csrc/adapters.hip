@@ -190,7 +190,7 @@ __global__ __launch_bounds__(256) void k_shrink(const elem_t* __restrict__ x, co
 
 // The same for many rows: tiles of 64 rows, x and the rank rows through a ring of LDS stages (buffer_load ... lds, whole 128-byte lines,
 // three stages in flight), a wave 16 rows.  Against the kernel above, whose fragments are gathered from 16 rows by every load: rank 64 of
-// [24576, 5120] 187 -> 66 us.
+// [24576, 5120] 187 -> 70 us.
 template <int NR>
 __global__ __launch_bounds__(256) void k_shrink_ring(const elem_t* __restrict__ x, const elem_t* __restrict__ A, Rows rows, int K, int R, float scale,
                                                      elem_t* __restrict__ u, float* __restrict__ us, int* __restrict__ who) {
@@ -667,7 +667,8 @@ __global__ __launch_bounds__(256) void k_adapter_transpose(const elem_t* __restr
 
 // ------------------------------------------------------------------------------------------------ weight gradient
 // Plan (one workgroup): first[e] = rows of adapters < e, item[e] = row ranges ("items" of `chunk` rows) of adapters < e, and perm =
-// the rows in adapter order, ascending inside an adapter (-1: no row; only where offsets do not ascend).  Requests in batches of 1024 through LDS; thread e adds up adapter e's.
+// the rows in adapter order, ascending inside an adapter (-1: no row; only where offsets do not ascend).  Requests in batches of 1024 through
+// LDS; thread e adds up adapter e's.
 __device__ __forceinline__ void request_rows(const Rows& r, int i, long long& lo, long long& hi) {
     lo = r.offsets ? r.offsets[i] : i * r.each;
     hi = r.offsets ? r.offsets[i + 1] : (i + 1) * r.each;
@@ -680,7 +681,8 @@ __global__ __launch_bounds__(1024) void k_wgrad_plan(Rows rows, int chunk, int* 
     __shared__ int id[1024], len[1024];
     const int tid = threadIdx.x, E = rows.E;
     for (long long m = tid; m < rows.M; m += 1024) perm[m] = kNone;
-    // counts into first[e + 1]
+    // a thousand adapters at a time: their rows, then (one thread, in LDS) the running sums
+    int f = 0, it = 0;
     for (int e0 = 0; e0 < E; e0 += 1024) {
         int count = 0;
         for (int b = 0; b < rows.n; b += 1024) {
@@ -693,25 +695,28 @@ __global__ __launch_bounds__(1024) void k_wgrad_plan(Rows rows, int chunk, int* 
             }
             __syncthreads();
             const int n = min(1024, rows.n - b);
-            {
-                const unsigned most = (unsigned)rows.M;              // (sums of two stay below 2^32)
+            const unsigned most = (unsigned)rows.M;                  // (sums of two stay below 2^32)
 #pragma unroll 8
-                for (int i = 0; i < n; ++i) count = (int)min(most, (unsigned)count + (id[i] == e0 + tid ? (unsigned)len[i] : 0u));
+            for (int i = 0; i < n; ++i) count = (int)min(most, (unsigned)count + (id[i] == e0 + tid ? (unsigned)len[i] : 0u));
+        }
+        __syncthreads();
+        id[tid] = count;
+        __syncthreads();
+        if (tid == 0) {
+            for (int e = 0; e < min(1024, E - e0); ++e) {
+                const int c = min(id[e], (int)rows.M - f);           // (offsets that do not ascend: never more than M rows)
+                it += (c + chunk - 1) / chunk;
+                id[e] = f += c;
+                len[e] = it;
             }
         }
-        if (e0 + tid < E) first[e0 + tid + 1] = count;
-    }
-    __syncthreads();
-    if (tid == 0) {
-        int f = 0, it = 0;
-        first[0] = item[0] = 0;
-        for (int e = 0; e < E; ++e) {
-            const int c = min(first[e + 1], (int)rows.M - f);       // (offsets that do not ascend: never more than M rows)
-            it += (c + chunk - 1) / chunk;
-            first[e + 1] = f += c;
-            item[e + 1] = it;
+        __syncthreads();
+        if (e0 + tid < E) {
+            first[e0 + tid + 1] = id[tid];
+            item[e0 + tid + 1] = len[tid];
         }
     }
+    if (tid == 0) first[0] = item[0] = 0;
     __syncthreads();
     // start[i] = place of request i's first row
     for (int e0 = 0; e0 < E; e0 += 1024) {
@@ -909,25 +914,58 @@ __global__ __launch_bounds__(256) void k_wgrad(WgradArgs a) {
     }
 }
 
-// dA[e][r][c] and dB[e][c][r] = the sums of the adapter's items in a fixed order (four shares, eight loads in flight each), rounded once; an
-// adapter without rows gets zeros.  Workgroup = 64 columns x one rank; blockIdx.x: the column blocks of dA, then those of dB.
+// dA[e][r][c] and dB[e][c][r] = the sums of the adapter's items in a fixed order (eight loads in flight), rounded once; an adapter without rows
+// gets zeros.  Workgroup = 64 columns x RANKS ranks; blockIdx.x: the column blocks of dA, then those of dB.  RANKS 1: the waves share the
+// items.  16: four ranks per wave, stored in runs of 32 bytes on the dB side, whose ranks are adjacent (64 ranks of [1280 + 5120] for 8
+// adapters of 3 or 4 items each: 14 us, 27 with one rank per workgroup).
+template <int RANKS>
 __global__ __launch_bounds__(256) void k_wgrad_join(WgradArgs a, int blocks_a, int Rp) {
-    __shared__ float red[4][64];
+    __shared__ float red[RANKS == 1 ? 4 : RANKS][65];
     const int side = (int)blockIdx.x >= blocks_a, C = a.C[side];
-    const int e = blockIdx.z, r = blockIdx.y, tx = threadIdx.x & 63, q = threadIdx.x >> 6, c = ((int)blockIdx.x - (side ? blocks_a : 0)) * 64 + tx;
+    const int e = blockIdx.z, tx = threadIdx.x & 63, q = threadIdx.x >> 6, c0 = ((int)blockIdx.x - (side ? blocks_a : 0)) * 64, c = c0 + tx;
     const int lo = a.item[e], n = a.item[e + 1] - lo;
-    const float* p = a.part[side] + ((long long)lo * Rp + r) * C + c;
-    float s = 0.f;
-    if (c < C) {
+    if constexpr (RANKS == 1) {
+        const int r = blockIdx.y;
+        const float* p = a.part[side] + ((long long)lo * Rp + r) * C + c;
+        float s = 0.f;
+        if (c < C) {
 #pragma unroll 8
-        for (int i = q; i < n; i += 4) s += p[(long long)i * Rp * C];
+            for (int i = q; i < n; i += 4) s += p[(long long)i * Rp * C];
+        }
+        red[q][tx] = s;
+        __syncthreads();
+        if (q || c >= C) return;
+        s = red[0][tx] + red[1][tx] + red[2][tx] + red[3][tx];
+        if (side) a.out[1][((long long)e * C + c) * a.R + r] = (elem_t)s;
+        else a.out[0][((long long)e * a.R + r) * C + c] = (elem_t)s;
+    } else {
+        const int r0 = blockIdx.y * RANKS + q * (RANKS / 4);
+        const float* p = a.part[side] + ((long long)lo * Rp + r0) * C + c;
+        float s[RANKS / 4];
+#pragma unroll
+        for (int k = 0; k < RANKS / 4; ++k) s[k] = 0.f;
+        if (c < C) {
+#pragma unroll 2
+            for (int i = 0; i < n; ++i)
+#pragma unroll
+                for (int k = 0; k < RANKS / 4; ++k) s[k] += p[((long long)i * Rp + k) * C];      // (r0 + k < Rp: whole sixteens)
+        }
+        if (!side) {
+#pragma unroll
+            for (int k = 0; k < RANKS / 4; ++k)
+                if (c < C && r0 + k < a.R) a.out[0][((long long)e * a.R + r0 + k) * C + c] = (elem_t)s[k];
+            return;
+        }
+#pragma unroll
+        for (int k = 0; k < RANKS / 4; ++k) red[q * (RANKS / 4) + k][tx] = s[k];
+        __syncthreads();
+        const int cc = threadIdx.x >> 2, rk = (threadIdx.x & 3) * 4, r1 = blockIdx.y * RANKS + rk;
+        if (c0 + cc >= C) return;
+        elem_t* to = a.out[1] + ((long long)e * C + c0 + cc) * a.R + r1;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (r1 + k < a.R) to[k] = (elem_t)red[rk + k][cc];
     }
-    red[q][tx] = s;
-    __syncthreads();
-    if (q || c >= C) return;
-    s = red[0][tx] + red[1][tx] + red[2][tx] + red[3][tx];
-    if (side) a.out[1][((long long)e * C + c) * a.R + r] = (elem_t)s;
-    else a.out[0][((long long)e * a.R + r) * C + c] = (elem_t)s;
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -1151,7 +1189,10 @@ int DM_T(dm_linear_adapted_bwd_, )(const void* x, const void* dy, const void* w_
             default: hipLaunchKernelGGL(k_wgrad<128>, grid, dim3(256), 0, stream, g); break;
         }
         const int ba = da ? (K + 63) / 64 : 0, bb = db ? (N + 63) / 64 : 0;
-        hipLaunchKernelGGL(k_wgrad_join, dim3((unsigned)(ba + bb), (unsigned)R, (unsigned)E), dim3(256), 0, stream, g, ba, Rp);
+        // 16 ranks per workgroup where adapters have few items and that leaves two workgroups per CU
+        if (items <= 8LL * E && (long long)(ba + bb) * ((R + 15) / 16) * E >= 512)
+            hipLaunchKernelGGL(k_wgrad_join<16>, dim3((unsigned)(ba + bb), (unsigned)((R + 15) / 16), (unsigned)E), dim3(256), 0, stream, g, ba, Rp);
+        else hipLaunchKernelGGL(k_wgrad_join<1>, dim3((unsigned)(ba + bb), (unsigned)R, (unsigned)E), dim3(256), 0, stream, g, ba, Rp);
         DM_LAUNCH_CHECK();
     }
     return DM_OK;

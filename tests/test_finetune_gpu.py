@@ -117,6 +117,8 @@ ADAPTER_CASES = [
     ((150, 64), 64, 5, 40, [(7 * i) % 40 for i in range(150)], False, True, None),     # a row each, many adapters
     ((1, 640), 1280, 16, 9, [8], False, True, None),
     ((2, 1024, 64), 64, 16, 2, [-1, -1], False, True, None),                          # nobody has an adapter
+    ((300, 512), 1024, 33, 8, [7, 0, 1, 2, 9, 3, 4, 5, 6, 1], False, True, [0, 3, 60, 61, 61, 100, 170, 200, 230, 290, 299]),      # wide, few rows each
+    ((1500, 64), 64, 4, 1100, [(37 * i) % 1101 for i in range(1500)], False, True, None),      # more than 1024 adapters and requests
 ]
 
 

@@ -93,7 +93,8 @@ __device__ __forceinline__ int next_adapter(const int* aid, int cur) {
 
 // Tile of 16 RT rows; the four waves take 64-wide slices of K in turn, so a tile reads its x rows once (128-byte lines) and the rank
 // rows of A once from L2; a slice is requested before the last one is multiplied; the partial products meet in LDS.  One pass per adapter
-// that occurs in the tile.  Bound by the x read.
+// that occurs in the tile.  Bound by the x read, with few rows by latency (the search of the row's request, then K): 1851 ragged rows of 1024
+// halves, rank 32: 12 us.
 template <int RT, int NR>
 __global__ __launch_bounds__(256) void k_shrink(const elem_t* __restrict__ x, const elem_t* __restrict__ A, Rows rows, int K, int R, float scale,
                                                 elem_t* __restrict__ u, float* __restrict__ us, int* __restrict__ who) {
@@ -190,7 +191,7 @@ __global__ __launch_bounds__(256) void k_shrink(const elem_t* __restrict__ x, co
 
 // The same for many rows: tiles of 64 rows, x and the rank rows through a ring of LDS stages (buffer_load ... lds, whole 128-byte lines,
 // three stages in flight), a wave 16 rows.  Against the kernel above, whose fragments are gathered from 16 rows by every load: rank 64 of
-// [24576, 5120] 187 -> 70 us.
+// [24576, 5120] 187 -> 70 us (3.6 TB/s), rank 64 of [24576, 1280] 21 us.
 template <int NR>
 __global__ __launch_bounds__(256) void k_shrink_ring(const elem_t* __restrict__ x, const elem_t* __restrict__ A, Rows rows, int K, int R, float scale,
                                                      elem_t* __restrict__ u, float* __restrict__ us, int* __restrict__ who) {
@@ -285,7 +286,7 @@ __global__ __launch_bounds__(256) void k_shrink_ring(const elem_t* __restrict__ 
 }
 
 // One row per workgroup, one rank row per wave: requests of a few rows each, where a tile would hold many adapters.  Every row reads
-// its own adapter (R K 2 bytes).  f32out: plain fp32 [M][Rp] for the skinny product, else the pair format.
+// its own adapter (R K 2 bytes).  f32out: plain fp32 [M][Rp] for the skinny product, else the pair format.  16 rows of 1280, rank 16: 3.7 us.
 __global__ __launch_bounds__(1024) void k_shrink_rows(const elem_t* __restrict__ x, const elem_t* __restrict__ A, Rows rows, int K, int R, float scale,
                                                       elem_t* __restrict__ u, float* __restrict__ us, int* __restrict__ who, float* __restrict__ f32out) {
     __shared__ float row[kMaxRank];
@@ -335,7 +336,9 @@ struct ExpandArgs {
 // BM x BN x 64 tile, WM x WN waves, NST LDS stages filled by buffer_load ... lds (16 bytes per lane, range-checked: rows and
 // columns past the end read as zeros).  LDS rows are 128 bytes, the 16-byte chunks XOR-swizzled by (row >> 1) & 7 at the source address
 // and at the fragment read: conflict-free without padding.  The weights are the matrix instruction's A operand, so a lane holds one row
-// of y and four consecutive columns per register group: 16-byte stores after one exchange between the wave's halves.
+// of y and four consecutive columns per register group: 16-byte stores after one exchange between the wave's halves.  Bound by the matrix pipe (feeding
+// it: two workgroups per CU cover each other's waits): bf16, rank 64, [24576, 1280 -> 5120] 448 us = 720 TF/s of the plain product, [24576,
+// 5120 -> 1280] 370 us = 870; [24576, 640 -> 640] rank 16 with residual 38 us, 2.5 TB/s.
 template <int BM, int BN, int WM, int WN, int NST>
 __global__ __launch_bounds__(WM * WN * 64) void k_expand(ExpandArgs a) {
     [[maybe_unused]] constexpr int NW = WM * WN, ROWB = 128;
@@ -571,7 +574,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_expand(ExpandArgs a) {
 
 // M <= 32 rows (single tokens of a few requests): 16 columns per workgroup, eight waves split K and read W straight from memory (each
 // element is used once per 16 rows); the low-rank part is one fp32 dot product per output with the row's own adapter.  Bound by the
-// W read -- below a few MB by the launch.
+// W read -- below a few MB by the launch (1280 x 1280 for 16 rows: 5.5-6 us).
 template <int MT>
 __global__ __launch_bounds__(512) void k_expand_skinny(ExpandArgs a, const float* __restrict__ u) {
     __shared__ float part[8][MT * 16][17];
@@ -779,6 +782,7 @@ struct WgradArgs {
 // rows in stages of 64 through LDS (requested a stage ahead), both operands read with the transposing LDS read (the contraction index
 // is the row).  The rows of a stage sit at a pitch of 16 or 48 dwords past a multiple of 64: the four rows and two column groups of a
 // transposing read hit disjoint banks.  In half precision the pair is rescaled to the item's largest row scale while it is staged.
+// Bound by the read of X: [24576, 1280 + 5120] rank 64 in 78 us, 4 TB/s.
 template <int Rp>
 __global__ __launch_bounds__(256) void k_wgrad(WgradArgs a) {
     constexpr int UC = 2 * Rp, UF = UC / 32;                       // columns of the pair, 32-row fragments

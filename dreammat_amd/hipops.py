@@ -1881,7 +1881,7 @@ class _LinearAdapted(torch.autograd.Function):
 
 def linear_adapted_autograd(x, w, w_t, bias, lora_a, lora_b, ids, scale=1.0, residual=None, offsets=None):
     """linear_adapted, differentiable with respect to x, lora_a, lora_b and the residual; w and bias are frozen, w_t = w.t().contiguous()
-    [K, N] (prepared once by the caller, as for linear_frozen_autograd).  An adapter without rows gets a zero gradient."""
+    [K, N] (prepared once by the caller, as for linear_frozen_autograd).  An adapter without rows gets a zero gradient.  At most 60000 adapters."""
     if torch.is_grad_enabled() and (w.requires_grad or (bias is not None and bias.requires_grad)):
         raise ValueError("linear_adapted_autograd: the projection is frozen (w or bias requires a gradient)")
     if w_t.shape != w.shape[::-1] or w_t.dtype != w.dtype or w_t.device != w.device:
@@ -2052,7 +2052,8 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
         m <- momentum m + g;  u = g + momentum m (nesterov) or m;  p <- p (1 - lr weight_decay) - lr s orthogonalize(u)
 
     s = 0.2 sqrt(max(rows, cols)) for scale = "rms" (updates as large as Adam's, so its learning rate and decay carry over),
-    sqrt(max(1, rows / cols)) for "spectral", or the given number.  The matrices share their launches in groups of 16, largest first."""
+    sqrt(max(1, rows / cols)) for "spectral", or the given number.  The matrices share their launches in groups of 16, largest first.
+    No parameter or momentum buffer may share memory with another one or with a gradient."""
     params, grads, momenta = list(params), list(grads), list(momenta)
     if not len(params) == len(grads) == len(momenta):
         raise ValueError("muon_step: one gradient and one momentum buffer per parameter")

@@ -84,7 +84,7 @@ def controlnet_training_loss(vae, unet, controlnet, scheduler, pixel_values, con
 
 
 class MuonAdamW:
-    """Orthogonalised momentum steps (hipops.muon_step: the matrices of one shape share their launches) for every parameter that is a matrix --
+    """Orthogonalised momentum steps (hipops.muon_step: the matrices share their launches in groups) for every parameter that is a matrix --
     Linear weights, convolution weights as [Cout, Cin kh kw] -- and AdamW for the others (biases, norms).  The "rms" scale of the orthogonalised
     step is AdamW's update size, so both halves share one learning rate and one weight decay.  GPU only: the products have no CPU form."""
 

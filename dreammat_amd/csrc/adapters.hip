@@ -424,12 +424,14 @@ __global__ __launch_bounds__(WM * WN * 64) void k_expand(ExpandArgs a) {
     // one (NST - 1 ahead of the one being multiplied) and returns whether there was one.
     const int steps = (K + 63) / 64;
     int i_step = 0, i_stage = 0, i_e = kNone, i_c0 = 2 * Rp;
+    int only = 0x7fffffff;                                           // the tile's first adapter
+    bool mixed = false;                                              // whether its rows differ
     auto issue = [&]() __attribute__((always_inline)) {
         if (i_step < steps) issue_main(i_step, i_stage);
         else {
             if (i_c0 >= 2 * Rp) {
                 if (i_e == 0x7fffffff) return false;
-                i_e = next_adapter<BM>(aid, i_e);
+                i_e = mixed ? next_adapter<BM>(aid, i_e) : i_e == kNone ? only : 0x7fffffff;
                 i_c0 = 0;
                 if (i_e == 0x7fffffff) { i_c0 = 2 * Rp; return false; }
             }
@@ -451,13 +453,14 @@ __global__ __launch_bounds__(WM * WN * 64) void k_expand(ExpandArgs a) {
     }
     for (int t = tid; t < BN; t += NW * 64) bias_of[t] = a.bias && n0 + t < a.N ? (float)a.bias[n0 + t] : 0.f;
     plain = __syncthreads_and(plain);
+    int others = 0;
+    for (int t = lane; t < mrows; t += 64) others |= aid[t] != aid[0];
+    mixed = __any(others);
+    only = mixed ? next_adapter<BM>(aid, kNone) : aid[0] == kNone ? 0x7fffffff : __builtin_amdgcn_readfirstlane(aid[0]);
 #pragma unroll
     for (int q = 1; q < NST - 1; ++q) ahead += issue();
     // A tile of one adapter without row scales (nearly all: a request is longer than a tile): its low-rank columns are K steps like others
-    const int only = next_adapter<BM>(aid, kNone);
-    int others = 0;
-    for (int t = lane; t < mrows; t += 64) others |= aid[t] != only;
-    const bool uniform = plain && only != 0x7fffffff && !__any(others);
+    const bool uniform = plain && only != 0x7fffffff && !mixed;
     f32x16 acc[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; ++i)

@@ -358,9 +358,10 @@ __global__ __launch_bounds__(WM * WN * 64) void k_expand(ExpandArgs a) {
     const int per = (a.tiles + 7) / 8, id = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
     if ((int)(blockIdx.x >> 3) >= per || id >= a.tiles) return;
     constexpr int BAND = 8;
-    const int band = id / (BAND * a.n_nt), in_band = id - band * BAND * a.n_nt, height = min(BAND, a.n_mt - band * BAND);
-    const long long m0 = (long long)(band * BAND + in_band % height) * BM;
-    const int n0 = in_band / height * BN;
+    const int band = (int)((unsigned)id / (unsigned)(BAND * a.n_nt)), in_band = id - band * BAND * a.n_nt, height = min(BAND, a.n_mt - band * BAND);
+    const int column = height == BAND ? in_band / BAND : (int)((unsigned)in_band / (unsigned)height);      // (a division by a number in a register: 0.1 us)
+    const long long m0 = (long long)(band * BAND + in_band - column * height) * BM;
+    const int n0 = column * BN;
     const int mrows = (int)min((long long)BM, a.rows.M - m0), nrows = min(BN, a.N - n0);
     const int K = a.K, Rp = rank_pad(a.R);
 
@@ -443,24 +444,32 @@ __global__ __launch_bounds__(WM * WN * 64) void k_expand(ExpandArgs a) {
         return true;
     };
     issue();                                                         // (the first step of K)
-    int ahead = 1, plain = 1;
-    for (int t = tid; t < BM; t += NW * 64) {
-        const int e = t < mrows ? a.who[m0 + t] : kNone;
-        const float scale = t < mrows ? a.us[m0 + t] : 1.f;
-        aid[t] = e;
-        scale_of[t] = e != kNone ? scale : 1.f;
-        if (scale_of[t] != 1.f) plain = 0;
+    int ahead = 1;
+    static_assert(BM <= NW * 64 && BN <= NW * 64, "a row and a column per thread");
+    if (tid < BM) {
+        const int e = tid < mrows ? a.who[m0 + tid] : kNone;
+        aid[tid] = e;
+#if defined(DM_F16)
+        const float scale = tid < mrows ? a.us[m0 + tid] : 1.f;
+        scale_of[tid] = e != kNone ? scale : 1.f;
+#endif
     }
-    for (int t = tid; t < BN; t += NW * 64) bias_of[t] = a.bias && n0 + t < a.N ? (float)a.bias[n0 + t] : 0.f;
-    plain = __syncthreads_and(plain);
-    int others = 0;
-    for (int t = lane; t < mrows; t += 64) others |= aid[t] != aid[0];
+    if (tid < BN) bias_of[tid] = a.bias && tid < nrows ? (float)a.bias[n0 + tid] : 0.f;
+    __syncthreads();
+    int others = 0, scaled = 0;
+#pragma unroll
+    for (int t = lane; t < BM; t += 64) {
+        others |= t < mrows && aid[t] != aid[0];
+#if defined(DM_F16)
+        scaled |= scale_of[t] != 1.f;
+#endif
+    }
     mixed = __any(others);
     only = mixed ? next_adapter<BM>(aid, kNone) : aid[0] == kNone ? 0x7fffffff : __builtin_amdgcn_readfirstlane(aid[0]);
 #pragma unroll
     for (int q = 1; q < NST - 1; ++q) ahead += issue();
     // A tile of one adapter without row scales (nearly all: a request is longer than a tile): its low-rank columns are K steps like others
-    const bool uniform = plain && only != 0x7fffffff && !mixed;
+    const bool uniform = only != 0x7fffffff && !mixed && !__any(scaled);
     f32x16 acc[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -510,7 +519,11 @@ __global__ __launch_bounds__(WM * WN * 64) void k_expand(ExpandArgs a) {
         for (int i = 0; i < MT; ++i) {
             const int row = TM * wm + 32 * i + l31;
             const bool mine = aid[row] == e;
+#if defined(DM_F16)
             const float scale = scale_of[row];
+#else
+            constexpr float scale = 1.f;                             // (pow2_scale)
+#endif
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 f32x16 t;

@@ -337,8 +337,9 @@ struct ExpandArgs {
 // columns past the end read as zeros).  LDS rows are 128 bytes, the 16-byte chunks XOR-swizzled by (row >> 1) & 7 at the source address
 // and at the fragment read: conflict-free without padding.  The weights are the matrix instruction's A operand, so a lane holds one row
 // of y and four consecutive columns per register group: 16-byte stores after one exchange between the wave's halves.  Bound by the matrix pipe (feeding
-// it: two workgroups per CU cover each other's waits): bf16, rank 64, [24576, 1280 -> 5120] 448 us = 720 TF/s of the plain product, [24576,
-// 5120 -> 1280] 370 us = 870; [24576, 640 -> 640] rank 16 with residual 38 us, 2.5 TB/s.
+// it: two workgroups per CU cover each other's waits): bf16, rank 64, [24576, 1280 -> 5120] 435 us = 740 TF/s of the plain product, [24576,
+// 5120 -> 1280] 375 us = 860; [24576, 640 -> 640] rank 16 with residual 37 us, 2.5 TB/s.  With a short K by the latencies of a tile (its
+// adapters, two loads, the store): [24576, 64 -> 4096] rank 16 in 67 us.
 template <int BM, int BN, int WM, int WN, int NST>
 __global__ __launch_bounds__(WM * WN * 64) void k_expand(ExpandArgs a) {
     [[maybe_unused]] constexpr int NW = WM * WN, ROWB = 128;
@@ -467,7 +468,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_expand(ExpandArgs a) {
     mixed = __any(others);
     only = mixed ? next_adapter<BM>(aid, kNone) : aid[0] == kNone ? 0x7fffffff : __builtin_amdgcn_readfirstlane(aid[0]);
 #pragma unroll
-    for (int q = 1; q < NST - 1; ++q) ahead += issue();
+    for (int q = 1; q < NST; ++q) ahead += issue();                  // (at first the whole ring is free)
     // A tile of one adapter without row scales (nearly all: a request is longer than a tile): its low-rank columns are K steps like others
     const bool uniform = only != 0x7fffffff && !mixed && !__any(scaled);
     f32x16 acc[MT][NT];
@@ -482,18 +483,20 @@ __global__ __launch_bounds__(WM * WN * 64) void k_expand(ExpandArgs a) {
         return *reinterpret_cast<const elem8*>(base + row * ROWB + (((2 * kk + hi) ^ ((row >> 1) & 7)) << 4));
     };
     int stage = 0;
-    // waits until the step to multiply has landed (at most the younger NST - 2 steps' pieces stay in flight), then requests another one
-    auto advance = [&]() __attribute__((always_inline)) {
-        if (NST > 2 && ahead == NST - 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 2) * (AP + BP)) : "memory");
+    // waits until the step to multiply has landed (the younger steps' pieces stay in flight), then requests another one into the stage that
+    // all waves have read
+    auto advance = [&](bool first) __attribute__((always_inline)) {
+        if (ahead == NST) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 1) * (AP + BP)) : "memory");
+        else if (NST > 2 && ahead == NST - 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 2) * (AP + BP)) : "memory");
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         --ahead;
-        ahead += issue();
+        if (!first) ahead += issue();
     };
     const int low = (2 * Rp + 63) / 64, last = uniform ? steps + low : steps;
     for (int s = 0; s < last; ++s) {
-        advance();
+        advance(s == 0);
         const char* ab = smem + stage * STAGE;
         const char* bb = ab + A_BYTES;
 #pragma unroll
@@ -512,7 +515,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_expand(ExpandArgs a) {
     }
     int e = uniform ? 0x7fffffff : only, c0 = 0;
     while (e != 0x7fffffff) {
-        advance();
+        advance(false);
         const char* ab = smem + stage * STAGE;
         const char* bb = ab + A_BYTES;
 #pragma unroll

@@ -12,22 +12,18 @@
 // storage) leave 1e-2 of error in the result and 11 bits (half) 1e-3, 1e-2 where a few directions dominate the matrix.  Numbers are
 // therefore kept as a PAIR of halves, value + rest (22 bits; scaled by 2^13, so that neither leaves half's range: |X| <= 1.2, |S| <=
 // 1.5, |P + a| <= 3.5), and a product is value value + value rest + rest value with fp32 sums: the result agrees with fp32 arithmetic to its
-// own rounding (1.7e-6 against 1.7e-6 of the fp32 form on a 1024^2 Gaussian).  For bf16 input the last two iterations, whose
-// errors are hardly amplified any more, take (and are given) the values only: 1e-3 of error under the 1.7e-3 of the rounding to bf16.
+// own rounding (1.7e-6 against 1.7e-6 of the fp32 form on a 1024^2 Gaussian), and a 16-bit result is off by its one rounding.  Values alone in
+// the last two iterations would save a seventh of the time (16 x [1280, 1280]: 1859 against 2159 us) and leave 1e-3 of error, as much again as
+// the rounding to bf16 and far more than an fp32 parameter's: not taken for any type.
 // (Taking the polynomials of S = X X^T alone and multiplying X0 once saves half the products of a wide matrix, but S holds squared singular
 // values: on the gradients of a small ControlNet, which a few directions dominate, the result was 1e-3 to 1e-2 off where this form is 3e-5.)
-// Pairs are stored as 128-byte blocks, 32 values then their 32 rests: a K step of the paired product loads the same lines as a K
-// step of 64 plain halves.
+// Pairs are stored as 128-byte blocks, 32 values then their 32 rests: a K step loads whole lines.
 #include <algorithm>
-#include <type_traits>
+#include <new>
+#include <vector>
 
 #include "dm_common.h"
 #include "dm_elem.h"
-
-#include <algorithm>
-#include <new>
-#include <type_traits>
-#include <vector>
 
 namespace {
 
@@ -188,8 +184,8 @@ __device__ __forceinline__ int tile_at(int row, int blk, int chunk) {
 
 // The products of the iteration over pair matrices:
 //   GRAM  S = X X^T
-//   POLY  P = b S + c S S^T (pairs: + a on the diagonal)
-//   STEP  X' = a X + P X (pairs: P X), from one copy of X into the other
+//   POLY  P = a + b S + c S S^T (a on the diagonal, so that X is not read again for a X)
+//   STEP  X' = P X, from one copy of X into the other
 //   LAST  the same, into the parameter or the output
 enum { NS_GRAM = 0, NS_POLY = 1, NS_STEP = 2, NS_LAST = 3 };
 
@@ -203,7 +199,7 @@ struct Class {
 struct Launch {
     Class c[kGroup];
     float* part;             // fp32 partial sums [share][T * T]
-    int classes, in, rests;  // which copy of X is read; whether the result's readers take its rests
+    int classes, in;         // which copy of X is read
 };
 
 // block -> class, unit.  Block b runs on XCD b % 8: every XCD gets an eighth of each class's units, neighbours of a matrix together; the odd
@@ -233,28 +229,26 @@ __device__ __forceinline__ void tile_of(const Class& c, int rem, int& ti, int& t
     }
 }
 
-// Tile T x T, two rows of WJ waves of T/2 x T/WJ.  K goes in steps of 32 pairs (PAIR: three products) or the values of 64, through a ring of
+// Tile T x T, two rows of WJ waves of T/2 x T/WJ.  K goes in steps of 32 pairs (three products), through a ring of
 // NST LDS stages filled by buffer_load ... lds, NST - 1 of them in flight.  A stage holds T rows of the left operand, 128 bytes of K each
-// (chunks XOR-swizzled by (row >> 1) & 7), and of the right one, S or X^T, the same -- or, in P X, the 32 or 64 rows of X along K,
+// (chunks XOR-swizzled by (row >> 1) & 7), and of the right one, S or X^T, the same -- or, in P X, the 32 rows of X along K,
 // T columns each, which the transposing LDS read turns (chunks XOR-swizzled by 4 (row & 3): its four rows meet different banks).
 // GRAM and POLY are symmetric: tiles i >= j, stored twice.
-// The epilogue goes through LDS: the tile of S or X arrives as whole lines, every lane replaces its own entries, and whole lines leave (GRAM,
+// The epilogue goes through LDS: the tile of S arrives as whole lines (POLY), every lane replaces its own entries, and whole lines leave (GRAM,
 // POLY: in both orientations, the transposed one by the transposing read); a 256 tile does that half by half.  A share of a split
 // contraction leaves its fp32 sums in l.part instead, for k_ns_join.
 // Bound by the matrix pipe, of a 256 tile by the rounds and by the epilogue, which one workgroup per CU does not overlap.  16 x [1280, 1280],
-// 256 tiles, in TF/s of half products: pairs X X^T 116 us = 1040, S S^T 127 us = 950, P X 206 us = 980 (1.56 tiles per CU in two rounds);
-// values 65, 78 and 138 us.  One [320, 320]: 7 to 8 us each, all latency.
-template <int KIND, int T, int NST, bool PAIR, typename OT>
+// 256 tiles, in TF/s of half products: X X^T 116 us = 1040, S S^T 127 us = 950, P X 206 us = 980 (1.56 tiles per CU in two rounds).
+// One [320, 320]: 7 to 8 us each, all latency.
+template <int KIND, int T, int NST, typename OT>
 __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
     [[maybe_unused]] constexpr int NT = threads_of(T), NW = NT / 64, WJ = NW / 2, ROWB = 128, STAGE = 2 * T * ROWB, TI = T / 2, TJ = T / WJ, FI = TI / 32, FJ = TJ / 32,
                                    PIECES = T / 8 / NW, H = T == 256 ? 2 : 1, TR = T / H;       // TR rows per epilogue pass
-    [[maybe_unused]] constexpr bool SYM = KIND <= NS_POLY, LAST = KIND == NS_LAST;
-    // pairs: the a of a X sits on the diagonal of P, so X is not read again; values alone would round it to 11 bits
-    [[maybe_unused]] constexpr bool DIAG = KIND == NS_POLY && PAIR, SRC = KIND == NS_POLY || (!SYM && !PAIR);
+    [[maybe_unused]] constexpr bool SYM = KIND <= NS_POLY, LAST = KIND == NS_LAST, POLY = KIND == NS_POLY;
     // the result in units of 2^13 (LAST: 1) from products in units of 2^26
-    [[maybe_unused]] constexpr float ACC = LAST ? kInv * kInv : KIND == NS_POLY ? kC * kInv : kInv, OLD = LAST ? kA * kInv : KIND == NS_POLY ? kB : kA;
-    // A 64 tile has LDS to spare for its source tile: requested before the products instead of waited for behind them
-    [[maybe_unused]] constexpr bool EARLY = SRC && T == 64;
+    [[maybe_unused]] constexpr float ACC = LAST ? kInv * kInv : POLY ? kC * kInv : kInv;
+    // A 64 tile has LDS to spare for its tile of S: requested before the products instead of waited for behind them
+    [[maybe_unused]] constexpr bool EARLY = POLY && T == 64;
     extern __shared__ __attribute__((aligned(16))) char smem[];      // EARLY: NST * STAGE + 4 TR T, else the larger of the two
 #if defined(__HIP_DEVICE_COMPILE__)
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, hi = lane >> 5, l31 = lane & 31;
@@ -271,19 +265,18 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
     const int mp = t.mp(), np = t.np();
     const int i0 = ti * T, j0 = tj * T;
     const int kw = KIND == NS_GRAM ? np : mp, ow = SYM ? mp : np, oh = mp;      // contraction; the result's columns and rows
-    // rows of X of a stage (P X), their bytes and 16-byte chunks; the swizzle of row's chunks (64 values of a row are half the banks wide)
-    [[maybe_unused]] constexpr int KR = PAIR ? 32 : 64, RB = PAIR ? 4 * T : 2 * T, CPR = RB / 16;
-    [[maybe_unused]] auto turn = [](int row) __attribute__((always_inline)) { return CPR == 8 ? (row & 2) << 1 : (row & 3) << 2; };
+    // bytes of a row of X in a stage (P X) and its 16-byte chunks; the swizzle of row's chunks
+    [[maybe_unused]] constexpr int RB = 4 * T, CPR = RB / 16;
+    [[maybe_unused]] auto turn = [](int row) __attribute__((always_inline)) { return (row & 3) << 2; };
     char* const pane = smem + (EARLY ? NST * STAGE : 0);
-    auto source = [&](int r0) __attribute__((always_inline)) {         // rows r0 .. r0 + TR of the source tile
+    [[maybe_unused]] auto source = [&](int r0) __attribute__((always_inline)) {         // rows r0 .. r0 + TR of the tile of S
         constexpr int P = TR * T / 256 / NW;                           // 1 KB = 8 blocks per wave and request
-        const _Float16* src = KIND == NS_POLY ? t.s() : t.x(l.in);
-        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(src + (long long)r0 * 2 * ow), 0, min(TR, oh - r0) * ow * 4, 0x00020000);
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(t.s() + (long long)r0 * 2 * ow), 0, min(TR, oh - r0) * ow * 4, 0x00020000);
 #pragma unroll
         for (int p = 0; p < P; ++p) {
             const int q = (wave * P + p) * 8 + (lane >> 3), row = q / (T / 32), blk = (q % (T / 32)) ^ ((row >> 3) & 1);
             const int chunk = (lane & 7) ^ (row & 7);
-            const unsigned o = PAIR || chunk < 4 ? (unsigned)row * (unsigned)ow * 4u + (unsigned)((j0 / 32 + blk) * 128 + (chunk << 4)) : 0x80000000u;
+            const unsigned o = (unsigned)row * (unsigned)ow * 4u + (unsigned)((j0 / 32 + blk) * 128 + (chunk << 4));
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(pane + (wave * P + p) * 1024), 16, (int)o, 0, 0, 0);
         }
     };
@@ -298,28 +291,27 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
             const int row = wave * (T / NW) + 8 * p + (lane >> 3);
-            const int chunk = (lane & 7) ^ ((row >> 1) & 7);       // (values only: chunks 4 .. 7 are the next block's values)
-            off[p] = (unsigned)row * (unsigned)kw * 4u + (unsigned)(PAIR ? chunk * 16 : (chunk >> 2) * 128 + (chunk & 3) * 16);
+            off[p] = (unsigned)row * (unsigned)kw * 4u + (unsigned)(((lane & 7) ^ ((row >> 1) & 7)) * 16);
         }
         [[maybe_unused]] unsigned xoff[PIECES];                    // P X: rows along K of X, columns past it out of range
         if constexpr (!SYM) {
 #pragma unroll
             for (int p = 0; p < PIECES; ++p) {
-                const int q = (wave * PIECES + p) * 64 + lane, row = q / CPR, chunk = (q % CPR) ^ turn(row), blk = chunk >> (PAIR ? 3 : 2);
-                xoff[p] = j0 + 32 * blk < ow ? (unsigned)row * (unsigned)ow * 4u + (unsigned)((j0 / 32 + blk) * 128 + (chunk & (PAIR ? 7 : 3)) * 16) : 0x80000000u;
+                const int q = (wave * PIECES + p) * 64 + lane, row = q / CPR, chunk = (q % CPR) ^ turn(row), blk = chunk >> 3;
+                xoff[p] = j0 + 32 * blk < ow ? (unsigned)row * (unsigned)ow * 4u + (unsigned)((j0 / 32 + blk) * 128 + (chunk & 7) * 16) : 0x80000000u;
             }
         }
         auto issue = [&](int s, int stage) __attribute__((always_inline)) {
             char* base = smem + stage * STAGE;
 #pragma unroll
             for (int p = 0; p < PIECES; ++p)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(ars, (__attribute__((address_space(3))) void*)(base + (wave * (T / NW) + 8 * p) * ROWB), 16, (int)off[p], s * (PAIR ? 128 : 256), 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(ars, (__attribute__((address_space(3))) void*)(base + (wave * (T / NW) + 8 * p) * ROWB), 16, (int)off[p], s * 128, 0, 0);
             if constexpr (SYM) {
 #pragma unroll
                 for (int p = 0; p < PIECES; ++p)
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(brs, (__attribute__((address_space(3))) void*)(base + T * ROWB + (wave * (T / NW) + 8 * p) * ROWB), 16, (int)off[p], s * (PAIR ? 128 : 256), 0, 0);
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(brs, (__attribute__((address_space(3))) void*)(base + T * ROWB + (wave * (T / NW) + 8 * p) * ROWB), 16, (int)off[p], s * 128, 0, 0);
             } else {
-                const __amdgpu_buffer_rsrc_t xrs = __builtin_amdgcn_make_buffer_rsrc((void*)(t.x(l.in) + (long long)s * KR * 2 * ow), 0, KR * ow * 4, 0x00020000);
+                const __amdgpu_buffer_rsrc_t xrs = __builtin_amdgcn_make_buffer_rsrc((void*)(t.x(l.in) + (long long)s * 64 * ow), 0, 32 * ow * 4, 0x00020000);
 #pragma unroll
                 for (int p = 0; p < PIECES; ++p)
                     __builtin_amdgcn_raw_ptr_buffer_load_lds(xrs, (__attribute__((address_space(3))) void*)(base + T * ROWB + (wave * PIECES + p) * 1024), 16, (int)xoff[p], 0, 0, 0);
@@ -342,56 +334,46 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
             for (int j = 0; j < FJ; ++j)
 #pragma unroll
                 for (int part = 0; part < 2; ++part) {
-                    const int blk = TJ / 32 * wj + j, chunk = (PAIR ? 8 * blk + 4 * part : 4 * blk) + (col >> 3);
+                    const int chunk = 8 * (TJ / 32 * wj + j) + 4 * part + (col >> 3);
                     at[j][part] = T * ROWB + first * RB + ((chunk ^ turn(first)) << 4) + ((col & 4) << 1);
                 }
         }
         // All of a stage's fragments of X before the next stage is requested: the compiler lets a transposing read wait for every request in flight,
         // which costs nothing while there is none.  The deeper ring of 64 tiles always has some: there the reads bring their own wait.
-        [[maybe_unused]] half8 xt[PAIR ? 2 : 4][FJ][PAIR ? 2 : 1];
+        [[maybe_unused]] half8 xt[2][FJ][2];
         auto turned = [&](const char* base) __attribute__((always_inline)) {
-            constexpr int KK = PAIR ? 2 : 4, PARTS = PAIR ? 2 : 1;
-            elem4 q[KK][FJ][PARTS][2];
+            elem4 q[2][FJ][2][2];
             if constexpr (T == 64) {
-                const unsigned p0 = (unsigned)(uintptr_t)(base + at[0][0]), p1 = (unsigned)(uintptr_t)(base + at[0][PARTS - 1]);
-                if constexpr (PAIR)
-                    asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%10\n\t"
-                                 "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%10\n\t"
-                                 "ds_read_b64_tr_b16 %4, %8 offset:%11\n\tds_read_b64_tr_b16 %5, %8 offset:%12\n\t"
-                                 "ds_read_b64_tr_b16 %6, %9 offset:%11\n\tds_read_b64_tr_b16 %7, %9 offset:%12\n\ts_waitcnt lgkmcnt(0)"
-                                 : "=&v"(q[0][0][0][0]), "=&v"(q[0][0][0][1]), "=&v"(q[0][0][1][0]), "=&v"(q[0][0][1][1]), "=&v"(q[1][0][0][0]),
-                                   "=&v"(q[1][0][0][1]), "=&v"(q[1][0][1][0]), "=&v"(q[1][0][1][1])
-                                 : "v"(p0), "v"(p1), "n"(4 * RB), "n"(16 * RB), "n"(20 * RB) : "memory");
-                else
-                    asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%9\n\t"
-                                 "ds_read_b64_tr_b16 %2, %8 offset:%10\n\tds_read_b64_tr_b16 %3, %8 offset:%11\n\t"
-                                 "ds_read_b64_tr_b16 %4, %8 offset:%12\n\tds_read_b64_tr_b16 %5, %8 offset:%13\n\t"
-                                 "ds_read_b64_tr_b16 %6, %8 offset:%14\n\tds_read_b64_tr_b16 %7, %8 offset:%15\n\ts_waitcnt lgkmcnt(0)"
-                                 : "=&v"(q[0][0][0][0]), "=&v"(q[0][0][0][1]), "=&v"(q[1][0][0][0]), "=&v"(q[1][0][0][1]), "=&v"(q[KK - 2][0][0][0]),
-                                   "=&v"(q[KK - 2][0][0][1]), "=&v"(q[KK - 1][0][0][0]), "=&v"(q[KK - 1][0][0][1])
-                                 : "v"(p0), "n"(4 * RB), "n"(16 * RB), "n"(20 * RB), "n"(32 * RB), "n"(36 * RB), "n"(48 * RB), "n"(52 * RB) : "memory");
+                const unsigned p0 = (unsigned)(uintptr_t)(base + at[0][0]), p1 = (unsigned)(uintptr_t)(base + at[0][1]);
+                asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%10\n\t"
+                             "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%10\n\t"
+                             "ds_read_b64_tr_b16 %4, %8 offset:%11\n\tds_read_b64_tr_b16 %5, %8 offset:%12\n\t"
+                             "ds_read_b64_tr_b16 %6, %9 offset:%11\n\tds_read_b64_tr_b16 %7, %9 offset:%12\n\ts_waitcnt lgkmcnt(0)"
+                             : "=&v"(q[0][0][0][0]), "=&v"(q[0][0][0][1]), "=&v"(q[0][0][1][0]), "=&v"(q[0][0][1][1]), "=&v"(q[1][0][0][0]),
+                               "=&v"(q[1][0][0][1]), "=&v"(q[1][0][1][0]), "=&v"(q[1][0][1][1])
+                             : "v"(p0), "v"(p1), "n"(4 * RB), "n"(16 * RB), "n"(20 * RB) : "memory");
             } else {
 #pragma unroll
-                for (int kk = 0; kk < KK; ++kk)
+                for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
                     for (int j = 0; j < FJ; ++j)
 #pragma unroll
-                        for (int part = 0; part < PARTS; ++part) {
+                        for (int part = 0; part < 2; ++part) {
                             q[kk][j][part][0] = dm_ds_read_tr16_b64(base + at[j][part] + 16 * kk * RB);
                             q[kk][j][part][1] = dm_ds_read_tr16_b64(base + at[j][part] + (16 * kk + 4) * RB);
                         }
             }
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk)
+            for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
                 for (int j = 0; j < FJ; ++j)
 #pragma unroll
-                    for (int part = 0; part < PARTS; ++part) {
+                    for (int part = 0; part < 2; ++part) {
                         const elem4 u = q[kk][j][part][0], v = q[kk][j][part][1];
                         xt[kk][j][part] = __builtin_bit_cast(half8, elem8{u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]});
                     }
         };
-        const int all = kw / (PAIR ? 32 : 64);
+        const int all = kw / 32;
         const int s_lo = (int)((long long)all * z / splits), s_hi = (int)((long long)all * (z + 1) / splits);
 #pragma unroll
         for (int q = 0; q < NST - 1; ++q)
@@ -409,23 +391,23 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
             if (s + NST - 1 < s_hi) issue(s + NST - 1, fill);
             const char* bb = ab + T * ROWB;
 #pragma unroll
-            for (int kk = 0; kk < (PAIR ? 2 : 4); ++kk) {
+            for (int kk = 0; kk < 2; ++kk) {
                 half8 ah[FI], al[FI], bh[FJ], bl[FJ];
 #pragma unroll
                 for (int i = 0; i < FI; ++i) {
                     const int row = TI * wi + 32 * i + l31;
                     ah[i] = frag(ab, row, 2 * kk + hi);
-                    if constexpr (PAIR) al[i] = frag(ab, row, 4 + 2 * kk + hi);
+                    al[i] = frag(ab, row, 4 + 2 * kk + hi);
                 }
 #pragma unroll
                 for (int j = 0; j < FJ; ++j) {
                     if constexpr (SYM) {
                         const int row = TJ * wj + 32 * j + l31;
                         bh[j] = frag(bb, row, 2 * kk + hi);
-                        if constexpr (PAIR) bl[j] = frag(bb, row, 4 + 2 * kk + hi);
+                        bl[j] = frag(bb, row, 4 + 2 * kk + hi);
                     } else {
                         bh[j] = xt[kk][j][0];
-                        if constexpr (PAIR) bl[j] = xt[kk][j][1];
+                        bl[j] = xt[kk][j][1];
                     }
                 }
                 // B as the matrix instruction's first operand: a lane holds one row i and four consecutive columns j per group
@@ -433,10 +415,8 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
                 for (int i = 0; i < FI; ++i)
 #pragma unroll
                     for (int j = 0; j < FJ; ++j) {
-                        if constexpr (PAIR) {
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bl[j], ah[i], acc[i][j], 0, 0, 0);
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bh[j], al[i], acc[i][j], 0, 0, 0);
-                        }
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bl[j], ah[i], acc[i][j], 0, 0, 0);
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bh[j], al[i], acc[i][j], 0, 0, 0);
                         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bh[j], ah[i], acc[i][j], 0, 0, 0);
                     }
             }
@@ -462,7 +442,7 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
         const int r0 = i0 + h * TR;                                    // first row of this pass
         if (h && r0 >= oh) break;
         __syncthreads();                                               // every wave has read its last fragments (its share of the last pass)
-        if constexpr (SRC && !EARLY) {
+        if constexpr (POLY && !EARLY) {
             source(r0);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
@@ -480,14 +460,11 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
                         float v[4];
 #pragma unroll
                         for (int r = 0; r < 4; ++r) v[r] = acc[fi][fj][4 * q + r] * ACC;
-                        if constexpr (SRC) {
+                        if constexpr (POLY) {
                             const half4 hv = *vp, lv = *rp;
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) v[r] += OLD * ((float)hv[r] + (float)lv[r]);
-                            if constexpr (DIAG) {
-#pragma unroll
-                                for (int r = 0; r < 4; ++r) v[r] += r0 + row == j0 + 32 * blk + 8 * q + 4 * hi + r ? kA * kScale : 0.f;
-                            }
+                            for (int r = 0; r < 4; ++r)
+                                v[r] += kB * ((float)hv[r] + (float)lv[r]) + (r0 + row == j0 + 32 * blk + 8 * q + 4 * hi + r ? kA * kScale : 0.f);
                         }
                         if constexpr (LAST) {                          // fp32 in the pair's place: columns 0, 1 | 2, 3 of the four
                             *reinterpret_cast<float2*>(vp) = make_float2(v[0], v[1]);
@@ -563,18 +540,17 @@ __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {
             }
         } else {
             _Float16* D = KIND == NS_GRAM ? t.s() : KIND == NS_POLY ? t.pm() : t.x(l.in ^ 1);
-            const bool rests = KIND == NS_STEP ? l.rests : PAIR;
 #pragma unroll 4
             for (int q = tid; q < TR * T / 4; q += NT) {               // 16-byte chunks, whole rows of blocks
                 const int chunk = q & 7, blk = (q >> 3) % (T / 32), row = (q >> 3) / (T / 32);
-                if (r0 + row < oh && j0 + 32 * blk < ow && (chunk < 4 || rests))
+                if (r0 + row < oh && j0 + 32 * blk < ow)
                     *reinterpret_cast<u32x4*>(D + (long long)(r0 + row) * 2 * ow + (j0 / 32 + blk) * 64 + chunk * 8) =
                         *reinterpret_cast<const u32x4*>(pane + tile_at<T>(row, blk, chunk));
             }
             if (SYM && ti != tj) {                                     // the other half: rows j, blocks of 32 i
                 const int l15 = lane & 15, grp = lane >> 4;
-                for (int u = wave; u < (T / 16) * (TR / 32) * (1 + rests); u += NW) {
-                    const int part = rests ? u & 1 : 0, v = u >> (int)rests, ib = v % (TR / 32), c0 = v / (TR / 32) * 16;
+                for (int u = wave; u < (T / 16) * (TR / 32) * 2; u += NW) {
+                    const int part = u & 1, v = u >> 1, ib = v % (TR / 32), c0 = v / (TR / 32) * 16;
                     const int row = 32 * ib + 8 * grp + (l15 >> 2), cc = (c0 & 31) + 4 * (l15 & 3);
                     const char* p0 = pane + tile_at<T>(row, c0 >> 5, (cc >> 3) + 4 * part) + ((cc & 4) << 1);
                     const char* p1 = pane + tile_at<T>(row + 4, c0 >> 5, (cc >> 3) + 4 * part) + ((cc & 4) << 1);
@@ -641,7 +617,7 @@ __global__ __launch_bounds__(256) void k_ns_join(NsArgs a, Launch l) {
 }
 
 // A launch of one kind over a group, and what it should take, in K steps of 32 pairs on one CU with a 256 tile (2.8 us).
-// Measured on 1280^2, paired: a 256 tile needs a third of a 128 tile's LDS and request traffic per product; 128 tiles run two per CU and a
+// Measured on 1280^2: a 256 tile needs a third of a 128 tile's LDS and request traffic per product; 128 tiles run two per CU and a
 // round of 512 costs 1.15, half a round 0.6; 64 tiles 0.3 per 512, 0.18 where a CU gets one (then with a ring as deep as LDS allows: its
 // loads have nothing else to hide behind).  Rounds: of equal units, whole ones; of unequal ones (longest first) the longest, or a tenth more
 // than their mean over the CUs.
@@ -715,16 +691,15 @@ Plan plan(const Mat* t, int count, int kind) {
     return best;
 }
 
-template <int KIND, int T, int NST, bool PAIR, typename OT>
-int launch_tile(const NsArgs& a, const Plan& p, int in, bool rests, float* part, hipStream_t stream) {
-    constexpr int RING = NST * 2 * T * 128, TILE = T == 256 ? 2 * T * T : 4 * T * T, LDS = T == 64 && (KIND == NS_POLY || (KIND >= NS_STEP && !PAIR)) ? RING + TILE : std::max(RING, TILE);
+template <int KIND, int T, int NST, typename OT>
+int launch_tile(const NsArgs& a, const Plan& p, int in, float* part, hipStream_t stream) {
+    constexpr int RING = NST * 2 * T * 128, TILE = T == 256 ? 2 * T * T : 4 * T * T, LDS = T == 64 && KIND == NS_POLY ? RING + TILE : std::max(RING, TILE);
     static unsigned long long devices = 0;
-    DM_HIP(dm_dynamic_lds(reinterpret_cast<const void*>(&k_ns_gemm<KIND, T, NST, PAIR, OT>), LDS, devices));
+    DM_HIP(dm_dynamic_lds(reinterpret_cast<const void*>(&k_ns_gemm<KIND, T, NST, OT>), LDS, devices));
     Launch l = p.l;
     l.in = in;
-    l.rests = rests;
     l.part = part;
-    hipLaunchKernelGGL((k_ns_gemm<KIND, T, NST, PAIR, OT>), dim3(p.blocks), dim3(threads_of(T)), LDS, stream, a, l);
+    hipLaunchKernelGGL((k_ns_gemm<KIND, T, NST, OT>), dim3(p.blocks), dim3(threads_of(T)), LDS, stream, a, l);
     DM_LAUNCH_CHECK();
     if constexpr (KIND == NS_GRAM) {
         if (!p.shares) return DM_OK;
@@ -742,12 +717,12 @@ int launch_tile(const NsArgs& a, const Plan& p, int in, bool rests, float* part,
     return DM_OK;
 }
 
-template <int KIND, bool PAIR, typename OT>
-int launch_gemm(const NsArgs& a, const Plan& p, int in, bool rests, float* part, hipStream_t stream) {
-    if (p.tile == 256) return launch_tile<KIND, 256, 2, PAIR, OT>(a, p, in, rests, part, stream);
-    if (p.tile == 128) return launch_tile<KIND, 128, 2, PAIR, OT>(a, p, in, rests, part, stream);
-    if (p.units <= 256) return launch_tile<KIND, 64, 8, PAIR, OT>(a, p, in, rests, part, stream);
-    return launch_tile<KIND, 64, 4, PAIR, OT>(a, p, in, rests, part, stream);
+template <int KIND, typename OT>
+int launch_gemm(const NsArgs& a, const Plan& p, int in, float* part, hipStream_t stream) {
+    if (p.tile == 256) return launch_tile<KIND, 256, 2, OT>(a, p, in, part, stream);
+    if (p.tile == 128) return launch_tile<KIND, 128, 2, OT>(a, p, in, part, stream);
+    if (p.units <= 256) return launch_tile<KIND, 64, 8, OT>(a, p, in, part, stream);
+    return launch_tile<KIND, 64, 4, OT>(a, p, in, part, stream);
 }
 
 #define NS_TRY(call) do { if (int rc_ = (call)) return rc_; } while (0)
@@ -764,20 +739,11 @@ int run_group(const NsArgs& a, int count, int steps, float* part, hipStream_t st
     hipLaunchKernelGGL((k_ns_pack<T>), dim3(np / 64, mp / 64, count), dim3(256), 0, stream, a);
     DM_LAUNCH_CHECK();
     const Plan gram = plan(a.t, count, NS_GRAM), poly = plan(a.t, count, NS_POLY), step = plan(a.t, count, NS_STEP);
-    constexpr bool SHORT = std::is_same<T, __bf16>::value;       // bf16: the last two iterations without the rests, see the head of the file
-    const int plain_from = SHORT ? std::max(1, steps - 2) : steps;
     for (int k = 0; k < steps; ++k) {
-        if (k < plain_from) {
-            NS_TRY((launch_gemm<NS_GRAM, true, float>(a, gram, k & 1, true, part, stream)));
-            NS_TRY((launch_gemm<NS_POLY, true, float>(a, poly, 0, true, part, stream)));
-            if (k + 1 < steps) NS_TRY((launch_gemm<NS_STEP, true, float>(a, step, k & 1, k + 1 < plain_from, part, stream)));
-            else NS_TRY((launch_gemm<NS_LAST, true, T>(a, step, k & 1, false, part, stream)));
-        } else if constexpr (SHORT) {
-            NS_TRY((launch_gemm<NS_GRAM, false, float>(a, gram, k & 1, false, part, stream)));
-            NS_TRY((launch_gemm<NS_POLY, false, float>(a, poly, 0, false, part, stream)));
-            if (k + 1 < steps) NS_TRY((launch_gemm<NS_STEP, false, float>(a, step, k & 1, false, part, stream)));
-            else NS_TRY((launch_gemm<NS_LAST, false, T>(a, step, k & 1, false, part, stream)));
-        }
+        NS_TRY((launch_gemm<NS_GRAM, float>(a, gram, k & 1, part, stream)));
+        NS_TRY((launch_gemm<NS_POLY, float>(a, poly, 0, part, stream)));
+        if (k + 1 < steps) NS_TRY((launch_gemm<NS_STEP, float>(a, step, k & 1, part, stream)));
+        else NS_TRY((launch_gemm<NS_LAST, T>(a, step, k & 1, part, stream)));
     }
     return DM_OK;
 }

@@ -2025,7 +2025,8 @@ def _overlap(written, read):
 def orthogonalize(g, steps=5, eps=1e-7):
     """The Newton-Schulz orthogonalisation of g [..., rows, cols] (bf16, f16, fp32), matrix by matrix: x = g / (|g|_F + eps), then `steps` times
     x <- a x + (b x x^T + c (x x^T)^2) x on the shorter side, (a, b, c) = (3.4445, -4.7750, 2.0315): the matrix with g's singular vectors and
-    singular values near 1.  The products carry 22 bits (bf16 input: 11 in the last two steps), sums are fp32 (forward only)."""
+    singular values near 1.  Every product carries 22 bits (entries of x down to 2^-38, where |x|_F = 1 at the start), sums are fp32, and the result is
+    rounded once to g's type (forward only)."""
     if g.dim() < 2 or g.dtype not in _NS_DTYPES:
         raise ValueError("orthogonalize: a bf16, f16 or fp32 tensor [..., rows, cols] expected")
     if not 1 <= steps <= 64:

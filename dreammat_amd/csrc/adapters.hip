@@ -8,7 +8,8 @@
 // Three kernels:
 //   shrink  u = s x A_e^T, one pass over x; u is kept as a PAIR of 16-bit numbers (value and remainder: 16-22 significant bits), so
 //           the second product loses nothing against fp32 and still runs on the 16-bit matrix pipe.  In half precision a row is
-//           scaled by a power of two where its largest entry leaves [2^-3, 2^14): half's exponent range must not bound u.
+//           scaled by the power of two that brings its largest entry to [2^13, 2^14): half's exponent range must not bound u, and
+//           entries down to 2^-22 of the largest keep 16 bits (2^-27: 11), so that a small rank beside a large one keeps its gradient.
 //   expand  the big product, its K loop extended by [u_value | u_rest] [B | B]^T: the low-rank product costs 2 ceil(R/16) 16
 //           columns of K and no pass over y.  Rows of a tile that belong to another adapter are left out by selection (never by
 //           a multiplication with zero: 0 * inf of another request's adapter would reach them).
@@ -57,11 +58,12 @@ __device__ __forceinline__ int adapter_of(const Rows& r, long long m) {
 
 __device__ __forceinline__ float pow2_scale(float biggest) {
 #if defined(DM_F16)
-    // 1 where half holds the row's largest entry with a normal remainder (and for zeros, infinities, NaN), else 2^k that brings it to [2^8, 2^9)
-    if (!(biggest > 0.f) || biggest > 3.0e38f || (biggest >= 0.125f && biggest < 16384.f)) return 1.f;
+    // 2^k that brings the row's largest entry to [2^13, 2^14); 1 for zeros, infinities and NaN.  k >= -60, because the big product divides
+    // x W^T (below 2^52) by it in fp32: an even smaller u has fewer bits, and adds less than the smallest half.
+    if (!(biggest > 0.f) || biggest > 3.0e38f) return 1.f;
     int e;
     frexpf(biggest, &e);
-    return ldexpf(1.f, min(max(e - 9, -100), 100));
+    return ldexpf(1.f, max(e - 14, -60));
 #else
     return 1.f;
 #endif
@@ -452,25 +454,20 @@ __global__ __launch_bounds__(WM * WN * 64) void k_expand(ExpandArgs a) {
         aid[tid] = e;
 #if defined(DM_F16)
         const float scale = tid < mrows ? a.us[m0 + tid] : 1.f;
-        scale_of[tid] = e != kNone ? scale : 1.f;
+        scale_of[tid] = e != kNone ? scale : 1.f;                    // (us is written where there is an adapter)
 #endif
     }
     if (tid < BN) bias_of[tid] = a.bias && tid < nrows ? (float)a.bias[n0 + tid] : 0.f;
     __syncthreads();
-    int others = 0, scaled = 0;
+    int others = 0;
 #pragma unroll
-    for (int t = lane; t < BM; t += 64) {
-        others |= t < mrows && aid[t] != aid[0];
-#if defined(DM_F16)
-        scaled |= scale_of[t] != 1.f;
-#endif
-    }
+    for (int t = lane; t < BM; t += 64) others |= t < mrows && aid[t] != aid[0];
     mixed = __any(others);
     only = mixed ? next_adapter<BM>(aid, kNone) : aid[0] == kNone ? 0x7fffffff : __builtin_amdgcn_readfirstlane(aid[0]);
 #pragma unroll
     for (int q = 1; q < NST; ++q) ahead += issue();                  // (at first the whole ring is free)
-    // A tile of one adapter without row scales (nearly all: a request is longer than a tile): its low-rank columns are K steps like others
-    const bool uniform = only != 0x7fffffff && !mixed && !__any(scaled);
+    // A tile of one adapter (nearly all: a request is longer than a tile): its low-rank columns are K steps like others
+    const bool uniform = only != 0x7fffffff && !mixed;
     f32x16 acc[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -494,9 +491,8 @@ __global__ __launch_bounds__(WM * WN * 64) void k_expand(ExpandArgs a) {
         --ahead;
         if (!first) ahead += issue();
     };
-    const int low = (2 * Rp + 63) / 64, last = uniform ? steps + low : steps;
-    for (int s = 0; s < last; ++s) {
-        advance(s == 0);
+    auto multiply = [&](bool first) __attribute__((always_inline)) {
+        advance(first);
         const char* ab = smem + stage * STAGE;
         const char* bb = ab + A_BYTES;
 #pragma unroll
@@ -512,6 +508,27 @@ __global__ __launch_bounds__(WM * WN * 64) void k_expand(ExpandArgs a) {
                 for (int j = 0; j < NT; ++j) acc[i][j] = DM_MFMA_32x32x16(bf[j], af[i], acc[i][j]);
         }
         stage = stage + 1 == NST ? 0 : stage + 1;
+    };
+    for (int s = 0; s < steps; ++s) multiply(s == 0);
+    if (uniform) {
+        // in units of the row's power of two (exact; a lane's accumulators are one row per i)
+        [[maybe_unused]] auto rescale = [&](auto factor) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const float f = factor(scale_of[TM * wm + 32 * i + l31]);
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[i][j][r] *= f;
+            }
+        };
+#if defined(DM_F16)
+        rescale([](float p) { return 1.f / p; });
+#endif
+        for (int s = 0; s < 2 * Rp; s += 64) multiply(false);
+#if defined(DM_F16)
+        rescale([](float p) { return p; });
+#endif
     }
     int e = uniform ? 0x7fffffff : only, c0 = 0;
     while (e != 0x7fffffff) {

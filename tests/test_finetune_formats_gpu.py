@@ -1,11 +1,9 @@
 """GPU: the fine-tuning operators at the borders of their number formats -- the result's type only rounds it, one rank or one row far smaller than
 the others keeps its digits, an infinite entry gives what the formula gives.  Tolerances as in test_finetune_gpu.py."""
-import math
-
 import pytest
 import torch
 
-from tests.test_finetune_gpu import BF, DEV, FP, HF, adapter_inputs, adapter_reference, gen, near, ns_formula, rand, rel
+from tests.test_finetune_gpu import BF, DEV, HF, adapter_inputs, adapter_reference, gen, half, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -33,3 +31,58 @@ def test_muon_step_of_16_bit_gradients_is_the_fp32_step(nesterov, gdtype):
     hipops.muon_step(p, gr, m, lr=0.02, nesterov=nesterov)
     hipops.muon_step(p2, [q.float() for q in gr], m2, lr=0.02, nesterov=nesterov)
     assert all(torch.equal(a, b) for a, b in zip(p + m, p2 + m2))
+
+
+# ------------------------------------------------------------------------------------------------ adapters: unequal ranks and rows
+def close(got, ref, terms, n):
+    """`near`, down into the subnormals: the floor is half their step"""
+    t = got.dtype
+    tol = half(t) * ref.abs() * 1.001 + (n * 2.0 ** -23 + 2.0 ** -17) * terms + torch.finfo(t).tiny * half(t)
+    worst = ((got.double() - ref).abs() / tol).max().item()
+    assert torch.isfinite(got).all() and worst <= 1.0, worst
+
+
+def check_all(s, scale=1.0):
+    """forward and gradients against 64 bits -> the outputs"""
+    from dreammat_amd import hipops
+    ref = adapter_reference(s, scale)
+    K, N, R, M = s["x"].shape[-1], s["w"].shape[0], s["a"].shape[1], s["x"].numel() // s["x"].shape[-1]
+    x, a, b = (s[k].detach().requires_grad_() for k in ("x", "a", "b"))
+    y = hipops.linear_adapted_autograd(x, s["w"], s["w"].t().contiguous(), s["bias"], a, b, s["ids"], scale, s["residual"], s["offsets"])
+    dx, da, db = torch.autograd.grad(y, (x, a, b), s["dy"])
+    close(y.detach().reshape(M, N), *ref["y"], K + 2 * R)
+    close(dx.reshape(M, K), *ref["dx"], N + 2 * R)
+    close(da, *ref["da"], M + N)
+    close(db, *ref["db"], M + K)
+    return y.detach(), dx, da, db
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("rows", [96, 12400])
+@pytest.mark.parametrize("side", ["a", "b"])
+def test_linear_adapted_of_ranks_of_unequal_size(side, rows, dtype):
+    """rank r is 2^-r of the first one in A (so in u), or in B (so in du): every rank's gradients keep their digits.  Half: entries down to 2^-22 of
+    their row's largest keep 2^-16 of themselves, smaller ones are off by no more than those; a rank of 2^-15 is that far down only where its
+    product is 2^-7 of its usual size, and those rows hardly count in its sum."""
+    s = adapter_inputs(21, dtype, (rows, 64), 136, 16, 2, [0, 1, 1, 0])
+    down = 2.0 ** -torch.arange(16, device=DEV)
+    if side == "a":                                      # u = 1 ... 2^-15; dy large, so that the results stay normal halves
+        s["a"] = (s["a"].float() * down[None, :, None]).to(dtype)
+        s["b"] = (s["b"].float() / 64).to(dtype)
+        s["dy"] = (s["dy"].float() * 100).to(dtype)
+    else:                                                # du = 0.5 ... 2^-16; x large
+        s["b"] = (s["b"].float() * down[None, None, :]).to(dtype)
+        s["x"] = (s["x"].float() * 100).to(dtype)
+        s["dy"] = (s["dy"].float() / 6).to(dtype)
+    check_all(s, 1.0)
+
+
+@pytest.mark.parametrize("rows", [96, 12400])
+def test_linear_adapted_half_of_rows_of_unequal_size(rows):
+    """rows of x and of dy from 2^-12 to 2^11 next to each other, in a tile and in a range of the weight gradients (both products of a row are
+    then of one size: every row counts)"""
+    s = adapter_inputs(22, HF, (rows, 64), 136, 16, 2, [0, 1])
+    size = 2.0 ** (torch.arange(rows, device=DEV) % 24 - 12.0)[:, None]
+    s["x"] = (s["x"].float() * size).to(HF)
+    s["dy"] = (s["dy"].float() * size.flip(0) * 2.0 ** -10).to(HF)
+    check_all(s, 1.0)

@@ -10,6 +10,8 @@
 //           the second product loses nothing against fp32 and still runs on the 16-bit matrix pipe.  In half precision a row is
 //           scaled by the power of two that brings its largest entry to [2^13, 2^14): half's exponent range must not bound u, and
 //           entries down to 2^-22 of the largest keep 16 bits (2^-27: 11), so that a small rank beside a large one keeps its gradient.
+//           Infinities come out as the formula has them: an infinite u has a zero rest, and where the other factor is infinite the
+//           rest takes no part (the value's product decides; the rest's would turn it into NaN).
 //   expand  the big product, its K loop extended by [u_value | u_rest] [B | B]^T: the low-rank product costs 2 ceil(R/16) 16
 //           columns of K and no pass over y.  Rows of a tile that belong to another adapter are left out by selection (never by
 //           a multiplication with zero: 0 * inf of another request's adapter would reach them).
@@ -58,9 +60,9 @@ __device__ __forceinline__ int adapter_of(const Rows& r, long long m) {
 
 __device__ __forceinline__ float pow2_scale(float biggest) {
 #if defined(DM_F16)
-    // 2^k that brings the row's largest entry to [2^13, 2^14); 1 for zeros, infinities and NaN.  k >= -60, because the big product divides
+    // 2^k that brings the row's largest entry to [2^13, 2^14); 1 for a row of zeros.  k >= -60, because the big product divides
     // x W^T (below 2^52) by it in fp32: an even smaller u has fewer bits, and adds less than the smallest half.
-    if (!(biggest > 0.f) || biggest > 3.0e38f) return 1.f;
+    if (!(biggest > 0.f)) return 1.f;
     int e;
     frexpf(biggest, &e);
     return ldexpf(1.f, max(e - 14, -60));
@@ -72,10 +74,31 @@ __device__ __forceinline__ float pow2_scale(float biggest) {
 // ------------------------------------------------------------------------------------------------ shrink
 // u rows are stored [value: Rp | rest: Rp] elem_t (Rp = rank_pad(R), columns past R zero) with us[m] = the row's power of two and who[m] = the
 // row's adapter, which the big product then reads instead of searching for it.
+__device__ __forceinline__ elem_t rest_of(float v, elem_t hi) {
+    const float h = (float)hi;
+    return fabsf(h) <= 3.4028235e38f ? (elem_t)(v - h) : (elem_t)0.f;
+}
+
 __device__ __forceinline__ void store_pair(elem_t* u, int Rp, int r, float v) {
     const elem_t hi = (elem_t)v;
     u[r] = hi;
-    u[Rp + r] = (elem_t)(v - (float)hi);
+    u[Rp + r] = rest_of(v, hi);
+}
+
+// |v| where v is finite, for the largest entry of a row
+__device__ __forceinline__ float finite_abs(float v) { return fabsf(v) <= 3.4028235e38f ? fabsf(v) : 0.f; }
+
+// the entries with infinities and NaN as zeros (an exponent of ones), two to a dword
+__device__ __forceinline__ elem8 finite_only(elem8 v) {
+    typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+#if defined(DM_F16)
+    constexpr unsigned short biggest = 0x7bff;
+#else
+    constexpr unsigned short biggest = 0x7f7f;
+#endif
+    const u16x8 bits = __builtin_bit_cast(u16x8, v), one = 1;
+    const u16x8 over = __builtin_elementwise_sub_sat(bits & (unsigned short)0x7fff, u16x8(biggest));        // 0 where finite
+    return __builtin_bit_cast(elem8, bits & (__builtin_elementwise_min(over, one) - one));
 }
 
 // the smallest entry of a tile's adapters above cur (INT_MAX: none), the same in every wave
@@ -174,7 +197,7 @@ __global__ __launch_bounds__(256) void k_shrink(const elem_t* __restrict__ x, co
             for (int q = 0; q < NR; ++q) {
                 const int r = 16 * q + l15;
                 v[q] = r < R ? scale * (part[0][t][r] + part[1][t][r] + part[2][t][r] + part[3][t][r]) : 0.f;
-                big = fmaxf(big, fabsf(v[q]));
+                big = fmaxf(big, finite_abs(v[q]));
             }
 #if defined(DM_F16)
 #pragma unroll
@@ -269,7 +292,7 @@ __global__ __launch_bounds__(256) void k_shrink_ring(const elem_t* __restrict__ 
 #pragma unroll
             for (int q = 0; q < NR; ++q) {
                 v[q] = 16 * q + l15 < R ? scale * acc[q][i] : 0.f;
-                big = fmaxf(big, fabsf(v[q]));
+                big = fmaxf(big, finite_abs(v[q]));
             }
 #if defined(DM_F16)
 #pragma unroll
@@ -315,7 +338,7 @@ __global__ __launch_bounds__(1024) void k_shrink_rows(const elem_t* __restrict__
             for (int r = tid; r < Rp; r += blockDim.x) f32out[m * Rp + r] = r < R ? row[r] : 0.f;
         } else {
             float big = 0.f;
-            for (int r = 0; r < R; ++r) big = fmaxf(big, fabsf(row[r]));
+            for (int r = 0; r < R; ++r) big = fmaxf(big, finite_abs(row[r]));
             const float p = pow2_scale(big);
             for (int r = tid; r < Rp; r += blockDim.x) store_pair(u + m * 2 * Rp, Rp, r, r < R ? row[r] / p : 0.f);
             if (tid == 0) us[m] = p;
@@ -491,7 +514,8 @@ __global__ __launch_bounds__(WM * WN * 64) void k_expand(ExpandArgs a) {
         --ahead;
         if (!first) ahead += issue();
     };
-    auto multiply = [&](bool first) __attribute__((always_inline)) {
+    // low: the step's columns from Rp on are rests
+    auto multiply = [&](bool first, auto low, int c0) __attribute__((always_inline)) {
         advance(first);
         const char* ab = smem + stage * STAGE;
         const char* bb = ab + A_BYTES;
@@ -501,7 +525,10 @@ __global__ __launch_bounds__(WM * WN * 64) void k_expand(ExpandArgs a) {
 #pragma unroll
             for (int i = 0; i < MT; ++i) af[i] = frag(ab, TM * wm + 32 * i + l31, kk);
 #pragma unroll
-            for (int j = 0; j < NT; ++j) bf[j] = frag(bb, TN * wn + 32 * j + l31, kk);
+            for (int j = 0; j < NT; ++j) {
+                bf[j] = frag(bb, TN * wn + 32 * j + l31, kk);
+                if constexpr (decltype(low)::value) if (c0 + 16 * kk >= Rp) bf[j] = finite_only(bf[j]);
+            }
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -509,7 +536,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_expand(ExpandArgs a) {
         }
         stage = stage + 1 == NST ? 0 : stage + 1;
     };
-    for (int s = 0; s < steps; ++s) multiply(s == 0);
+    for (int s = 0; s < steps; ++s) multiply(s == 0, std::false_type{}, 0);
     if (uniform) {
         // in units of the row's power of two (exact; a lane's accumulators are one row per i)
         [[maybe_unused]] auto rescale = [&](auto factor) __attribute__((always_inline)) {
@@ -525,7 +552,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_expand(ExpandArgs a) {
 #if defined(DM_F16)
         rescale([](float p) { return 1.f / p; });
 #endif
-        for (int s = 0; s < 2 * Rp; s += 64) multiply(false);
+        for (int c0 = 0; c0 < 2 * Rp; c0 += 64) multiply(false, std::true_type{}, c0);
 #if defined(DM_F16)
         rescale([](float p) { return p; });
 #endif
@@ -550,8 +577,10 @@ __global__ __launch_bounds__(WM * WN * 64) void k_expand(ExpandArgs a) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) t[r] = 0.f;
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk)                       // (columns past 2 Rp are zeros)
-                    t = DM_MFMA_32x32x16(frag(bb, TN * wn + 32 * j + l31, kk), frag(ab, row, kk), t);
+                for (int kk = 0; kk < 4; ++kk) {                     // (columns past 2 Rp are zeros)
+                    const elem8 bf = frag(bb, TN * wn + 32 * j + l31, kk);
+                    t = DM_MFMA_32x32x16(c0 + 16 * kk >= Rp ? finite_only(bf) : bf, frag(ab, row, kk), t);
+                }
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[i][j][r] += mine ? t[r] * scale : 0.f;
                 __builtin_amdgcn_sched_barrier(0);                   // one fragment at a time: the accumulators leave no registers for more
@@ -913,7 +942,7 @@ __global__ __launch_bounds__(256) void k_wgrad(WgradArgs a) {
             for (int k = 0; k < 8; ++k) {
                 const float w = ((float)ph[q][k] + (float)pl[q][k]) * pf[q];
                 ph[q][k] = (elem_t)w;
-                pl[q][k] = (elem_t)(w - (float)ph[q][k]);
+                pl[q][k] = rest_of(w, ph[q][k]);
             }
 #endif
             *reinterpret_cast<elem8*>(ub + row * UP + c * 2) = ph[q];
@@ -943,14 +972,15 @@ __global__ __launch_bounds__(256) void k_wgrad(WgradArgs a) {
     const int c = c0 + 32 * wave + l31;
     if (c >= C) return;
     float* out = a.part[side] + (long long)it * Rp * C + c;
+    auto both = [&](float value, float rest) { return (fabsf(value) <= 3.4028235e38f ? value + rest : value) * top; };      // (an infinite x: the value decides)
     if constexpr (Rp == 16) {
 #pragma unroll
-        for (int r = 0; r < 8; ++r) out[(long long)((r & 3) + 8 * (r >> 2) + 4 * hi) * C] = (acc[0][r] + acc[0][r + 8]) * top;
+        for (int r = 0; r < 8; ++r) out[(long long)((r & 3) + 8 * (r >> 2) + 4 * hi) * C] = both(acc[0][r], acc[0][r + 8]);
     } else {
 #pragma unroll
         for (int f = 0; f < UF / 2; ++f)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) out[(long long)(32 * f + (r & 3) + 8 * (r >> 2) + 4 * hi) * C] = (acc[f][r] + acc[f + UF / 2][r]) * top;
+            for (int r = 0; r < 16; ++r) out[(long long)(32 * f + (r & 3) + 8 * (r >> 2) + 4 * hi) * C] = both(acc[f][r], acc[f + UF / 2][r]);
     }
 }
 

@@ -3,7 +3,7 @@ the others keeps its digits, an infinite entry gives what the formula gives.  To
 import pytest
 import torch
 
-from tests.test_finetune_gpu import BF, DEV, HF, adapter_inputs, adapter_reference, gen, half, rand
+from tests.test_finetune_gpu import BF, DEV, HF, adapter_inputs, adapter_reference, gen, half, near, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -86,3 +86,36 @@ def test_linear_adapted_half_of_rows_of_unequal_size(rows):
     s["x"] = (s["x"].float() * size).to(HF)
     s["dy"] = (s["dy"].float() * size.flip(0) * 2.0 ** -10).to(HF)
     check_all(s, 1.0)
+
+
+# ------------------------------------------------------------------------------------------------ adapters: infinite entries
+def same_with_infinities(got, ref, terms, n):
+    """finite, +inf, -inf and NaN where the formula has them; `near` on the finite ones"""
+    assert torch.equal(torch.isnan(got), torch.isnan(ref))
+    inf = torch.isinf(ref)
+    assert torch.equal(torch.isinf(got), inf) and torch.equal(got[inf].double(), ref[inf])
+    fine = torch.isfinite(ref)
+    near(torch.where(fine, got, 0.0), torch.where(fine, ref, 0.0), torch.where(fine, terms, 0.0), n, 2.0 ** -17)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("R", [8, 16, 24, 40, 100])
+@pytest.mark.parametrize("rows", [24, 384, 12400])
+@pytest.mark.parametrize("where", ["a", "b", "x", "dy"])
+def test_linear_adapted_infinite_entry(where, rows, R, dtype):
+    """one infinite entry: +-inf where the formula says so, whatever the number of rows, and nothing elsewhere"""
+    from dreammat_amd import hipops
+    s = adapter_inputs(23, dtype, (rows, 64), 136, R, 3, [0, 1, -1, 2])
+    at = {"a": (1, R - 1, 5), "b": (1, 9, R - 1), "x": (rows // 4 + 1, 5), "dy": (rows // 4 + 1, 9)}[where]
+    s[where][at] = float("inf")
+    ref = {k: (v, t.nan_to_num(0.0, 0.0, 0.0)) for k, (v, t) in adapter_reference(s, 1.0).items()}
+    if where == "a":                                     # 0 inf of rows of other adapters is no part of the formula
+        assert torch.isinf(ref["y"][0][rows // 4:rows // 2]).all()
+    y = hipops.linear_adapted(s["x"], s["w"], s["bias"], s["a"], s["b"], s["ids"])
+    same_with_infinities(y, *ref["y"], 64 + 2 * R)
+    x, a, b = (s[k].detach().requires_grad_() for k in ("x", "a", "b"))
+    y = hipops.linear_adapted_autograd(x, s["w"], s["w"].t().contiguous(), s["bias"], a, b, s["ids"])
+    grads = torch.autograd.grad(y, (x, a, b), s["dy"])
+    same_with_infinities(y.detach(), *ref["y"], 64 + 2 * R)
+    for name, got, n in zip(("dx", "da", "db"), grads, (136 + 2 * R, rows + 136, rows + 64)):
+        same_with_infinities(got, *ref[name], n)

@@ -1982,7 +1982,7 @@ class _GatedAddNorm(torch.autograd.Function):
 
 def gated_add_norm(x, h, gate=None, post=None, pre=None, scale=1.0, eps=1e-5, kind="layer"):
     """y = x + scale * gate * N_post(h) and, with `pre`, z = N_pre(y): a block's residual step with the norm behind the block, its gate and
-    residual scale, and the norm in front of the next block, in one pass (differentiable in every tensor).
+    residual scale, and the norm in front of the next block, in one pass (differentiable in every tensor, in backward mode).
 
     x, h [..., C] bf16, f16 or fp32 (C <= 8192); gate [C] or one row per leading item of x [items, C]; post / pre = (gamma, beta), either may
     be None inside; kind "layer" (mean and variance) or "rms".  -> y, or (y, z) with pre.  Statistics and sums in fp32; z is formed from the
@@ -1991,7 +1991,8 @@ def gated_add_norm(x, h, gate=None, post=None, pre=None, scale=1.0, eps=1e-5, ki
     flat = [x, h, gate, *(post or (None, None)), *(pre or (None, None))]
     flat = [t if t is None or t.is_contiguous() else t.contiguous() for t in flat]
     flags, scale, eps = (int(post is not None), int(pre is not None), int(kind == "rms")), float(scale), float(eps)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in flat):
+    # (inside a forward-mode level too: the function has no jvp and refuses a tangent, where the plain call would drop it)
+    if torch.autograd.forward_ad._current_level >= 0 or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in flat)):
         return _GatedAddNorm.apply(*flat, flags, item_rows, scale, eps)
     y, z, _ = _gated_forward(*flat, flags, item_rows, scale, eps, False)
     return y if z is None else (y, z)

@@ -119,3 +119,18 @@ def test_linear_adapted_infinite_entry(where, rows, R, dtype):
     same_with_infinities(y.detach(), *ref["y"], 64 + 2 * R)
     for name, got, n in zip(("dx", "da", "db"), grads, (136 + 2 * R, rows + 136, rows + 64)):
         same_with_infinities(got, *ref[name], n)
+
+
+# ------------------------------------------------------------------------------------------------ norms
+def test_gated_add_norm_refuses_forward_mode():
+    """a tangent is refused, not dropped: the operator has a backward pass only"""
+    from torch.autograd import forward_ad
+    from dreammat_amd import hipops
+    x, h = rand(gen(1), 4, 64), rand(gen(2), 4, 64)
+    with forward_ad.dual_level():
+        for v in ((forward_ad.make_dual(x, h), h), (x, forward_ad.make_dual(h, x))):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError):
+                    hipops.gated_add_norm(*v, pre=(None, None))
+        y = hipops.gated_add_norm(x, h)                                # no tangent: as ever
+    assert torch.equal(y, hipops.gated_add_norm(x, h))

@@ -1144,7 +1144,8 @@ int check_product(const Rows& r, const void* x, const void* w, const void* lora_
 // row ranges of the weight gradients: enough workgroups to fill the chip (four per CU over the 128-column tiles of both), but whole 64-row
 // stages and few partial sums
 int wgrad_chunk(long long M, int K, int N) { return (int)std::max<long long>(128, (M * ((K + N + 127) / 128) / 1024 + 63) / 64 * 64); }
-long long wgrad_items(long long M, int E, int chunk) { return std::min<long long>(M, M / chunk + E); }
+// the most row ranges: full ones, and one that ends early for every adapter that a request can name
+long long wgrad_items(long long M, int E, long long n, int chunk) { return std::min<long long>(M, M / chunk + std::min<long long>(E, n)); }
 
 }  // namespace
 
@@ -1162,7 +1163,7 @@ size_t dm_linear_adapted_bwd_workspace_bytes(long long M, int K, int N, int R, i
     if (M <= 0 || K <= 0 || N <= 0 || R <= 0 || R > kMaxRank || E <= 0 || n <= 0) return 0;
     const int Rp = rank_pad(R);
     return (size_t)(u_bytes(M, R) + align256(2LL * E * K * Rp) + align256(2LL * E * N * R) + align256(4 * (2LL * (E + 1) + n + M)) +
-                    4LL * wgrad_items(M, E, wgrad_chunk(M, K, N)) * Rp * (K + N));
+                    4LL * wgrad_items(M, E, n, wgrad_chunk(M, K, N)) * Rp * (K + N));
 }
 #endif
 
@@ -1215,7 +1216,7 @@ int DM_T(dm_linear_adapted_bwd_, )(const void* x, const void* dy, const void* w_
     if (int rc = check_product(rows, x, w_t, lora_a, lora_b, K, N, R)) return rc;
     if (!dy || !ws || M == 0 || (dx && !w_t) || (db && !u) || (((uintptr_t)dy | (uintptr_t)u | (uintptr_t)ws | (uintptr_t)dx) & 15)) return DM_ERR_ARG;
     const int Rp = rank_pad(R), chunk = wgrad_chunk(M, K, N);
-    const long long items = wgrad_items(M, E, chunk);
+    const long long items = wgrad_items(M, E, n, chunk);
     if (items > 65535) return DM_ERR_UNSUPPORTED;
     if ((long long)ws_bytes < u_bytes(M, R) + align256(2LL * E * K * Rp) + align256(2LL * E * N * R) + align256(4 * (2LL * (E + 1) + n + M)) + 4LL * items * Rp * (K + N))
         return DM_ERR_WORKSPACE;

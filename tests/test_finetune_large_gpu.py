@@ -59,6 +59,18 @@ def test_linear_adapted_large_half_rows_of_every_scale(rows, size):
         check_adapter(s, 0.5, True)
 
 
+def test_linear_adapted_gradients_of_many_stored_adapters():
+    """more stored adapters than requests, R off 8 and on it: the row ranges follow the adapters that are used, the others get zeros"""
+    for E, rows, ids, R in ((3000, 1500, [2999, 7, 7, -1, 0], 4), (500, 12400, [499, 0], 16), (900, 8200, None, 12)):
+        offsets = None
+        if ids is None:
+            offsets, ids = cuts(rows, 60, 9), [(53 * i) % (E + 1) - 1 for i in range(60)]
+        s = adapter_inputs(31, BF, (rows, 72), 136, R, E, ids, False, True, offsets)
+        _, _, da, db = check_adapter(s, 0.5, True)
+        unused = [e for e in range(E) if e not in ids]
+        assert not da[unused].any() and not db[unused].any()
+
+
 LARGE_NORMS = [
     # shape, gate, post, pre, kind, type
     ((3, 5001, 320), "item", (1, 1), (1, 1), "layer", BF),          # rows of a quarter wave: two workgroups per CU, gates change inside a workgroup

@@ -1039,10 +1039,12 @@ __global__ __launch_bounds__(256) void k_wgrad_join(WgradArgs a, int blocks_a, i
 }
 
 // ------------------------------------------------------------------------------------------------ host side
+constexpr long long kMostRows = 1 << 30;        // a grid holds fewer than 2^32 threads: 256 per 64 rows of x A^T, and of a result of up to 64 columns
+
 int check_rows(const int* ids, long long n, long long M, int E, bool offsets) {
     if (!ids || n <= 0 || n > 0x7fffffff || M < 0 || M > 0x7fffffff || E <= 0) return DM_ERR_ARG;
     if (!offsets && (M % n)) return DM_ERR_ARG;
-    return DM_OK;
+    return M < kMostRows ? DM_OK : DM_ERR_UNSUPPORTED;
 }
 
 Rows make_rows(const int* ids, const int* offsets, long long n, long long M, int E) {
@@ -1108,7 +1110,7 @@ int launch_expand(ExpandArgs a, hipStream_t stream) {
     constexpr int LDS = NST * (BM + BN) * 128 + BM * 8 + BN * 4;
     const long long n_mt = (a.rows.M + BM - 1) / BM;
     a.n_nt = (a.N + BN - 1) / BN;
-    if (n_mt * a.n_nt > (1LL << 30)) return DM_ERR_UNSUPPORTED;
+    if (n_mt * a.n_nt > (1LL << 24) - 8) return DM_ERR_UNSUPPORTED;        // 2^32 threads; past the memory of any result that takes 128 tiles
     a.n_mt = (int)n_mt;
     a.tiles = (int)(n_mt * a.n_nt);
     static unsigned long long devices = 0;

@@ -1811,8 +1811,8 @@ def _adapter_sizes(x, w, bias, lora_a, lora_b, ids, residual, offsets):
         raise ValueError("linear_adapted: bias [N] expected")
     if residual is not None and residual.shape != (*x.shape[:-1], N):
         raise ValueError("linear_adapted: the residual has the result's shape")
-    if M >= 1 << 31:
-        raise ValueError("linear_adapted: fewer than 2^31 rows")
+    if M >= 1 << 30:
+        raise ValueError(f"linear_adapted: {M} rows: fewer than 2^30 are supported")
     return M, K, N, R, E, n
 
 

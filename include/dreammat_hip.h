@@ -553,8 +553,8 @@ int dm_gated_add_norm_bwd_f32(const void* x, const void* h, const void* gate, lo
 /* Low-rank adapters of many requests beside a frozen projection (csrc/adapters.hip); the _f16 forms take IEEE half.
  *   y = x w^T + bias + scale (x A_e^T) B_e^T + residual,   e = ids[request of the row]
  * x [M, K], w [N, K], bias [N] / residual [M, N] or NULL, lora_a [E, R, K], lora_b [E, N, R], R <= 128; ids int32 [n]; offsets int32 [n + 1],
- * ascending, or NULL (n requests of M / n rows).  Rows of no request and ids outside [0, E) have no adapter.  K, N multiples of 8, pointers
- * 16-byte aligned.  ws: dm_linear_adapted_workspace_bytes; keep_u != 0 leaves scale x A^T in it for the backward. */
+ * ascending, or NULL (n requests of M / n rows).  Rows of no request and ids outside [0, E) have no adapter.  K, N multiples of 8, M < 2^30,
+ * pointers 16-byte aligned.  ws: dm_linear_adapted_workspace_bytes; keep_u != 0 leaves scale x A^T in it for the backward. */
 size_t dm_linear_adapted_workspace_bytes(long long M, int N, int R, int E);
 int dm_linear_adapted_bf16(const void* x, const void* w, const void* bias, const void* residual, const void* lora_a, const void* lora_b,
                            const int32_t* ids, const int32_t* offsets, long long n, float scale, void* ws, size_t ws_bytes, void* y, long long M, int K,

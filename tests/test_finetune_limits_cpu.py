@@ -20,3 +20,17 @@ def test_backward_workspace_follows_the_adapters_a_call_can_use():
     assert bwd(sizes(1000, 24) - 1) == -2
     # as many adapters as an id can name, one request: 64 K adapters of one row range each were refused
     assert L.dm_linear_adapted_bwd_bf16(P, P, P, P, P, P, None, 1, 1.0, P, P, 16, P, P, P, 128 * 70000, 64, 64, 16, 65535, None) == -2
+
+
+def test_adapters_refuse_more_rows_than_a_grid_holds():
+    """2^30 rows would take grids of 2^32 threads"""
+    BF, rows = torch.bfloat16, 1 << 30
+    x, w = torch.zeros(1, 8, dtype=BF).expand(rows, 8), torch.zeros(8, 8, dtype=BF)
+    args = (torch.zeros(1, 16, 8, dtype=BF), torch.zeros(1, 8, 16, dtype=BF), torch.zeros(1, dtype=torch.int32))
+    with pytest.raises(ValueError, match="rows"):
+        hipops.linear_adapted(x, w, None, *args)
+    with pytest.raises(ValueError, match="rows"):
+        hipops.linear_adapted_autograd(x, w, w, None, *args)
+    L, P = _lib.lib(), 1 << 12
+    assert L.dm_linear_adapted_bf16(P, P, None, None, P, P, P, None, 1, 1.0, P, 1 << 50, P, rows, 8, 8, 16, 1, 0, None) == -3
+    assert L.dm_linear_adapted_bwd_bf16(P, P, P, P, P, P, None, 1, 1.0, P, P, 1 << 50, P, P, P, rows, 8, 8, 16, 1, None) == -3

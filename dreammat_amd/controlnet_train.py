@@ -116,15 +116,17 @@ class MuonAdamW:
             self.adamw.zero_grad(set_to_none=set_to_none)
 
     def state_dict(self):
-        return {"momenta": self.momenta, "adamw": self.adamw.state_dict() if self.adamw is not None else None}
+        return {"momenta": self.momenta, "adamw": self.adamw.state_dict() if self.adamw is not None else None, "lr": self.lr,
+                "weight_decay": self.weight_decay, "momentum": self.momentum}
 
     def load_state_dict(self, state):
         if len(state["momenta"]) != len(self.matrices) or (state["adamw"] is None) != (self.adamw is None):
             raise ValueError("MuonAdamW: the state belongs to other parameters")
         self.momenta = [None if m is None else m.to(p.device, torch.float32).reshape(p.shape).clone(memory_format=torch.contiguous_format)
                         for m, p in zip(state["momenta"], self.matrices)]
+        self.lr, self.weight_decay, self.momentum = (state.get(k, getattr(self, k)) for k in ("lr", "weight_decay", "momentum"))
         if self.adamw is not None:
-            self.adamw.load_state_dict(state["adamw"])
+            self.adamw.load_state_dict(state["adamw"])               # (brings its rate and decay the same way)
 
 
 class ControlNetTrainer:

@@ -34,3 +34,17 @@ def test_adapters_refuse_more_rows_than_a_grid_holds():
     L, P = _lib.lib(), 1 << 12
     assert L.dm_linear_adapted_bf16(P, P, None, None, P, P, P, None, 1, 1.0, P, 1 << 50, P, rows, 8, 8, 16, 1, 0, None) == -3
     assert L.dm_linear_adapted_bwd_bf16(P, P, P, P, P, P, None, 1, 1.0, P, P, 1 << 50, P, P, P, rows, 8, 8, 16, 1, None) == -3
+
+
+def test_muon_state_brings_its_learning_rate_to_both_halves():
+    """a restored state sets rate and decay of the matrices as torch's AdamW sets those of the rest: one rate for both"""
+    from dreammat_amd.controlnet_train import MuonAdamW
+    params = [torch.nn.Parameter(torch.zeros(4, 6)), torch.nn.Parameter(torch.zeros(4))]
+    a, b = MuonAdamW(params, lr=1e-3, weight_decay=0.1, momentum=0.9), MuonAdamW(params, lr=1e-5)
+    b.load_state_dict(a.state_dict())
+    assert (b.lr, b.weight_decay, b.momentum) == (1e-3, 0.1, 0.9)
+    assert all(g["lr"] == b.lr and g["weight_decay"] == b.weight_decay for g in b.adamw.param_groups)
+    # a state without them (saved before it held them) leaves the matrices' own
+    c = MuonAdamW(params, lr=1e-5)
+    c.load_state_dict({"momenta": [None], "adamw": c.adamw.state_dict()})
+    assert c.lr == 1e-5

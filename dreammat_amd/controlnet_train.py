@@ -120,9 +120,10 @@ class MuonAdamW:
                 "weight_decay": self.weight_decay, "momentum": self.momentum}
 
     def load_state_dict(self, state):
-        if len(state["momenta"]) != len(self.matrices) or (state["adamw"] is None) != (self.adamw is None):
+        if (len(state["momenta"]) != len(self.matrices) or (state["adamw"] is None) != (self.adamw is None)
+                or any(m is not None and m.shape != p.shape for m, p in zip(state["momenta"], self.matrices))):
             raise ValueError("MuonAdamW: the state belongs to other parameters")
-        self.momenta = [None if m is None else m.to(p.device, torch.float32).reshape(p.shape).clone(memory_format=torch.contiguous_format)
+        self.momenta = [None if m is None else m.to(p.device, torch.float32).clone(memory_format=torch.contiguous_format)
                         for m, p in zip(state["momenta"], self.matrices)]
         self.lr, self.weight_decay, self.momentum = (state.get(k, getattr(self, k)) for k in ("lr", "weight_decay", "momentum"))
         if self.adamw is not None:

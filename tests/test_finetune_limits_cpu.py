@@ -48,3 +48,12 @@ def test_muon_state_brings_its_learning_rate_to_both_halves():
     c = MuonAdamW(params, lr=1e-5)
     c.load_state_dict({"momenta": [None], "adamw": c.adamw.state_dict()})
     assert c.lr == 1e-5
+
+
+def test_muon_state_of_other_shapes_is_refused():
+    from dreammat_amd.controlnet_train import MuonAdamW
+    one, other = (MuonAdamW([torch.nn.Parameter(torch.zeros(*s))], lr=1e-3) for s in ((4, 6), (6, 4)))
+    one.momenta[0] = torch.ones(4, 6)
+    with pytest.raises(ValueError, match="other parameters"):
+        other.load_state_dict(one.state_dict())
+    assert other.momenta == [None]

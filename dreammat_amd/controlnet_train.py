@@ -164,13 +164,13 @@ class ControlNetTrainer:
         params = self._params()
         self._opt_dtype = params[0].dtype
         self._opt_device = params[0].device
-        if any(p.dtype != torch.float32 for p in params):
-            self.master = [p.detach().float().clone(memory_format=torch.contiguous_format if self.optimizer == "muon" else torch.preserve_format)
-                           .requires_grad_() for p in params]
+        muon = self.optimizer == "muon"                              # (its step takes contiguous matrices)
+        if any(p.dtype != torch.float32 or (muon and not p.is_contiguous()) for p in params):
+            self.master = [p.detach().float().clone(memory_format=torch.contiguous_format if muon else torch.preserve_format).requires_grad_() for p in params]
             target = self.master
         else:
             self.master, target = None, params
-        make = MuonAdamW if self.optimizer == "muon" else torch.optim.AdamW
+        make = MuonAdamW if muon else torch.optim.AdamW
         self.opt = make(target, lr=self.lr, weight_decay=self.weight_decay)
 
     def apply_gradients(self, world=1):

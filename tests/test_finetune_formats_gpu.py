@@ -134,3 +134,21 @@ def test_gated_add_norm_refuses_forward_mode():
                     hipops.gated_add_norm(*v, pre=(None, None))
         y = hipops.gated_add_norm(x, h)                                # no tangent: as ever
     assert torch.equal(y, hipops.gated_add_norm(x, h))
+
+
+def test_controlnet_trainer_takes_channels_last_weights():
+    """fp32 weights in channels_last: the same step, bit for bit, as from contiguous ones"""
+    from dreammat_amd import controlnet_train as ct
+    from dreammat_amd.sd import ARCHS, AutoencoderKLEncoder, UNet2DConditionModel
+    a = ARCHS["tiny"]
+    out = []
+    for form in (torch.contiguous_format, torch.channels_last):
+        torch.manual_seed(0)
+        unet = UNet2DConditionModel(a).to(DEV)
+        tr = ct.ControlNetTrainer(AutoencoderKLEncoder(a).to(DEV), unet, ct.init_controlnet(unet).to(DEV, memory_format=form), lr=1e-3, max_grad_norm=1e9,
+                                  optimizer="muon")
+        for i, p in enumerate(tr._params()):
+            p.grad = rand(gen(i), *p.shape).to(memory_format=form if p.dim() == 4 else torch.contiguous_format)
+        tr.apply_gradients()
+        out.append([p.detach().clone() for p in tr._params()])
+    assert all(torch.equal(p, q) for p, q in zip(*out))

@@ -57,3 +57,15 @@ def test_muon_state_of_other_shapes_is_refused():
     with pytest.raises(ValueError, match="other parameters"):
         other.load_state_dict(one.state_dict())
     assert other.momenta == [None]
+
+
+def test_trainer_steps_matrices_of_any_memory_format():
+    """fp32 weights that are not contiguous (channels_last) get contiguous masters: the step takes no others"""
+    from dreammat_amd import controlnet_train as ct
+    from dreammat_amd.sd import ARCHS, AutoencoderKLEncoder, UNet2DConditionModel
+    a = ARCHS["tiny"]
+    unet = UNet2DConditionModel(a)
+    net = ct.init_controlnet(unet).to(memory_format=torch.channels_last)
+    tr = ct.ControlNetTrainer(AutoencoderKLEncoder(a), unet, net, optimizer="muon")
+    assert any(not p.is_contiguous() for p in tr._params()) and all(p.is_contiguous() for p in tr.opt.matrices)
+    assert ct.ControlNetTrainer(AutoencoderKLEncoder(a), unet, net).master is None

@@ -1832,6 +1832,8 @@ def _adapter_forward(x, w, bias, lora_a, lora_b, ids, scale, residual, offsets, 
         with _timed(lambda: f"linear_adapted[M={M},K={K},N={N},R={R}]", 2.0 * M * (K * N + R * (K + N))):
             check(fn(x.data_ptr(), w.data_ptr(), _ptr(bias), _ptr(residual), lora_a.data_ptr(), lora_b.data_ptr(), ids.data_ptr(), _ptr(offsets), n, scale,
                      ws.data_ptr(), nb, y.data_ptr(), M, K, N, R, E, keep_u, _stream_of(device)), name)
+        if keep_u and R % 8:                                         # u alone, without the padded adapters behind it
+            ws = ws[:_lib.lib().dm_linear_adapted_workspace_bytes(M, N, (R + 7) // 8 * 8, E)].clone()
     return y, ws
 
 

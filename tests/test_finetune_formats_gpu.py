@@ -152,3 +152,15 @@ def test_controlnet_trainer_takes_channels_last_weights():
         tr.apply_gradients()
         out.append([p.detach().clone() for p in tr._params()])
     assert all(torch.equal(p, q) for p, q in zip(*out))
+
+
+def test_linear_adapted_autograd_keeps_the_low_rank_factor_only():
+    """ranks off 8: the adapters' padded copy is the forward's scratch, not kept until the backward"""
+    from dreammat_amd import _lib
+    from dreammat_amd import hipops
+    s = adapter_inputs(24, BF, (200, 64), 136, 12, 50, [0, 49])
+    y = hipops.linear_adapted_autograd(s["x"], s["w"], s["w"].t().contiguous(), s["bias"], s["a"].requires_grad_(), s["b"], s["ids"])
+    kept = [t.untyped_storage().nbytes() for t in y.grad_fn.saved_tensors if t is not None and t.dtype == torch.uint8]
+    assert kept == [_lib.lib().dm_linear_adapted_workspace_bytes(200, 136, 16, 50)] == [(200 * 72 + 255) // 256 * 256]
+    s = adapter_inputs(24, BF, (200, 64), 136, 12, 50, [0, 49])
+    check_all(s, 0.5)

@@ -213,8 +213,9 @@ __global__ __launch_bounds__(threads_of(L)) void k_gan_fwd(GanArgs a) {
 // Rows as in the forward.  Column sums that run over all rows go to part[slot][b][C], one slot per wanted vector.  The gate's gradient is
 // per item where the gate is: rows of an item may span workgroups and a workgroup may hold several items, so its partial sums are flushed
 // at every item boundary to gate_part[item + b][C] -- along a walk over the rows (item, b) only grows, so item + b names the pair -- behind
-// the other slots.  Bound by HBM, and in 16 bits by the vector pipe (eight entries of six tensors and five sums per chunk): [24, 1024, 1280] fp32
-// 160 us, 4.7 TB/s; [4, 4096, 640] bf16 50 us, 2.5 TB/s.
+// the other slots.  fp32: bound by HBM, [24, 1024, 1280] 160 us, 4.7 TB/s.  16 bits: by the vector pipe (eight entries of six tensors and five
+// sums per chunk), whose instructions take two thirds of the cycles, a third of its lanes without a chunk at these widths (80 chunks on 128
+// lanes): [4, 4096, 640] bf16 50 us, 2.5 TB/s.
 template <typename T, int VEC, int L, int NC>
 __global__ __launch_bounds__(threads_of(L)) void k_gan_bwd(GanArgs a) {
     __shared__ float red[16];
@@ -474,7 +475,8 @@ struct Fwd {
     static int go(GanArgs& a, hipStream_t stream) {
         constexpr int G = threads_of(L) / L;
         // workgroups: rows of a wave two per CU, which loop over rows that are requested ahead ([24, 4096, 320] bf16 44 us against 47 with
-        // eight); rows of a workgroup, whose loads wait for its barriers, eight ([24, 1024, 1280] fp32 93 against 118 us with two)
+        // eight); rows of 256 threads, whose loads wait for their barriers, eight ([24, 1024, 1280] fp32 93 against 118 us with two); rows of
+        // 512 and 1024 threads, which fill a CU with two, two ([12000, 8192] bf16 164 against 181 us with eight, [9000, 5001] 167 against 193)
         const long long most = 256 * (L == 256 ? 8 : 2);
         a.rows_per_block = ((a.rows + most - 1) / most + G - 1) / G * G;
         hipLaunchKernelGGL((k_gan_fwd<T, VEC, L, NC>), dim3((unsigned)((a.rows + a.rows_per_block - 1) / a.rows_per_block)), dim3(threads_of(L)), 0, stream, a);

@@ -12,7 +12,7 @@
 // storage) leave 1e-2 of error in the result and 11 bits (half) 1e-3, 1e-2 where a few directions dominate the matrix.  Numbers are
 // therefore kept as a PAIR of halves, value + rest (22 bits; scaled by 2^13, so that neither leaves half's range: |X| <= 1.2, |S| <=
 // 1.5, |P + a| <= 3.5), and a product is value value + value rest + rest value with fp32 sums: the result agrees with fp32 arithmetic to its
-// own rounding (1.7e-6 against 1.7e-6 of the fp32 form on a 1024^2 Gaussian), and a 16-bit result is off by its one rounding.  Values alone in
+// own rounding (2.1e-6 of error against 3.1e-6 of the fp32 form on a 1024^2 Gaussian), and a 16-bit result is off by its one rounding.  Values alone in
 // the last two iterations would save a seventh of the time (16 x [1280, 1280]: 1859 against 2159 us) and leave 1e-3 of error, as much again as
 // the rounding to bf16 and far more than an fp32 parameter's: not taken for any type.
 // (Taking the polynomials of S = X X^T alone and multiplying X0 once saves half the products of a wide matrix, but S holds squared singular
@@ -237,8 +237,8 @@ __device__ __forceinline__ void tile_of(const Class& c, int rem, int& ti, int& t
 // The epilogue goes through LDS: the tile of S arrives as whole lines (POLY), every lane replaces its own entries, and whole lines leave (GRAM,
 // POLY: in both orientations, the transposed one by the transposing read); a 256 tile does that half by half.  A share of a split
 // contraction leaves its fp32 sums in l.part instead, for k_ns_join.
-// Bound by the matrix pipe, of a 256 tile by the rounds and by the epilogue, which one workgroup per CU does not overlap.  16 x [1280, 1280],
-// 256 tiles, in TF/s of half products: X X^T 116 us = 1040, S S^T 127 us = 950, P X 206 us = 980 (1.56 tiles per CU in two rounds).
+// Bound by feeding the matrix pipe (busy 51 to 57 % of the cycles of a 256 tile), by the rounds and by the epilogue, which one workgroup per CU
+// does not overlap.  16 x [1280, 1280], 256 tiles, in TF/s of half products: X X^T 116 us = 1040, S S^T 127 us = 950, P X 206 us = 980 (1.56 tiles per CU in two rounds).
 // One [320, 320]: 7 to 8 us each, all latency.
 template <int KIND, int T, int NST, typename OT>
 __global__ __launch_bounds__(threads_of(T)) void k_ns_gemm(NsArgs a, Launch l) {

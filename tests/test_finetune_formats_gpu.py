@@ -164,3 +164,30 @@ def test_linear_adapted_autograd_keeps_the_low_rank_factor_only():
     assert kept == [_lib.lib().dm_linear_adapted_workspace_bytes(200, 136, 16, 50)] == [(200 * 72 + 255) // 256 * 256]
     s = adapter_inputs(24, BF, (200, 64), 136, 12, 50, [0, 49])
     check_all(s, 0.5)
+
+
+def test_linear_adapted_half_training_step_captured_and_replayed():
+    """half, a rank off 8 and rows of every scale in a captured graph: replays on new inputs match the eager step bit for bit"""
+    from dreammat_amd import hipops
+    s = adapter_inputs(25, HF, (300, 64), 136, 12, 3, [0, -1, 2], True)
+    wt = s["w"].t().contiguous()
+
+    def step(x, dy):
+        v = [t.detach().requires_grad_() for t in (x, s["a"], s["b"])]
+        y = hipops.linear_adapted_autograd(v[0], s["w"], wt, s["bias"], v[1], v[2], s["ids"], 0.5, s["residual"])
+        return [y.detach(), *torch.autograd.grad(y, v, dy)]
+    x, dy = s["x"].clone(), s["dy"].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x, dy)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(x, dy)
+    for k in range(3):
+        x.copy_(rand(gen(70 + k), 300, 64) * 8.0 ** (torch.arange(300, device=DEV) % 5 - 2.0)[:, None])
+        dy.copy_(rand(gen(80 + k), 300, 136))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, step(x, dy)))

@@ -360,11 +360,11 @@ struct ExpandArgs {
 
 // BM x BN x 64 tile, WM x WN waves, NST LDS stages filled by buffer_load ... lds (16 bytes per lane, range-checked: rows and
 // columns past the end read as zeros).  LDS rows are 128 bytes, the 16-byte chunks XOR-swizzled by (row >> 1) & 7 at the source address
-// and at the fragment read: conflict-free without padding.  The weights are the matrix instruction's A operand, so a lane holds one row
-// of y and four consecutive columns per register group: 16-byte stores after one exchange between the wave's halves.  Bound by feeding the matrix
-// pipe (two workgroups per CU cover each other's waits; it is busy 46 to 49 % of the cycles, LDS without conflicts): bf16, rank 64, [24576, 1280 -> 5120] 435 us = 740 TF/s of the plain product, [24576,
-// 5120 -> 1280] 375 us = 860; [24576, 640 -> 640] rank 16 with residual 37 us, 2.5 TB/s.  With a short K by the latencies of a tile (its
-// adapters, two loads, the store): [24576, 64 -> 4096] rank 16 in 67 us.
+// and at the fragment read: conflict-free without padding.  The weights are the matrix instruction's A operand, so a lane holds one row of y
+// and four consecutive columns per register group: 16-byte stores after one exchange between the wave's halves.  Bound by feeding the matrix
+// pipe (two workgroups per CU cover each other's waits; it is busy 46 to 49 % of the cycles, LDS without conflicts): bf16, rank 64, [24576,
+// 1280 -> 5120] 435 us = 740 TF/s of the plain product, [24576, 5120 -> 1280] 375 us = 860; [24576, 640 -> 640] rank 16 with residual 37 us,
+// 2.5 TB/s.  With a short K by the latencies of a tile (its adapters, two loads, the store): [24576, 64 -> 4096] rank 16 in 67 us.
 template <int BM, int BN, int WM, int WN, int NST>
 __global__ __launch_bounds__(WM * WN * 64) void k_expand(ExpandArgs a) {
     [[maybe_unused]] constexpr int NW = WM * WN, ROWB = 128;
